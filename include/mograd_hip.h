@@ -541,6 +541,64 @@ int mg_flash_attn_bwd_packed(const void* d_o, const void* o, const void* qkv, co
                              int64_t D, float scale, int causal, int has_bias, int dtype,
                              mg_stream stream);
 
+/* ------------------------------------------------------------------------------------ */
+/* The residual path between two blocks, and activations kept in 8 bits.  No counterpart  */
+/* in the reference, whose blocks add their output to the stream as it is                 */
+/* (examples/tinyshakespear/model.mojo:62-64,120-121).                                    */
+/* ------------------------------------------------------------------------------------ */
+
+/* Activations in 8 bits ("act8"): what a forward pass keeps for the backward, in about half the bytes of a 16-bit tensor.  32
+ * consecutive columns of a row (the last ones of a row may be fewer) share a power of two 2^k, the least one for which
+ * rint(max|x| / 2^k) <= 127; a value is kept as q = rint(x / 2^k) (to even), and stands for q 2^k, a number that bf16, fp32
+ * and, for fp16 tensors, fp16 hold as it is.  k is kept within -126 .. 121 (fp16: -24 .. 9, so that fp16 values past 65024
+ * become 65024).  A block that holds an infinity or a NaN is restored as NaNs.
+ * One run of mg_act8_bytes(rows, cols) bytes, starting on a 16-byte boundary, holds them: rows x ld signed bytes q, ld being
+ * cols rounded up to 32 (zeros past cols), then rows x ld / 32 bytes k + 133 (255: not finite).
+ * dtype: F32, F16, BF16 of contiguous (rows, cols) tensors at any address of their elements. */
+int64_t mg_act8_bytes(int64_t rows, int64_t cols); /* 0 where there is nothing to hold, or too much */
+/* keep_sign != 0: a value that is not zero is kept as at least one step of its sign, so that the mask x > 0 of a ReLU's output
+ * can be taken from q (see mg_linear_bwd_act8). */
+int mg_act8_store(const void* x, void* act8, int64_t rows, int64_t cols, int keep_sign, int dtype, mg_stream stream);
+int mg_act8_load(const void* act8, void* x, int64_t rows, int64_t cols, int dtype, mg_stream stream);
+
+/* mg_linear_bwd_fused for an input X (M,K) that is kept in 8 bits: with X' the values that x8 stands for,
+ *   dx(M,K) = dY W     (NULL to skip; x_is_relu_output != 0: where X' > 0, else 0; dx_accumulate != 0: added to dx)
+ *   dw(N,K) = dY^T X'
+ *   db(N)   = column sums of dY (NULL to skip).
+ * `x8` was stored from a tensor of `dtype`.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the unrounded fp32 sums.
+ * M == 0: dw and db are zeros. */
+int mg_linear_bwd_act8(const void* dy, const void* x8, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t N,
+                       int64_t K, int dx_accumulate, int x_is_relu_output, int dtype, int grad_dtype, mg_stream stream);
+
+/* From a block's output f (rows, cols) and the residual stream h (rows, cols) to the stream h_out and the next block's input x:
+ *   z     = LayerNorm(f; post_gamma, post_beta)     the norm after a block (without one, z = f: post_* all NULL)
+ *   h_out = residual_scale h + gate z               gate (rows / gate_rows, cols): each row of it serves gate_rows consecutive
+ *                                                   rows (gate_rows == rows: a number a channel; a sequence's length: a vector
+ *                                                   a sequence); NULL: 1, and gate_rows is not looked at
+ *   x     = LayerNorm(h_out; pre_gamma, pre_beta)   the norm before the next block (without one, pre_* and x all NULL)
+ * in fp32, each output rounded once (x is the norm of h_out before its rounding).  The statistics (rows each, fp32) are for the
+ * backward.  f8, x8 (each may be NULL): f and x as mg_act8_store(keep_sign = 0) would keep them, written by the same launch.
+ * h_out may be h; nothing else overlaps.  gamma, beta and gate are of `dtype`. */
+int mg_residual_norm_fwd(const void* f, const void* h, const void* gate, const void* post_gamma, const void* post_beta,
+                         const void* pre_gamma, const void* pre_beta, void* h_out, void* x, float* post_mean, float* post_rstd,
+                         float* pre_mean, float* pre_rstd, void* f8, void* x8, int64_t rows, int64_t cols, int64_t gate_rows,
+                         float residual_scale, float eps, int dtype, mg_stream stream);
+
+/* Its gradients.  dx is the gradient of x (NULL, like pre_* and dpre_*, without a pre norm), dh_out what reaches h_out by other
+ * ways (NULL for none, where there is a dx); f as it was, or f8 as it is kept in 8 bits, the other NULL; h_out as stored.
+ *   df, dh (rows, cols); dgate like gate; dpost_gamma, dpost_beta, dpre_gamma, dpre_beta (cols)
+ * The parameters' gradients are of `grad_dtype`: `dtype`, or MG_F32 for the unrounded fp32 sums; they are fully overwritten, and
+ * summed in a fixed order without atomics.  dh may be dh_out; nothing else overlaps.  rows == 0: the sums over no rows are zeros
+ * (dgate: `cols` of them if gate_rows is 0 too, the gate that all rows share; otherwise there is no row of it). */
+int mg_residual_norm_bwd(const void* dx, const void* dh_out, const void* f, const void* f8, const void* h_out, const void* gate,
+                         const void* post_gamma, const void* post_beta, const void* pre_gamma, const float* post_mean,
+                         const float* post_rstd, const float* pre_mean, const float* pre_rstd, void* df, void* dh, void* dgate,
+                         void* dpost_gamma, void* dpost_beta, void* dpre_gamma, void* dpre_beta, int64_t rows, int64_t cols,
+                         int64_t gate_rows, float residual_scale, int dtype, int grad_dtype, mg_stream stream);
+
+/* mg_linear_bwd_act8 and mg_residual_norm_bwd take scratch from the pool.  Recorded into a HIP graph they keep it: what such a
+ * call took is in no later call's hands for as long as the process runs, so graphs and eager calls never share it. */
+
 #ifdef __cplusplus
 }
 #endif

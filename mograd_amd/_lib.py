@@ -132,6 +132,12 @@ PROTOTYPES = {
     "mg_flash_attn_fwd_bshd": (_i, [_p, _p, _p, _p, _p, _p, _l, _l, _l, _l, _f, _i, _i, _i, _p], True),
     "mg_flash_attn_bwd_bshd": (_i, [_p] * 10 + [_l, _l, _l, _l, _f, _i, _i, _i, _p], True),
     "mg_flash_attn_fwd_packed": (_i, [_p, _p, _p, _p, _l, _l, _l, _l, _f, _i, _i, _i, _p], True),
+    "mg_act8_bytes": (_l, [_l, _l], False),
+    "mg_act8_store": (_i, [_p, _p, _l, _l, _i, _i, _p], True),
+    "mg_act8_load": (_i, [_p, _p, _l, _l, _i, _p], True),
+    "mg_linear_bwd_act8": (_i, [_p] * 6 + [_l, _l, _l, _i, _i, _i, _i, _p], True),
+    "mg_residual_norm_fwd": (_i, [_p] * 15 + [_l, _l, _l, _f, _f, _i, _p], True),
+    "mg_residual_norm_bwd": (_i, [_p] * 20 + [_l, _l, _l, _f, _i, _i, _p], True),
     "mg_flash_attn_bwd_packed": (_i, [_p] * 6 + [_l, _l, _l, _l, _f, _i, _i, _i, _p], True),
 }
 

@@ -60,6 +60,21 @@ class Scratch {
   void* ptr_ = nullptr;
 };
 
+// For the length of an entry point's call on a stream that is being captured into a graph: what the call takes from the pool is
+// never handed to another call, since every replay of the graph writes it again, and the pool may ask the driver for memory in
+// the midst of the capture.  (No effect on other streams.)
+class CaptureHold {
+ public:
+  explicit CaptureHold(hipStream_t stream);
+  ~CaptureHold();
+  CaptureHold(const CaptureHold&) = delete;
+  CaptureHold& operator=(const CaptureHold&) = delete;
+
+ private:
+  bool on_ = false;
+  hipStreamCaptureMode mode_ = hipStreamCaptureModeRelaxed;
+};
+
 // A view of up to kMaxRank dimensions: extents and element strides, passed to kernels by
 // value.
 constexpr int kMaxRank = 8;

@@ -1,0 +1,3 @@
+#include "residual_norm_impl.h"
+
+MG_DEFINE_RESIDUAL_NORM(bf16_t)

@@ -157,6 +157,27 @@ static std::string summary_locked(Pool& pool) {
   return out;
 }
 
+// Set while a CaptureHold of this thread is in force: what is released stays taken.
+static thread_local bool t_hold_released = false;
+
+CaptureHold::CaptureHold(hipStream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (stream == nullptr || t_hold_released) return;  // (the default stream cannot be captured)
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return;
+  }
+  if (status != hipStreamCaptureStatusActive) return;
+  on_ = hipThreadExchangeStreamCaptureMode(&mode_) == hipSuccess;
+  t_hold_released = on_;
+}
+
+CaptureHold::~CaptureHold() {
+  if (!on_) return;
+  t_hold_released = false;
+  (void)hipThreadExchangeStreamCaptureMode(&mode_);
+}
+
 int pool_take(void** out, int64_t nbytes) {
   if (!out) return fail(MG_ERR_INVALID, "pool_alloc: null output pointer");
   if (nbytes < 0) return fail(MG_ERR_INVALID, "pool_alloc: negative size %lld", static_cast<long long>(nbytes));
@@ -210,7 +231,7 @@ int pool_take(void** out, int64_t nbytes) {
 }
 
 int pool_release(void* ptr) {
-  if (!ptr) return MG_OK;
+  if (!ptr || t_hold_released) return MG_OK;
   std::lock_guard<std::mutex> lock(g_pool_mu);
   Pool& pool = current_pool();
   auto it = pool.live.find(ptr);

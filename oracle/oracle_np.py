@@ -27,8 +27,10 @@ Pinning (what makes each function trustworthy without running the reference):
   adam_step / sgd_step  torch.optim.Adam / AdamW / SGD over several steps (f64)
   softmax / softmax_grad torch.softmax and its autograd (f64), rows sum to 1 / to 0
   argmax_axis           numpy.argmax on NaN-free input (first occurrence), hand cases
+  act8_*                by definition over all steps k (tests/test_act8.py), integers that are their own 8 bits
+  residual_norm_*       layer_norm_* above, torch autograd (f64), central differences (tests/test_residual_norm.py)
   round_class           tests/test_memory.mojo:18-30 (1000 -> 1024, 1025 -> 1152)
-All of the above are exercised in tests/test_oracle.py.
+All of the above are exercised in tests/test_oracle.py, where no other file is named.
 """
 from __future__ import annotations
 
@@ -525,6 +527,108 @@ def adam_step(w, g, m, v, lr, beta1, beta2, eps, weight_decay, t, decoupled):
 def sgd_step(w, g, lr):
     """w - g * lr.  mograd/nn/optim/sgd.mojo:33-36."""
     return np.asarray(w, dtype=F64) - np.asarray(g, dtype=F64) * lr
+
+
+# --------------------------------------------------------------------------- #
+# Activations in 8 bits (include/mograd_hip.h; no counterpart in the reference)
+# --------------------------------------------------------------------------- #
+
+ACT8_BLOCK = 32
+ACT8_RANGE = {"f32": (-126, 121), "bf16": (-126, 121), "f16": (-24, 9)}
+
+
+def act8_store(x, kind, keep_sign=False):
+    """x (rows, cols), float64 values of the type `kind` -> the bytes (uint8) that hold it in 8 bits."""
+    x = np.asarray(x, dtype=F64)
+    rows, cols = x.shape
+    blocks = -(-cols // ACT8_BLOCK)
+    v = np.zeros((rows, blocks * ACT8_BLOCK))
+    v[:, :cols] = x
+    v = v.reshape(rows, blocks, ACT8_BLOCK)
+    bad = ~np.isfinite(v).all(axis=2)
+    v = np.where(bad[:, :, None], 0.0, v)
+    part, power = np.frexp(np.abs(v).max(axis=2))  # max = part 2^power, 0.5 <= part < 1
+    lo, hi = ACT8_RANGE[kind]
+    k = np.clip(np.where(part > 0, power - 7 + (part * 128 >= 127.5), lo), lo, hi).astype(np.int64)
+    q = np.clip(np.rint(np.ldexp(v, -k[:, :, None])), -127, 127)
+    if keep_sign:
+        q = np.where(q == 0, np.sign(v), q)
+    k = np.where(bad, 255 - 133, k)
+    return np.concatenate([q.astype(np.int8).reshape(-1).view(np.uint8), (k + 133).astype(np.uint8).reshape(-1)])
+
+
+def act8_load(act8, rows, cols):
+    """The values (rows, cols) that the bytes stand for."""
+    blocks = -(-cols // ACT8_BLOCK)
+    act8 = np.asarray(act8, dtype=np.uint8)
+    q = act8[:rows * blocks * ACT8_BLOCK].view(np.int8).reshape(rows, blocks, ACT8_BLOCK).astype(F64)
+    e = act8[rows * blocks * ACT8_BLOCK:].reshape(rows, blocks, 1).astype(np.int64)
+    return np.where(e == 255, np.nan, np.ldexp(q, e - 133)).reshape(rows, -1)[:, :cols]
+
+
+# --------------------------------------------------------------------------- #
+# The residual path between two blocks (include/mograd_hip.h; no counterpart in the reference)
+# --------------------------------------------------------------------------- #
+
+
+def _norm_stats(x, eps):
+    mean = x.mean(axis=1)
+    return mean, 1.0 / np.sqrt(((x - mean[:, None]) ** 2).mean(axis=1) + eps)
+
+
+def residual_norm_fwd(f, h, gate=None, post=None, pre=None, scale=1.0, eps=1e-5):
+    """f, h (rows, cols); gate (G, cols) for rows / G rows each; post, pre: (gamma, beta).
+    -> {"h_out", "x", "post_mean", "post_rstd", "pre_mean", "pre_rstd"}, None without the norm."""
+    f, h = np.asarray(f, F64), np.asarray(h, F64)
+    out = {}
+    for name, norm in (("post", post), ("pre", pre)):
+        v = f if name == "post" else out["h_out"]
+        out[name + "_mean"] = out[name + "_rstd"] = None
+        if norm is not None:
+            mean, rstd = out[name + "_mean"], out[name + "_rstd"] = _norm_stats(v, eps)
+            v = (v - mean[:, None]) * rstd[:, None] * np.asarray(norm[0], F64) + np.asarray(norm[1], F64)
+        if name == "post":
+            if gate is not None:
+                v = v * np.repeat(np.asarray(gate, F64), v.shape[0] // len(gate), axis=0)
+            out["h_out"] = scale * h + v
+    out["x"] = v if pre is not None else None
+    return out
+
+
+def residual_norm_bwd(dx, dh_out, f, h_out, gate=None, post=None, pre=None, scale=1.0):
+    """post, pre: (gamma, beta, mean, rstd) with the saved statistics; dx None without a pre norm, dh_out None for zeros.
+    -> {"df", "dh", "dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta"}."""
+    f = np.asarray(f, F64)
+    rows, cols = f.shape
+    out = dict.fromkeys(("dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta"))
+
+    def norm_grad(dy, hat, rstd):
+        c1, c2 = dy.mean(axis=1, keepdims=True), (dy * hat).mean(axis=1, keepdims=True)
+        return rstd * (dy - c1 - hat * c2)
+
+    d = np.zeros_like(f) if dh_out is None else np.asarray(dh_out, F64)
+    if pre is not None:
+        gamma, _, mean, rstd = (np.asarray(a, F64) for a in pre)
+        dx = np.asarray(dx, F64)
+        hat = (np.asarray(h_out, F64) - mean[:, None]) * rstd[:, None]
+        d = d + norm_grad(dx * gamma, hat, rstd[:, None])
+        out["dpre_gamma"], out["dpre_beta"] = (dx * hat).sum(axis=0), dx.sum(axis=0)
+    out["dh"] = scale * d
+    hat = z = f
+    if post is not None:
+        gamma, beta, mean, rstd = (np.asarray(a, F64) for a in post)
+        hat = (f - mean[:, None]) * rstd[:, None]
+        z = hat * gamma + beta
+    u = d
+    if gate is not None:
+        gate = np.asarray(gate, F64)
+        out["dgate"] = (d * z).reshape(len(gate), -1, cols).sum(axis=1)
+        u = d * np.repeat(gate, rows // len(gate), axis=0)
+    if post is not None:
+        out["dpost_gamma"], out["dpost_beta"] = (u * hat).sum(axis=0), u.sum(axis=0)
+        u = norm_grad(u * gamma, hat, rstd[:, None])
+    out["df"] = u
+    return out
 
 
 # --------------------------------------------------------------------------- #
