@@ -212,6 +212,13 @@ __device__ __forceinline__ void row_allreduce_sum(float (&v)[K], float* slots, i
     // four rows side by side in a wave, each on one row of 16 lanes
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = row16_allreduce<SumOp>(v[k]);
+  } else if constexpr (TPR == 32) {
+    // two rows side by side in a wave
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = row16_allreduce<SumOp>(v[k]);
+      v[k] += __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v[k]), kSwizzleXor16));
+    }
   } else if constexpr (TPR == kWave) {
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);

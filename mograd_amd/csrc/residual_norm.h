@@ -32,14 +32,14 @@ struct ResidualNormBwd {
   int cols;
   uint32_t gate_rows;
   float scale;
-  // Workgroup g has piece g % pieces of gate row g / pieces (pieces > 1), or gate rows g * gates_per_group and on, whole.
+  // Workgroup (x, y) has piece x of the gate rows y gates_per_group and on: one gate row in several pieces, or several whole.
   // A piece's rows start piece * piece_start into the gate row's, are row_step apart for each of the rows in flight, and end
   // piece_span on or with the gate row.
   int64_t gates, gates_per_group, piece_start, piece_span, row_step;
   uint32_t pieces;
-  // Column sums of the workgroups, [5][groups][cols]: dpost_gamma, dpost_beta, dpre_gamma, dpre_beta, dgate (of a piece).
-  float* part;
-  int64_t part_stride;
+  // Column sums.  gate_sums [2][gates * pieces][cols]: of d and d fh over each piece of a gate row's rows; pre_sums
+  // [2][workgroups][cols]: of dx xh and dx.  Null where nobody asks.
+  float *gate_sums, *pre_sums;
   float* row_sums;  // (rows, 2), the kernels of wide rows: the two means of the pre norm's gradient
 };
 
@@ -63,10 +63,14 @@ struct ResidualNormRow {
   }
 };
 
+template <typename T>
 struct ResidualNormFinish {
-  const float* part;
-  void* out[5];
-  int64_t part_stride, cols, groups, pieces;
+  const float *gate_sums, *pre_sums;
+  const T *gate, *post_gamma, *post_beta;
+  void *dgate, *dpost_gamma, *dpost_beta, *dpre_gamma, *dpre_beta;
+  int64_t cols, groups, gates, pieces;
+  int split;  // lanes to a gate row: a power of two, 1 .. 32
+  int first;  // the first workgroups' job: 0 the gate and the post norm, 1 the pre norm
   int grad_f32;
 };
 

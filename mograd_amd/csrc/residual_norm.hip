@@ -76,7 +76,8 @@ int mg_residual_norm_bwd(const void* dx, const void* dh_out, const void* f, cons
                     mg::dtype_name(grad_dtype));
   if ((gate != nullptr) != (dgate != nullptr)) return mg::fail(MG_ERR_INVALID, "%s: gate and dgate come together", who);
   hipStream_t s = mg::to_stream(stream);
-  if (rows == 0) {  // the column sums of empty matrices are zero (an empty batch has no gate rows of its own, but one of all rows)
+  // The column sums of empty matrices are zero.  (An empty batch has no gate rows of its own, but may have the one of all rows.)
+  if (rows == 0) {
     MG_TRY(mg::norm_pointers(who, "post", {post_gamma, post_beta, dpost_gamma, dpost_beta}));
     MG_TRY(mg::norm_pointers(who, "pre", {pre_gamma, dpre_gamma, dpre_beta}));
     for (void* out : {dgate && gate_rows == 0 ? dgate : nullptr, dpost_gamma, dpost_beta, dpre_gamma, dpre_beta})

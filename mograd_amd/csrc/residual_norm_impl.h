@@ -53,7 +53,33 @@ struct RawRow {
       }
     }
   }
+  // Keeps the compiler from carrying unpacked values into what comes after, or out of the loop: twice the registers.
+  __device__ __forceinline__ void keep_packed() {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(w[i][j]));
+  }
+  __device__ __forceinline__ void zeros() {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i][j] = 0;
+  }
+  __device__ __forceinline__ void ones() {
+    float v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 1.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) VecAny<T, VEC>::pack(v, w[i]);
+  }
   __device__ __forceinline__ void values(int i, float (&v)[VEC]) const { VecAny<T, VEC>::unpack(w[i], v); }
+  // The values times `scale`, plus `shift`.
+  __device__ __forceinline__ void normalised(int i, float scale, float shift, float (&v)[VEC]) const {
+    values(i, v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = fmaf(v[e], scale, shift);
+  }
   // Whether element e of chunk i is one of the row's.
   static __device__ __forceinline__ bool in_row(int i, int e, int t, int cols) { return Tile::in_row(col(i, t), e, cols); }
   static __device__ __forceinline__ void store(T* row, int i, int t, int cols, const float (&v)[VEC]) {
@@ -101,15 +127,19 @@ struct Act8Row {
       }
     }
   }
-  __device__ __forceinline__ void values(int i, float (&v)[VEC]) const {
-    const float scale = act8_scale(e[i]);
+  __device__ __forceinline__ void keep_packed() {
 #pragma unroll
-    for (int j = 0; j < VEC / 4; ++j) {
-      float x[4];
-      act8_unpack4(q[i][j], scale, x);
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[4 * j + k] = x[k];
-    }
+      for (int j = 0; j < VEC / 4; ++j) asm volatile("" : "+v"(q[i][j]));
+  }
+  // The values times `scale`, plus `shift`.
+  __device__ __forceinline__ void normalised(int i, float scale, float shift, float (&v)[VEC]) const {
+    const float step = act8_scale(e[i]) * scale;
+#pragma unroll
+    for (int j = 0; j < VEC / 4; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * j + k] = fmaf(static_cast<float>(static_cast<int8_t>(q[i][j] >> 8 * k)), step, shift);
   }
 };
 
@@ -136,11 +166,19 @@ __device__ __forceinline__ void act8_store_chunk(uint8_t* q_row, uint8_t* e_row,
   if (t % LANES == 0) e_row[c / kAct8Block] = static_cast<uint8_t>(ex);
 }
 
+// row_thread, with a slot that the compiler knows to be the same for a whole wave: addresses and the row's statistics stay in
+// scalar registers (the backward of (16384, 384) bf16 spent a tenth of its vector instructions on 64-bit addresses).
+template <int TPR, int WG>
+__device__ __forceinline__ void wave_row_thread(int& t, int& sub) {
+  row_thread<TPR, WG>(t, sub);
+  if constexpr (TPR == kWave) sub = __builtin_amdgcn_readfirstlane(sub);
+}
+
 // Mean and rstd of a row: the mean first, then the squares about it (the row is in registers, and a first element far from
 // the others would cost the one-pass sums their digits).  `v` is zero past the row.
 template <typename Row, int TPR, int VPT, int WG>
-__device__ __forceinline__ void row_moments(const float (&v)[VPT][Row::VEC], int t, int cols, float inv_n, float eps, float* slots,
-                                            int& phase, float& mean, float& rstd) {
+__device__ __forceinline__ void row_moments(const float (&v)[VPT][Row::VEC], int t, int cols, float inv_n, float eps,
+                                            float* slots, int& phase, float& mean, float& rstd) {
   float s[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
@@ -151,95 +189,89 @@ __device__ __forceinline__ void row_moments(const float (&v)[VPT][Row::VEC], int
   s[0] = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i)
+    if (Row::col(i, t) < cols) {
 #pragma unroll
-    for (int e = 0; e < Row::VEC; ++e) {
-      const float d = Row::in_row(i, e, t, cols) ? v[i][e] - mean : 0.f;
-      s[0] += d * d;
+      for (int e = 0; e < Row::VEC; ++e) {
+        const float d = Row::in_row(i, e, t, cols) ? v[i][e] - mean : 0.f;
+        s[0] = fmaf(d, d, s[0]);
+      }
     }
   row_allreduce_sum<TPR, WG, 1>(s, slots, phase);
   rstd = rsqrtf(s[0] * inv_n + eps);
 }
 
-template <typename T, int TPR, int VPT, int WG, bool ANY>
+// Which norms there are, and whether f or x is kept in 8 bits, is known to the compiler: as branches in the kernel they cost
+// small calls most, which wait for every line of code that a row passes through.
+template <typename T, int TPR, int VPT, int WG, bool ANY, bool POST, bool PRE, bool KEEP>
 __global__ __launch_bounds__(WG) void residual_norm_fwd_kernel(const ResidualNormFwd<T> a) {
   using Row = RawRow<T, TPR, VPT, ANY>;
   constexpr int VEC = Row::VEC, RPW = WG / TPR;
   static_assert(TPR <= kWave || RPW == 1, "rows of several waves have a workgroup each");
   __shared__ float slots[2 * (WG / kWave)];
   int t, sub;
-  row_thread<TPR, WG>(t, sub);
+  wave_row_thread<TPR, WG>(t, sub);
   int phase = 0;
   const int cols = a.cols;
   const float inv_n = 1.0f / static_cast<float>(cols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * RPW;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * RPW + sub;
+  if (row >= a.rows) return;  // (the whole workgroup, where its waves share a row)
 
-  Row post_gamma, post_beta, pre_gamma, pre_beta, gate;
-  if (a.post_gamma) {
+  Row f, h, f_next, h_next, post_gamma, post_beta, pre_gamma, pre_beta, gate;
+  f.load(a.f + row * cols, t, cols);
+  h.load(a.h + row * cols, t, cols);
+  uint32_t gate_at = static_cast<uint32_t>(row) / a.gate_rows;
+  if (a.gate) gate.load(a.gate + static_cast<int64_t>(gate_at) * cols, t, cols);
+  else gate.ones();
+  if constexpr (POST) {
     post_gamma.load(a.post_gamma, t, cols);
     post_beta.load(a.post_beta, t, cols);
   }
-  if (a.pre_gamma) {
+  if constexpr (PRE) {
     pre_gamma.load(a.pre_gamma, t, cols);
     pre_beta.load(a.pre_beta, t, cols);
   }
-  uint32_t gate_at = 0xffffffffu;
-
-  const int64_t step = static_cast<int64_t>(gridDim.x) * RPW;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * RPW + sub;
-  Row f, h, f_next, h_next;
-  if (row < a.rows) {
-    f.load(a.f + row * cols, t, cols);
-    h.load(a.h + row * cols, t, cols);
-  }
-  for (; row < a.rows; row += step) {  // uniform per row of 16 lanes (TPR == 16), per wave (64) or per workgroup
+  while (true) {  // uniform per row of 16 lanes (TPR == 16), per wave (64) or per workgroup
     const int64_t next = row + step;
     if (next < a.rows) {
       f_next.load(a.f + next * cols, t, cols);
       h_next.load(a.h + next * cols, t, cols);
     }
-    if (a.gate) {
-      const uint32_t at = static_cast<uint32_t>(row) / a.gate_rows;
-      if (at != gate_at) gate.load(a.gate + static_cast<int64_t>(at) * cols, t, cols);
-      gate_at = at;
-    }
     float v[VPT][VEC];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) f.values(i, v[i]);
-    if (a.f8) {
-      uint8_t* const e_row = a.f8 + a.rows * a.ld + row * (a.ld / kAct8Block);
+    if constexpr (KEEP) {
+      if (a.f8) {
+        uint8_t* const e_row = a.f8 + a.rows * a.ld + row * (a.ld / kAct8Block);
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) act8_store_chunk<T, TPR>(a.f8 + row * a.ld, e_row, i, t, cols, v[i]);
+        for (int i = 0; i < VPT; ++i) act8_store_chunk<T, TPR>(a.f8 + row * a.ld, e_row, i, t, cols, v[i]);
+      }
     }
     float mean, rstd;
-    if (a.post_gamma) {
+    if constexpr (POST) {
       row_moments<Row, TPR, VPT, WG>(v, t, cols, inv_n, a.eps, slots, phase, mean, rstd);
       if (t == 0) {
         a.post_mean[row] = mean;
         a.post_rstd[row] = rstd;
       }
+    }
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < VPT; ++i) {
+      float hv[VEC], gt[VEC];
+      if constexpr (POST) {
         float g[VEC], b[VEC];
         post_gamma.values(i, g);
         post_beta.values(i, b);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] = (v[i][e] - mean) * rstd * g[e] + b[e];  // (zero past the row: g and b are)
+        for (int e = 0; e < VEC; ++e) v[i][e] = fmaf((v[i][e] - mean) * rstd, g[e], b[e]);  // (zero past the row: g and b are)
       }
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      float hv[VEC];
       h.values(i, hv);
-      if (a.gate) {
-        float g[VEC];
-        gate.values(i, g);
+      gate.values(i, gt);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] *= g[e];
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i][e] = fmaf(a.scale, hv[e], v[i][e]);
+      for (int e = 0; e < VEC; ++e) v[i][e] = fmaf(a.scale, hv[e], v[i][e] * gt[e]);
       Row::store(a.h_out + row * cols, i, t, cols, v[i]);
     }
-    if (a.pre_gamma) {
+    if constexpr (PRE) {
       row_moments<Row, TPR, VPT, WG>(v, t, cols, inv_n, a.eps, slots, phase, mean, rstd);
       if (t == 0) {
         a.pre_mean[row] = mean;
@@ -251,17 +283,24 @@ __global__ __launch_bounds__(WG) void residual_norm_fwd_kernel(const ResidualNor
         pre_gamma.values(i, g);
         pre_beta.values(i, b);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i][e] = (v[i][e] - mean) * rstd * g[e] + b[e];
+        for (int e = 0; e < VEC; ++e) v[i][e] = fmaf((v[i][e] - mean) * rstd, g[e], b[e]);
         Row::store(a.x + row * cols, i, t, cols, v[i]);
-        if (a.x8) {  // of x as it is stored
+        if constexpr (KEEP) {
+          if (a.x8) {  // of x as it is stored
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[i][e] = to_float(from_float<T>(v[i][e]));
-          act8_store_chunk<T, TPR>(a.x8 + row * a.ld, a.x8 + a.rows * a.ld + row * (a.ld / kAct8Block), i, t, cols, v[i]);
+            for (int e = 0; e < VEC; ++e) v[i][e] = to_float(from_float<T>(v[i][e]));
+            act8_store_chunk<T, TPR>(a.x8 + row * a.ld, a.x8 + a.rows * a.ld + row * (a.ld / kAct8Block), i, t, cols, v[i]);
+          }
         }
       }
     }
+    if (next >= a.rows) return;
+    row = next;
     f = f_next;
     h = h_next;
+    const uint32_t at = static_cast<uint32_t>(row) / a.gate_rows;
+    if (a.gate && at != gate_at) gate.load(a.gate + static_cast<int64_t>(at) * cols, t, cols);
+    gate_at = at;
   }
 }
 
@@ -322,213 +361,251 @@ __global__ __launch_bounds__(WG) void residual_norm_fwd_wide_kernel(const Residu
 
 // ------------------------------------------------------------------------------------
 // Backward, stage 1: df, dh, and column sums of the workgroup's rows.  A workgroup has either one piece of the rows of one
-// gate row, or several gate rows whole (the partition is the host's, ResidualNormBwd): the sums A and B are written out, as
-// gradients of the gate and of the post norm's parameters, where the gate row changes.  No atomics, fixed orders.
+// gate row, or several gate rows whole (the partition is the host's, ResidualNormBwd); the sums A and B go out where the gate
+// row changes.  No atomics, fixed orders.
 // ------------------------------------------------------------------------------------
 
-template <typename T, int TPR, int VPT, int WG, bool ANY, bool F8>
+template <typename T, int TPR, int VPT, int WG, bool ANY, bool F8, bool POST, bool PRE>
 __global__ __launch_bounds__(WG) void residual_norm_bwd_kernel(const ResidualNormBwd<T> a) {
   using Row = RawRow<T, TPR, VPT, ANY>;
+  using FRow = std::conditional_t<F8, Act8Row<T, TPR, VPT>, Row>;
   constexpr int VEC = Row::VEC, RPW = WG / TPR, NW = WG / kWave;
   constexpr int TILE_COLS = VPT * TPR * VEC;
   constexpr int SETS = TPR < kWave ? NW : RPW;  // column sums to add in the workgroup: one set a wave, or one a row
+  // (1024 threads have 128 registers each, and rows off the chunks take more: (2587, 1001) fp16 with | without 24.1 | 20.5 us)
+  constexpr bool PREFETCH = WG < 1024 && VPT * VEC <= (ANY ? 8 : 16);
   static_assert(TPR <= kWave || RPW == 1, "rows of several waves have a workgroup each");
   __shared__ float slots[2 * 2 * NW];
-  __shared__ float combine[RPW > 1 ? SETS * TILE_COLS : 1];
+  __shared__ __attribute__((aligned(16))) float combine[RPW > 1 ? 2 * SETS * TILE_COLS : 4];
   int t, sub;
-  row_thread<TPR, WG>(t, sub);
+  wave_row_thread<TPR, WG>(t, sub);
   int phase = 0;
   const int cols = a.cols;
   const float inv_n = 1.0f / static_cast<float>(cols);
-  const bool post = a.post_gamma != nullptr, pre = a.pre_gamma != nullptr;
 
-  Row post_gamma, pre_gamma, gate;
-  if (post) post_gamma.load(a.post_gamma, t, cols);
-  if (pre) pre_gamma.load(a.pre_gamma, t, cols);
-  float sum_d[VPT][VEC], sum_df[VPT][VEC], sum_g[VPT][VEC], sum_b[VPT][VEC];
-  auto clear = [](float (&s)[VPT][VEC]) {
+  float sums[4][VPT][VEC];  // of d, d fh (over the rows of a gate row), dx xh, dx
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s[i][e] = 0.f;
-  };
-  clear(sum_g);
-  clear(sum_b);
-
-  // One column's sums over the present gate row's rows, out to memory.
-  float* const part = a.part + static_cast<int64_t>(blockIdx.x) * cols;
-  const int64_t set = a.part_stride;
-  auto emit = [&](int c, float d, float df, int64_t gate_row, bool first) {
-    if (post) {
-      const float g = a.gate ? to_float(a.gate[gate_row * cols + c]) : 1.f;
-      const float pg = g * df, pb = g * d;
-      part[0 * set + c] = first ? pg : part[0 * set + c] + pg;
-      part[1 * set + c] = first ? pb : part[1 * set + c] + pb;
-      df = to_float(a.post_gamma[c]) * df + to_float(a.post_beta[c]) * d;
-    }
-    if (!a.gate) return;
-    if (a.pieces > 1) part[4 * set + c] = df;
-    else if (a.grad_f32) static_cast<float*>(a.dgate)[gate_row * cols + c] = df;
-    else static_cast<T*>(a.dgate)[gate_row * cols + c] = from_float<T>(df);
-  };
-  // The workgroup's column sums of two tiles of its threads, handed column by column to `out`.
-  auto columns = [&](float (&s0)[VPT][VEC], float (&s1)[VPT][VEC], auto&& out) {
+      for (int e = 0; e < VEC; ++e) sums[k][i][e] = 0.f;
+  // Sums k and k + 1 over the workgroup's rows to `out` and, `set` floats on, to the second one's place; back to zero.
+  auto flush = [&](int k, float* out, int64_t set) {
     if constexpr (RPW == 1) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = Row::col(i, t);
+        if (c >= cols) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float* const to = out + j * set + c;
+          if (!ANY) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+              const mg_f4 v = {sums[k + j][i][e], sums[k + j][i][e + 1], sums[k + j][i][e + 2], sums[k + j][i][e + 3]};
+              *reinterpret_cast<mg_f4*>(to + e) = v;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+              if (c + e < cols) to[e] = sums[k + j][i][e];
+          }
+        }
+      }
+    } else {
+      // The rows of the workgroup hold sums for the same columns: added through LDS, after those that share a wave.
+      const int mine = TPR < kWave ? static_cast<int>(threadIdx.x / kWave) : sub;
+      __syncthreads();  // (the sums before these have been read)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          if constexpr (TPR < kWave) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+#pragma unroll
+              for (int w = TPR; w < kWave; w *= 2) sums[k + j][i][e] += __shfl_xor(sums[k + j][i][e], w);
+          }
+          if (TPR >= kWave || threadIdx.x % kWave < TPR) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+              const mg_f4 v = {sums[k + j][i][e], sums[k + j][i][e + 1], sums[k + j][i][e + 2], sums[k + j][i][e + 3]};
+              *reinterpret_cast<mg_f4*>(combine + (j * SETS + mine) * TILE_COLS + Row::col(i, t) + e) = v;
+            }
+          }
+        }
+      __syncthreads();
+      for (int c = threadIdx.x; c < cols; c += WG) {
+        float v0 = combine[c], v1 = combine[SETS * TILE_COLS + c];
+#pragma unroll
+        for (int r = 1; r < SETS; ++r) {
+          v0 += combine[r * TILE_COLS + c];
+          v1 += combine[(SETS + r) * TILE_COLS + c];
+        }
+        out[c] = v0;
+        out[set + c] = v1;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int c = Row::col(i, t) + e;
-          if (c < cols) out(c, s0[i][e], s1[i][e]);
-        }
-    } else {
-      constexpr int PER = (TILE_COLS + WG - 1) / WG;
-      float total[2][PER];
-      const int mine = TPR < kWave ? static_cast<int>(threadIdx.x / kWave) : sub;
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            float v = which == 0 ? s0[i][e] : s1[i][e];
-            if constexpr (TPR < kWave) {
-#pragma unroll
-              for (int w = TPR; w < kWave; w *= 2) v += __shfl_xor(v, w);
-            }
-            if (TPR >= kWave || threadIdx.x % kWave < TPR) combine[mine * TILE_COLS + Row::col(i, t) + e] = v;
-          }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          const int c = threadIdx.x + k * WG;
-          float v = 0.f;
-          if (c < TILE_COLS)
-#pragma unroll
-            for (int r = 0; r < SETS; ++r) v += combine[r * TILE_COLS + c];
-          total[which][k] = v;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        const int c = threadIdx.x + k * WG;
-        if (c < TILE_COLS && c < cols) out(c, total[0][k], total[1][k]);
-      }
-    }
+        for (int e = 0; e < VEC; ++e) sums[k + j][i][e] = 0.f;
   };
 
-  const int64_t gate_first = a.pieces > 1 ? blockIdx.x / a.pieces : static_cast<int64_t>(blockIdx.x) * a.gates_per_group;
-  const int64_t gate_last = a.pieces > 1 ? gate_first + 1 : min(gate_first + a.gates_per_group, a.gates);
-  const int64_t piece = a.pieces > 1 ? blockIdx.x % a.pieces : 0;
-  for (int64_t gate_row = gate_first; gate_row < gate_last; ++gate_row) {
-    if (a.gate) gate.load(a.gate + gate_row * cols, t, cols);
-    clear(sum_d);
-    clear(sum_df);
-    const int64_t end = min((gate_row + 1) * static_cast<int64_t>(a.gate_rows),
-                            gate_row * static_cast<int64_t>(a.gate_rows) + piece * a.piece_start + a.piece_span);
-    int64_t row = gate_row * static_cast<int64_t>(a.gate_rows) + piece * a.piece_start + sub;
-    for (; row < end; row += a.row_step) {
-      Row dx, dh, h, f;
-      Act8Row<T, TPR, VPT> f8;
-      if constexpr (F8) f8.load(a.f8 + row * a.ld, a.f8 + a.rows * a.ld + row * (a.ld / kAct8Block), t, cols);
-      else f.load(a.f + row * cols, t, cols);
-      if (a.dh_out) dh.load(a.dh_out + row * cols, t, cols);
-      float d[VPT][VEC];
+  Row pre_gamma;
+  if constexpr (PRE) pre_gamma.load(a.pre_gamma, t, cols);
+  const uint32_t piece = blockIdx.x, group = blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * a.gates_per_group;
+  const int64_t last = min(first + a.gates_per_group, a.gates);
+  for (int64_t gate_row = first; gate_row < last; ++gate_row) {
+    const int64_t base = gate_row * static_cast<int64_t>(a.gate_rows) + piece * a.piece_start;
+    const int64_t end = min((gate_row + 1) * static_cast<int64_t>(a.gate_rows), base + a.piece_span);
+    int64_t row = base + sub;
+
+    Row dx, dh, h, dx_next, dh_next, h_next;
+    FRow f, f_next;
+    float pre_mean = 0.f, pre_rstd = 1.f, post_mean = 0.f, post_rstd = 1.f;
+    float pre_mean_next = 0.f, pre_rstd_next = 1.f, post_mean_next = 0.f, post_rstd_next = 1.f;
+    auto load = [&](int64_t r, FRow& f_, Row& dh_, Row& dx_, Row& h_, float& m0, float& r0, float& m1, float& r1) {
+      if constexpr (F8) f_.load(a.f8 + r * a.ld, a.f8 + a.rows * a.ld + r * (a.ld / kAct8Block), t, cols);
+      else f_.load(a.f + r * cols, t, cols);
+      if constexpr (PRE) {
+        dx_.load(a.dx + r * cols, t, cols);
+        h_.load(a.h_out + r * cols, t, cols);
+        m0 = a.pre_mean[r];
+        r0 = a.pre_rstd[r];
+      }
+      if (!PRE || a.dh_out) dh_.load(a.dh_out + r * cols, t, cols);
+      else dh_.zeros();
+      if constexpr (POST) {
+        m1 = a.post_mean[r];
+        r1 = a.post_rstd[r];
+      }
+    };
+    Row gate, post_gamma;
+    float w[VPT][VEC];  // gate post_gamma, or the gate
+    auto weights = [&] {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        if (a.dh_out) dh.values(i, d[i]);
-        else
+        gate.values(i, w[i]);
+        if constexpr (POST) {
+          float g[VEC];
+          post_gamma.values(i, g);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[i][e] = 0.f;
+          for (int e = 0; e < VEC; ++e) w[i][e] *= g[e];
+        }
       }
-      if (pre) {
-        dx.load(a.dx + row * cols, t, cols);
-        h.load(a.h_out + row * cols, t, cols);
-        const float mean = a.pre_mean[row], rstd = a.pre_rstd[row];
+    };
+    if (a.gate) gate.load(a.gate + gate_row * cols, t, cols);
+    else gate.ones();
+    if constexpr (POST) post_gamma.load(a.post_gamma, t, cols);
+    // The next row is on its way while a row is computed, where registers hold both.
+    if (PREFETCH && row < end) load(row, f, dh, dx, h, pre_mean, pre_rstd, post_mean, post_rstd);
+    weights();
+    for (; row < end; row += a.row_step) {
+      if constexpr (PREFETCH) {
+        const int64_t next = row + a.row_step;
+        if (next < end)
+          load(next, f_next, dh_next, dx_next, h_next, pre_mean_next, pre_rstd_next, post_mean_next, post_rstd_next);
+      } else {
+        load(row, f, dh, dx, h, pre_mean, pre_rstd, post_mean, post_rstd);
+      }
+      if constexpr (sizeof(T) == 2) {
+        dh.keep_packed();
+        f.keep_packed();
+        if constexpr (PRE) {
+          dx.keep_packed();
+          h.keep_packed();
+          pre_gamma.keep_packed();
+        }
+      }
+      float d[VPT][VEC], hat[VPT][VEC];
+      if constexpr (PRE) {
+        const float pre_shift = -pre_mean * pre_rstd;
         float s[2] = {0.f, 0.f};
-        float hat[VPT][VEC];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-          float dv[VEC], g[VEC];
-          dx.values(i, dv);
+          float g[VEC];
+          dx.values(i, d[i]);
           pre_gamma.values(i, g);
           h.values(i, hat[i]);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            hat[i][e] = (hat[i][e] - mean) * rstd;
-            const float dg = dv[e] * g[e];  // zero past the row
-            s[0] += dg;
-            s[1] += dg * hat[i][e];
-            sum_g[i][e] += dv[e] * hat[i][e];
-            sum_b[i][e] += dv[e];
+            hat[i][e] = fmaf(hat[i][e], pre_rstd, pre_shift);
+            sums[2][i][e] = fmaf(d[i][e], hat[i][e], sums[2][i][e]);
+            sums[3][i][e] += d[i][e];
+            d[i][e] *= g[e];  // zero past the row
+            s[0] += d[i][e];
+            s[1] = fmaf(d[i][e], hat[i][e], s[1]);
           }
         }
         row_allreduce_sum<TPR, WG, 2>(s, slots, phase);
-        const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
+        const float c1 = -pre_rstd * (s[0] * inv_n), c2 = -pre_rstd * (s[1] * inv_n);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-          float dv[VEC], g[VEC];
-          dx.values(i, dv);
-          pre_gamma.values(i, g);
+          float dv[VEC];
+          dh.values(i, dv);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[i][e] += rstd * (dv[e] * g[e] - c1 - hat[i][e] * c2);
+          for (int e = 0; e < VEC; ++e) d[i][e] = dv[e] + fmaf(d[i][e], pre_rstd, fmaf(hat[i][e], c2, c1));
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) dh.values(i, d[i]);
       }
+      // (what stands past the row in d meets w = 0, or is not stored)
+      const float post_shift = -post_mean * post_rstd;
+      float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         float out[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) out[e] = a.scale * d[i][e];
         Row::store(a.dh + row * cols, i, t, cols, out);
-      }
-      // (from here on d is gate d; what stands past the row in d meets gamma = 0 or is not stored)
-      float hat[VPT][VEC];
-      float mean = 0.f, rstd = 1.f;
-      if (post) {
-        mean = a.post_mean[row];
-        rstd = a.post_rstd[row];
-      }
-      float s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        if constexpr (F8) f8.values(i, hat[i]);
-        else f.values(i, hat[i]);
-        float g[VEC], pg[VEC];
-        if (a.gate) gate.values(i, g);
-        if (post) post_gamma.values(i, pg);
+        f.normalised(i, post_rstd, post_shift, hat[i]);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          hat[i][e] = (hat[i][e] - mean) * rstd;
-          sum_d[i][e] += d[i][e];
-          sum_df[i][e] += d[i][e] * hat[i][e];
-          if (a.gate) d[i][e] *= g[e];
-          if (post) {
-            d[i][e] *= pg[e];
+          sums[0][i][e] += d[i][e];
+          sums[1][i][e] = fmaf(d[i][e], hat[i][e], sums[1][i][e]);
+          d[i][e] *= w[i][e];
+          if constexpr (POST) {
             s[0] += d[i][e];
-            s[1] += d[i][e] * hat[i][e];
+            s[1] = fmaf(d[i][e], hat[i][e], s[1]);
           }
         }
       }
-      if (post) {
+      if constexpr (POST) {
         row_allreduce_sum<TPR, WG, 2>(s, slots, phase);
-        const float c1 = s[0] * inv_n, c2 = s[1] * inv_n;
+        const float c1 = -post_rstd * (s[0] * inv_n), c2 = -post_rstd * (s[1] * inv_n);
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[i][e] = rstd * (d[i][e] - c1 - hat[i][e] * c2);
+          for (int e = 0; e < VEC; ++e) d[i][e] = fmaf(d[i][e], post_rstd, fmaf(hat[i][e], c2, c1));
       }
 #pragma unroll
       for (int i = 0; i < VPT; ++i) Row::store(a.df + row * cols, i, t, cols, d[i]);
+      if constexpr (PREFETCH) {
+        f = f_next;
+        dh = dh_next;
+        if constexpr (PRE) {
+          dx = dx_next;
+          h = h_next;
+          pre_mean = pre_mean_next;
+          pre_rstd = pre_rstd_next;
+        }
+        if constexpr (POST) {
+          post_mean = post_mean_next;
+          post_rstd = post_rstd_next;
+        }
+      }
     }
-    columns(sum_d, sum_df, [&](int c, float d, float df) { emit(c, d, df, gate_row, gate_row == gate_first); });
+    const int64_t item = gate_row * a.pieces + piece;
+    if (POST || a.gate) flush(0, a.gate_sums + item * cols, a.gates * a.pieces * cols);
   }
-  if (pre) {
-    columns(sum_g, sum_b, [&](int c, float g, float b) {
-      part[2 * set + c] = g;
-      part[3 * set + c] = b;
-    });
-  }
+  const int64_t groups = gridDim.x * gridDim.y;
+  if constexpr (PRE) flush(2, a.pre_sums + static_cast<int64_t>(group) * cols, groups * cols);
 }
 
 // The backward of rows that registers do not hold, a workgroup a row: df and dh.  f in the type T.
@@ -579,18 +656,15 @@ template <typename T, int WG>
 __global__ __launch_bounds__(WG) void residual_norm_bwd_columns_kernel(const ResidualNormBwd<T> a) {
   const int c = static_cast<int>(blockIdx.x) * WG + threadIdx.x;
   if (c >= a.cols) return;
-  const int64_t set = a.part_stride;
-  const int64_t group = blockIdx.y;
-  float* const part = a.part + group * a.cols;
-  const int64_t gate_first = a.pieces > 1 ? group / a.pieces : group * a.gates_per_group;
-  const int64_t gate_last = a.pieces > 1 ? gate_first + 1 : min(gate_first + a.gates_per_group, a.gates);
-  const int64_t piece = a.pieces > 1 ? group % a.pieces : 0;
-  float pg = 0.f, pb = 0.f, sg = 0.f, sb = 0.f;
-  for (int64_t gate_row = gate_first; gate_row < gate_last; ++gate_row) {
-    const int64_t end = min((gate_row + 1) * static_cast<int64_t>(a.gate_rows),
-                            gate_row * static_cast<int64_t>(a.gate_rows) + piece * a.piece_start + a.piece_span);
+  const uint32_t piece = blockIdx.y, group = blockIdx.z * gridDim.y + blockIdx.y, groups = gridDim.y * gridDim.z;
+  const int64_t first = static_cast<int64_t>(blockIdx.z) * a.gates_per_group;
+  const int64_t last = min(first + a.gates_per_group, a.gates);
+  float sg = 0.f, sb = 0.f;
+  for (int64_t gate_row = first; gate_row < last; ++gate_row) {
+    const int64_t base = gate_row * static_cast<int64_t>(a.gate_rows) + piece * a.piece_start;
+    const int64_t end = min((gate_row + 1) * static_cast<int64_t>(a.gate_rows), base + a.piece_span);
     float sd = 0.f, sdf = 0.f;
-    for (int64_t row = gate_row * static_cast<int64_t>(a.gate_rows) + piece * a.piece_start; row < end; ++row) {
+    for (int64_t row = base; row < end; ++row) {
       const ResidualNormRow<T> r(a, row);
       const float d = r.stream(c, a.row_sums[2 * row], a.row_sums[2 * row + 1]);
       sd += d;
@@ -602,58 +676,122 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_columns_kernel(const Res
       }
       a.dh[row * a.cols + c] = from_float<T>(a.scale * d);
     }
-    float dg = sdf;
-    if (a.post_gamma) {
-      const float g = a.gate ? to_float(a.gate[gate_row * a.cols + c]) : 1.f;
-      pg += g * sdf;
-      pb += g * sd;
-      dg = to_float(a.post_gamma[c]) * sdf + to_float(a.post_beta[c]) * sd;
-    }
-    if (a.gate) {
-      if (a.pieces > 1) part[4 * set + c] = dg;
-      else if (a.grad_f32) static_cast<float*>(a.dgate)[gate_row * a.cols + c] = dg;
-      else static_cast<T*>(a.dgate)[gate_row * a.cols + c] = from_float<T>(dg);
+    const int64_t item = gate_row * a.pieces + piece;
+    if (a.gate_sums) {
+      a.gate_sums[item * a.cols + c] = sd;
+      a.gate_sums[(a.gates * a.pieces + item) * a.cols + c] = sdf;
     }
   }
-  part[0 * set + c] = pg;
-  part[1 * set + c] = pb;
-  part[2 * set + c] = sg;
-  part[3 * set + c] = sb;
+  if (a.pre_sums) {
+    a.pre_sums[static_cast<int64_t>(group) * a.cols + c] = sg;
+    a.pre_sums[static_cast<int64_t>(groups + group) * a.cols + c] = sb;
+  }
 }
 
-// Stage 2: the column sums over the workgroups' parts, in a fixed order.  32 columns by 32 lanes that share the parts;
-// blockIdx.y: 0 .. 3 the norms' parameters, from 4 on the pieces of a gate row each.
+// Stage 2: from the workgroups' column sums to the parameters' gradients, in a fixed order.  A workgroup has 32 columns and
+// 32 lanes for each; blockIdx.y: 0 the gate and the post norm, 1 the pre norm.  The lanes are `split` to a gate row, whose
+// pieces they share, so that many gate rows are walked side by side, and the pieces of one are.
 template <typename T>
-__global__ __launch_bounds__(1024) void residual_norm_finish_kernel(const ResidualNormFinish a) {
-  __shared__ float tile[32][33];
-  const int job = blockIdx.y < 4 ? blockIdx.y : 4;
-  void* const out = a.out[job];
-  if (!out) return;
-  const int64_t gate_row = job == 4 ? blockIdx.y - 4 : 0;
-  const float* part = a.part + job * a.part_stride + gate_row * a.pieces * a.cols;
-  const int64_t count = job == 4 ? a.pieces : a.groups;
+__global__ __launch_bounds__(1024) void residual_norm_finish_kernel(const ResidualNormFinish<T> a) {
+  __shared__ float tile[2][32][33];
   const int cx = threadIdx.x % 32, ly = threadIdx.x / 32;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + cx;
-  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-  if (c < a.cols) {
-    int64_t g = ly;
-    for (; g + 96 < count; g += 128) {
-      s0 += part[g * a.cols + c];
-      s1 += part[(g + 32) * a.cols + c];
-      s2 += part[(g + 64) * a.cols + c];
-      s3 += part[(g + 96) * a.cols + c];
-    }
-    for (; g < count; g += 32) s0 += part[g * a.cols + c];
-  }
-  tile[ly][cx] = (s0 + s1) + (s2 + s3);
-  __syncthreads();
-  if (ly == 0 && c < a.cols) {
-    float s = 0.f;
+  const int64_t cols = a.cols, c = static_cast<int64_t>(blockIdx.x) * 32 + cx;
+  const bool mine = c < cols;
+  // The sums of two arrays' rows first, first + step, ...: eight loads on their way at once, those past the end repeating the
+  // last row, to no effect.
+  auto walk = [&](const float* p0, const float* p1, int64_t first, int64_t count, int64_t step, float& s0, float& s1) {
+    s0 = s1 = 0.f;
+    if (!mine) return;
+    for (int64_t i = first; i < count; i += 4 * step) {
+      float v0[4], v1[4];
 #pragma unroll
-    for (int k = 0; k < 32; ++k) s += tile[k][cx];
-    const int64_t at = gate_row * a.cols + c;
-    if (a.grad_f32) static_cast<float*>(out)[at] = s;
-    else static_cast<T*>(out)[at] = from_float<T>(s);
+      for (int k = 0; k < 4; ++k) {
+        const int64_t at = min(i + k * step, count - 1) * cols;
+        v0[k] = p0[at];
+        v1[k] = p1[at];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        s0 += i + k * step < count ? v0[k] : 0.f;
+        s1 += i + k * step < count ? v1[k] : 0.f;
+      }
+    }
+  };
+  // Lanes 0 .. n - 1, n a power of two, of each `n` lanes added into the first one's.
+  auto add_lanes = [&](int n, float& s0, float& s1) {
+    tile[0][ly][cx] = s0;
+    tile[1][ly][cx] = s1;
+    for (int w = n / 2; w > 0; w /= 2) {
+      __syncthreads();
+      if (ly % n < w) {
+        tile[0][ly][cx] += tile[0][ly + w][cx];
+        tile[1][ly][cx] += tile[1][ly + w][cx];
+      }
+    }
+    __syncthreads();
+    s0 = tile[0][ly][cx];
+    s1 = tile[1][ly][cx];
+    __syncthreads();
+  };
+  // Over all 32 lanes, to lane 0: the two of a wave, then the sixteen waves.
+  auto add_all = [&](float& s0, float& s1) {
+    s0 += __shfl_xor(s0, 32);
+    s1 += __shfl_xor(s1, 32);
+    if (ly % 2 == 0) {
+      tile[0][ly / 2][cx] = s0;
+      tile[1][ly / 2][cx] = s1;
+    }
+    __syncthreads();
+    if (ly != 0) return;
+    s0 = s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      s0 += tile[0][k][cx];
+      s1 += tile[1][k][cx];
+    }
+  };
+  auto put = [&](void* out, int64_t at, float v) {
+    if (a.grad_f32) static_cast<float*>(out)[at] = v;
+    else static_cast<T*>(out)[at] = from_float<T>(v);
+  };
+  if (a.first + blockIdx.y == 1) {
+    float g, b;
+    walk(a.pre_sums + c, a.pre_sums + a.groups * cols + c, ly, a.groups, 32, g, b);
+    add_all(g, b);
+    if (ly == 0 && mine) {
+      put(a.dpre_gamma, c, g);
+      put(a.dpre_beta, c, b);
+    }
+    return;
+  }
+  const float pg = a.post_gamma && mine ? to_float(a.post_gamma[c]) : 1.f;
+  const float pb = a.post_gamma && mine ? to_float(a.post_beta[c]) : 0.f;
+  const int at_once = 32 / a.split;  // gate rows
+  const int64_t second = a.gates * a.pieces * cols;
+  float sg = 0.f, sb = 0.f;
+  for (int64_t gate0 = 0; gate0 < a.gates; gate0 += at_once) {
+    const int64_t gate_row = gate0 + ly / a.split;
+    const bool here = gate_row < a.gates;
+    float d, df;
+    const float* const p = a.gate_sums + gate_row * a.pieces * cols + c;
+    walk(p, p + second, ly % a.split, here ? a.pieces : 0, a.split, d, df);
+    if (a.split == 32) add_all(d, df);  // (of the one gate row)
+    else if (a.split > 1) add_lanes(a.split, d, df);
+    if (here && mine && ly % a.split == 0) {
+      float g = 1.f;
+      if (a.gate) {
+        put(a.dgate, gate_row * cols + c, pg * df + pb * d);
+        g = to_float(a.gate[gate_row * cols + c]);
+      }
+      sg += g * df;
+      sb += g * d;
+    }
+  }
+  if (!a.post_gamma) return;
+  if (a.split < 32) add_all(sg, sb);
+  if (ly == 0 && mine) {
+    put(a.dpost_gamma, c, sg);
+    put(a.dpost_beta, c, sb);
   }
 }
 
@@ -667,15 +805,23 @@ struct ResidualNormOps {
   struct Shape {
     int tpr, vpt;
   };
-  // How a row of `chunks` chunks is laid over threads.
-  static bool pick_shape(int64_t chunks, Shape* s) {
+  // How a row of `chunks` chunks is laid over threads: as few chunks to a thread as there are threads for, which takes the fewest
+  // instructions from a row's first to its last, since few rows, or few to a workgroup, is what a training step has; but
+  //  - forward, from 8192 rows on, half the threads with two chunks each: at the rate of memory, what is on its way counts
+  //    (bf16, us, one chunk | two: (2048, 2048) 9.1 | 11.0, (2048, 4096) 13.1 | 16.9, (8192, 4096) 56.8 | 52.8,
+  //    (16384, 1024) 24.9 | 23.4, (16384, 2048) 53.4 | 51.5, (16384, 4096) 110 | 103)
+  //  - backward, 65 to 128 chunks, one wave: no barriers, and a workgroup's rows share their column sums (bf16 1024 columns, two
+  //    waves | one: 2048 rows 20.4 | 16.0, 16384 rows 51.0 | 50.1)
+  //  - past 512 chunks two to a thread: 1024 threads have too few registers each (bf16 (2048, 8192) backward 58.0 | 54.8).
+  static bool pick_shape(bool forward, int64_t rows, int64_t chunks, Shape* s) {
+    const bool two = forward ? rows >= 8192 : false;
     if (chunks <= 16) *s = {16, 1};
-    else if (chunks <= 32) *s = {16, 2};
+    else if (chunks <= 32) *s = {32, 1};
     else if (chunks <= 64) *s = {64, 1};
-    else if (chunks <= 128) *s = {64, 2};
-    else if (chunks <= 256) *s = {256, 1};
-    else if (chunks <= 512) *s = {512, 1};
-    else if (chunks <= 1024) *s = {1024, 1};
+    else if (chunks <= 128) *s = two || !forward ? Shape{64, 2} : Shape{128, 1};
+    else if (chunks <= 256) *s = two ? Shape{128, 2} : Shape{256, 1};
+    else if (chunks <= 512) *s = two ? Shape{256, 2} : Shape{512, 1};
+    else if (chunks <= 1024) *s = {512, 2};
     else if (chunks <= 2048) *s = {1024, 2};
     else return false;
     return true;
@@ -687,40 +833,58 @@ struct ResidualNormOps {
     return true;
   }
 
-  template <int TPR, int VPT, bool ANY>
+  template <int TPR, int VPT, bool ANY, bool KEEP>
   static int launch_fwd(const ResidualNormFwd<T>& a, hipStream_t stream) {
     constexpr int WG = TPR <= 64 ? 256 : TPR;
     constexpr int RPW = WG / TPR;
     const int64_t want = ceil_div(a.rows, RPW);
     const int64_t cap = static_cast<int64_t>(device_info().cu_count) * (2048 / WG);
-    hipLaunchKernelGGL((residual_norm_fwd_kernel<T, TPR, VPT, WG, ANY>), dim3(static_cast<unsigned>(std::min(want, cap))),
-                       dim3(WG), 0, stream, a);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(std::min(want, cap))), dim3(WG), 0, stream, a);
+    };
+    if (a.post_gamma && a.pre_gamma) launch(residual_norm_fwd_kernel<T, TPR, VPT, WG, ANY, true, true, KEEP>);
+    else if (a.post_gamma) launch(residual_norm_fwd_kernel<T, TPR, VPT, WG, ANY, true, false, KEEP>);
+    else if (a.pre_gamma) launch(residual_norm_fwd_kernel<T, TPR, VPT, WG, ANY, false, true, KEEP>);
+    else launch(residual_norm_fwd_kernel<T, TPR, VPT, WG, ANY, false, false, KEEP>);
     MG_LAUNCH_CHECK();
     return MG_OK;
   }
 
-#define MG_RESIDUAL_NORM_SHAPES(CALL) \
-  CALL(16, 1);                        \
-  CALL(16, 2);                        \
-  CALL(64, 1);                        \
-  CALL(64, 2);                        \
-  CALL(256, 1);                       \
-  CALL(512, 1);                       \
-  CALL(1024, 1);                      \
+#define MG_RESIDUAL_NORM_FWD_SHAPES(CALL) \
+  CALL(16, 1);                            \
+  CALL(32, 1);                            \
+  CALL(64, 1);                            \
+  CALL(64, 2);                            \
+  CALL(128, 1);                           \
+  CALL(128, 2);                           \
+  CALL(256, 1);                           \
+  CALL(256, 2);                           \
+  CALL(512, 1);                           \
+  CALL(512, 2);                           \
+  CALL(1024, 2)
+#define MG_RESIDUAL_NORM_BWD_SHAPES(CALL) \
+  CALL(16, 1);                            \
+  CALL(32, 1);                            \
+  CALL(64, 1);                            \
+  CALL(64, 2);                            \
+  CALL(256, 1);                           \
+  CALL(512, 1);                           \
+  CALL(512, 2);                           \
   CALL(1024, 2)
 
   template <bool ANY>
   static int dispatch_fwd(Shape s, const ResidualNormFwd<T>& a, hipStream_t stream) {
-#define MG_CASE(TPR_, VPT_) \
-  if (s.tpr == TPR_ && s.vpt == VPT_) return launch_fwd<TPR_, VPT_, ANY>(a, stream)
-    MG_RESIDUAL_NORM_SHAPES(MG_CASE);
+#define MG_CASE(TPR_, VPT_)           \
+  if (s.tpr == TPR_ && s.vpt == VPT_) \
+  return a.f8 || a.x8 ? launch_fwd<TPR_, VPT_, ANY, true>(a, stream) : launch_fwd<TPR_, VPT_, ANY, false>(a, stream)
+    MG_RESIDUAL_NORM_FWD_SHAPES(MG_CASE);
 #undef MG_CASE
     return fail(MG_ERR_UNSUPPORTED, "residual_norm_fwd: no kernel for row shape (%d, %d)", s.tpr, s.vpt);
   }
 
   static int fwd(const ResidualNormFwd<T>& a, int dtype, hipStream_t stream) {
     Shape s;
-    if (a.cols >= VEC && pick_shape(ceil_div(a.cols, VEC), &s)) {
+    if (a.cols >= VEC && pick_shape(true, a.rows, ceil_div(a.cols, VEC), &s)) {
       if (aligned(a.cols, {a.f, a.h, a.gate, a.post_gamma, a.post_beta, a.pre_gamma, a.pre_beta, a.h_out, a.x}))
         return dispatch_fwd<false>(s, a, stream);
       return dispatch_fwd<true>(s, a, stream);
@@ -753,18 +917,40 @@ struct ResidualNormOps {
     return a.gates * a.pieces;
   }
 
-  static int finish(ResidualNormBwd<T>& a, int64_t groups, void* const (&out)[4], hipStream_t stream) {
-    ResidualNormFinish f{};
-    f.part = a.part;
-    f.part_stride = a.part_stride;
+  // Takes the column sums' scratch for `groups` workgroups.
+  static int take_sums(ResidualNormBwd<T>& a, int64_t groups, Scratch& scratch) {
+    const int64_t gate = a.post_gamma || a.gate ? 2 * a.gates * a.pieces * a.cols : 0;
+    const int64_t pre = a.pre_gamma ? 2 * groups * a.cols : 0;
+    // (the second array starts where float4s may)
+    const int64_t at = ceil_div(gate, 4) * 4;
+    MG_TRY(scratch.take(std::max<int64_t>(1, at + pre) * static_cast<int64_t>(sizeof(float))));
+    a.gate_sums = gate ? scratch.as<float>() : nullptr;
+    a.pre_sums = pre ? scratch.as<float>() + at : nullptr;
+    return MG_OK;
+  }
+
+  static int finish(const ResidualNormBwd<T>& a, int64_t groups, void* const (&out)[4], hipStream_t stream) {
+    if (!a.gate_sums && !a.pre_sums) return MG_OK;
+    ResidualNormFinish<T> f{};
+    f.gate_sums = a.gate_sums;
+    f.pre_sums = a.pre_sums;
+    f.gate = a.gate;
+    f.post_gamma = a.post_gamma;
+    f.post_beta = a.post_beta;
+    f.dgate = a.dgate;
+    f.dpost_gamma = out[0];
+    f.dpost_beta = out[1];
+    f.dpre_gamma = out[2];
+    f.dpre_beta = out[3];
     f.cols = a.cols;
     f.groups = groups;
+    f.gates = a.gates;
     f.pieces = a.pieces;
     f.grad_f32 = a.grad_f32;
-    for (int i = 0; i < 4; ++i) f.out[i] = out[i];
-    f.out[4] = a.gate && a.pieces > 1 ? a.dgate : nullptr;
-    if (!f.out[0] && !f.out[2] && !f.out[4]) return MG_OK;
-    const unsigned jobs = 4 + (f.out[4] ? static_cast<unsigned>(a.gates) : 0u);
+    f.split = 32;
+    while (f.split > 1 && (32 / f.split) < a.gates) f.split /= 2;
+    f.first = a.gate_sums ? 0 : 1;
+    const unsigned jobs = (a.gate_sums ? 1u : 0u) + (a.pre_sums ? 1u : 0u);
     hipLaunchKernelGGL((residual_norm_finish_kernel<T>), dim3(static_cast<unsigned>(ceil_div(a.cols, 32)), jobs), dim3(1024), 0,
                        stream, f);
     MG_LAUNCH_CHECK();
@@ -773,16 +959,22 @@ struct ResidualNormOps {
 
   template <int TPR, int VPT, bool ANY, bool F8>
   static int launch_bwd(ResidualNormBwd<T> a, void* const (&out)[4], hipStream_t stream) {
-    constexpr int WG = TPR <= 64 ? (VPT == 1 ? 512 : 256) : TPR;
+    constexpr int WG = TPR <= 64 ? 512 : TPR;
     constexpr int RPW = WG / TPR;
     const bool interleave = a.rows * a.cols * static_cast<int64_t>(sizeof(T)) >= (int64_t{16} << 20);
-    const int64_t groups = partition(a, static_cast<int64_t>(device_info().cu_count) * (WG >= 1024 ? 1 : 2), RPW, interleave);
-    a.part_stride = groups * a.cols;
-    Scratch part;
-    MG_TRY(part.take(5 * a.part_stride * static_cast<int64_t>(sizeof(float))));
-    a.part = part.as<float>();
-    hipLaunchKernelGGL((residual_norm_bwd_kernel<T, TPR, VPT, WG, ANY, F8>), dim3(static_cast<unsigned>(groups)), dim3(WG), 0,
-                       stream, a);
+    // Eight waves a CU: each workgroup has its parameters to load and its sums to write, and the next row is on its way anyway
+    // (us with 4 | 8 | 16 waves: (4096, 768) fp16 31 | 26 | 34, (16384, 384) bf16 - | 22 | 26, (8192, 4096) bf16 - | 79 | 88).
+    const int64_t most = static_cast<int64_t>(device_info().cu_count) * std::max(1, 8 * kWave / WG);
+    const int64_t groups = partition(a, most, RPW, interleave);
+    Scratch sums;
+    MG_TRY(take_sums(a, groups, sums));
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(a.pieces, static_cast<unsigned>(groups / a.pieces)), dim3(WG), 0, stream, a);
+    };
+    if (a.post_gamma && a.pre_gamma) launch(residual_norm_bwd_kernel<T, TPR, VPT, WG, ANY, F8, true, true>);
+    else if (a.post_gamma) launch(residual_norm_bwd_kernel<T, TPR, VPT, WG, ANY, F8, true, false>);
+    else if (a.pre_gamma) launch(residual_norm_bwd_kernel<T, TPR, VPT, WG, ANY, F8, false, true>);
+    else launch(residual_norm_bwd_kernel<T, TPR, VPT, WG, ANY, F8, false, false>);
     MG_LAUNCH_CHECK();
     return finish(a, groups, out, stream);
   }
@@ -792,16 +984,17 @@ struct ResidualNormOps {
 #define MG_CASE(TPR_, VPT_)           \
   if (s.tpr == TPR_ && s.vpt == VPT_) \
   return a.f8 ? launch_bwd<TPR_, VPT_, ANY, true>(a, out, stream) : launch_bwd<TPR_, VPT_, ANY, false>(a, out, stream)
-    MG_RESIDUAL_NORM_SHAPES(MG_CASE);
+    MG_RESIDUAL_NORM_BWD_SHAPES(MG_CASE);
 #undef MG_CASE
     return fail(MG_ERR_UNSUPPORTED, "residual_norm_bwd: no kernel for row shape (%d, %d)", s.tpr, s.vpt);
   }
-#undef MG_RESIDUAL_NORM_SHAPES
+#undef MG_RESIDUAL_NORM_FWD_SHAPES
+#undef MG_RESIDUAL_NORM_BWD_SHAPES
 
   // out: dpost_gamma, dpost_beta, dpre_gamma, dpre_beta.
   static int bwd(ResidualNormBwd<T> a, void* const (&out)[4], int dtype, hipStream_t stream) {
     Shape s;
-    if (a.cols >= VEC && pick_shape(ceil_div(a.cols, VEC), &s)) {
+    if (a.cols >= VEC && pick_shape(false, a.rows, ceil_div(a.cols, VEC), &s)) {
       if (aligned(a.cols, {a.dx, a.dh_out, a.f, a.h_out, a.gate, a.post_gamma, a.post_beta, a.pre_gamma, a.df, a.dh}))
         return dispatch_bwd<false>(s, a, out, stream);
       return dispatch_bwd<true>(s, a, out, stream);
@@ -819,11 +1012,10 @@ struct ResidualNormOps {
     const int64_t blocks = ceil_div(a.cols, 256);
     const int64_t most = std::max<int64_t>(1, ceil_div(static_cast<int64_t>(device_info().cu_count) * 4, blocks));
     const int64_t groups = partition(a, std::min<int64_t>(most, 65535), 1, false);
-    a.part_stride = groups * a.cols;
-    MG_TRY(part.take(5 * a.part_stride * static_cast<int64_t>(sizeof(float))));
-    a.part = part.as<float>();
-    hipLaunchKernelGGL((residual_norm_bwd_columns_kernel<T, 256>), dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(groups)),
-                       dim3(256), 0, stream, a);
+    MG_TRY(take_sums(a, groups, part));
+    hipLaunchKernelGGL((residual_norm_bwd_columns_kernel<T, 256>),
+                       dim3(static_cast<unsigned>(blocks), a.pieces, static_cast<unsigned>(groups / a.pieces)), dim3(256), 0,
+                       stream, a);
     MG_LAUNCH_CHECK();
     return finish(a, groups, out, stream);
   }
