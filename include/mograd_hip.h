@@ -585,7 +585,8 @@ int mg_residual_norm_fwd(const void* f, const void* h, const void* gate, const v
                          float residual_scale, float eps, int dtype, mg_stream stream);
 
 /* Its gradients.  dx is the gradient of x (NULL, like pre_* and dpre_*, without a pre norm), dh_out what reaches h_out by other
- * ways (NULL for none, where there is a dx); f as it was, or f8 as it is kept in 8 bits, the other NULL; h_out as stored.
+ * ways (NULL for none, where there is a dx); f as it was, or f8 as it is kept in 8 bits, the other NULL (both may be,
+ * where there is neither a gate nor a post norm); h_out as stored (not looked at without a pre norm).
  *   df, dh (rows, cols); dgate like gate; dpost_gamma, dpost_beta, dpre_gamma, dpre_beta (cols)
  * The parameters' gradients are of `grad_dtype`: `dtype`, or MG_F32 for the unrounded fp32 sums; they are fully overwritten, and
  * summed in a fixed order without atomics.  dh may be dh_out; nothing else overlaps.  rows == 0: the sums over no rows are zeros

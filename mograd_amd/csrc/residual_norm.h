@@ -54,7 +54,9 @@ struct ResidualNormRow {
         pre_rstd(args.pre_gamma ? args.pre_rstd[row] : 1.f), post_mean(args.post_gamma ? args.post_mean[row] : 0.f),
         post_rstd(args.post_gamma ? args.post_rstd[row] : 1.f) {}
   __device__ __forceinline__ float pre_hat(int c) const { return (to_float(a.h_out[at + c]) - pre_mean) * pre_rstd; }
-  __device__ __forceinline__ float post_hat(int c) const { return (to_float(a.f[at + c]) - post_mean) * post_rstd; }
+  __device__ __forceinline__ float post_hat(int c) const {
+    return a.f ? (to_float(a.f[at + c]) - post_mean) * post_rstd : 0.f;
+  }
   // The gradient of h', given the two means of the pre norm's.
   __device__ __forceinline__ float stream(int c, float c0, float c1) const {
     float d = a.dh_out ? to_float(a.dh_out[at + c]) : 0.f;

@@ -86,7 +86,8 @@ int mg_residual_norm_bwd(const void* dx, const void* dh_out, const void* f, cons
   }
   MG_TRY(mg::norm_pointers(who, "post", {post_gamma, post_beta, post_mean, post_rstd, dpost_gamma, dpost_beta}));
   MG_TRY(mg::norm_pointers(who, "pre", {pre_gamma, pre_mean, pre_rstd, dx, dpre_gamma, dpre_beta}));
-  if ((f != nullptr) == (f8 != nullptr)) return mg::fail(MG_ERR_INVALID, "%s: f or f8, one of them", who);
+  if (f && f8) return mg::fail(MG_ERR_INVALID, "%s: f or f8, not both", who);
+  if (!f && !f8 && (gate || post_gamma)) return mg::fail(MG_ERR_INVALID, "%s: f or f8 is needed for a gate or a post norm", who);
   if (!df || !dh || (!dh_out && !dx) || (!h_out && dx)) return mg::fail(MG_ERR_INVALID, "%s: null pointer argument", who);
   if (f8) {
     MG_TRY(mg::act8_check(who, rows, cols, dtype));

@@ -471,7 +471,8 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_kernel(const ResidualNor
     float pre_mean_next = 0.f, pre_rstd_next = 1.f, post_mean_next = 0.f, post_rstd_next = 1.f;
     auto load = [&](int64_t r, FRow& f_, Row& dh_, Row& dx_, Row& h_, float& m0, float& r0, float& m1, float& r1) {
       if constexpr (F8) f_.load(a.f8 + r * a.ld, a.f8 + a.rows * a.ld + r * (a.ld / kAct8Block), t, cols);
-      else f_.load(a.f + r * cols, t, cols);
+      else if (POST || a.f) f_.load(a.f + r * cols, t, cols);
+      else f_.zeros();  // (only the sums of d f ask for it, and nobody for them)
       if constexpr (PRE) {
         dx_.load(a.dx + r * cols, t, cols);
         h_.load(a.h_out + r * cols, t, cols);

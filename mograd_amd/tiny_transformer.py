@@ -29,6 +29,16 @@ straight into the gradient arena: no 16-bit rounding of the weight gradients and
 the compute dtype in an arena of their own, one cast to fp32), which the tests compare with.
 All activations and temporaries are allocated once per (batch, context) shape.  This module
 contains no arithmetic; there is no CPU fallback.
+
+Options that the reference's model does not have:
+
+    post_norm=True       h' = residual_scale h + gate * LN_post(block(x)), x' = LN(h'): each block's output is normalised and
+                         scaled by a gate (one number a channel) before it joins the stream; six more parameters a block,
+                         POST_NORM_PARAMS.  Block output to next block's input is one call, mg_residual_norm_fwd, and so are
+                         its gradients, mg_residual_norm_bwd.
+    act8=True            the activations that only the weight gradients and the post norms' backward read (x1, x2, the ReLU's
+                         output, and with post_norm the blocks' outputs) are kept in 8 bits (mg_act8_store, or written so by
+                         mg_residual_norm_fwd) and multiplied from there (mg_linear_bwd_act8): `kept_bytes` says what that saves.
 """
 from __future__ import annotations
 
@@ -42,6 +52,7 @@ from ._lib import BF16, F32, I32, I64, DTYPE_SIZE
 from .runtime import AnyBuffer, Device, MogradError
 
 BLOCK_PARAMS = ("ln1_g", "ln1_b", "wq", "wk", "wv", "wo", "ln2_g", "ln2_b", "w1", "b1", "w2")
+POST_NORM_PARAMS = ("post1_g", "post1_b", "gate1", "post2_g", "post2_b", "gate2")  # after attention, after the MLP
 _ALIGN = 64  # elements: every parameter starts on a 128-byte boundary in either arena
 
 
@@ -57,7 +68,8 @@ class _Slice:
 
 class TinyTransformer:
     def __init__(self, device: Device, vocab_size: int, d_model: int, d_ff: int, n_layers: int, n_heads: int,
-                 compute_dtype: int = BF16, eps: float = 1e-5, deferred: bool = True):
+                 compute_dtype: int = BF16, eps: float = 1e-5, deferred: bool = True, post_norm: bool = False,
+                 residual_scale: float = 1.0, act8: bool = False):
         if d_model % n_heads:
             raise MogradError(1, "d_model must be a multiple of n_heads")
         self.device, self.lib, self.stream = device, device.lib, device.stream
@@ -66,6 +78,7 @@ class TinyTransformer:
         self.cd = compute_dtype
         self.eps = eps
         self.deferred = deferred
+        self.post_norm, self.residual_scale, self.act8 = bool(post_norm), float(residual_scale), bool(act8)
         self.slices: Dict[str, _Slice] = {}
         off = 0
 
@@ -88,6 +101,9 @@ class TinyTransformer:
                     off += -(-3 * d * d // _ALIGN) * _ALIGN
                 elif name not in ("wk", "wv"):
                     place(f"blocks.{layer}.{name}", block_shapes[name])
+            if self.post_norm:
+                for name in POST_NORM_PARAMS:
+                    place(f"blocks.{layer}.{name}", (d,))
         place("lm_head", (V, d))
         self.total = off
         self.master = AnyBuffer.create(F32, device, self.total, fill=0.0)  # fp32 master weights
@@ -153,6 +169,9 @@ class TinyTransformer:
         new = lambda numel, dtype=cd: AnyBuffer.create(dtype, dev, numel)
         self.h = [new(n * d) for _ in range(self.L + 1)]  # residual stream entering each block, and the last
         self.saved: List[dict] = []
+        if self._residual_norm():
+            self._plan_residual_norm(B, T, new)
+            return
         for _ in range(self.L):
             self.saved.append({
                 # Q | K | V per token: the (n, 3d) output of the stacked projection
@@ -195,6 +214,8 @@ class TinyTransformer:
         P = lambda buf: buf.data_ptr()
 
         lib.mg_cast(P(self.master), P(self.work), self.total, F32, cd, s)
+        if self._residual_norm():
+            return self._step_residual_norm(ids, labels, B, T, linear, marks)
 
         # ---- forward
         lib.mg_gather(self._w("embed"), P(ids), P(self.h[0]), n, V, d, d, 1, ids.dtype, cd, s)
@@ -269,6 +290,144 @@ class TinyTransformer:
             marks("backward")
         return self.loss
 
+    # ------------------------------------------------------------------ the step with norms after the blocks, or 8-bit activations
+
+    def _residual_norm(self) -> bool:
+        """Whether the blocks' outputs join the stream by mg_residual_norm_fwd."""
+        return self.post_norm or self.act8 or self.residual_scale != 1.0
+
+    def _plan_residual_norm(self, B: int, T: int, new) -> None:
+        n, d, ff, V = B * T, self.d, self.ff, self.V
+        lib = self.lib
+        act8 = lambda cols: new(-(-lib.mg_act8_bytes(n, cols) // 4), I32)
+        for _ in range(self.L):
+            c = {"qkv": new(3 * n * d), "lse": new(B * self.H * T, F32), "ctx": new(n * d), "h_mid": new(n * d)}
+            for name in ("mean1", "rstd1", "mean2", "rstd2"):
+                c[name] = new(n, F32)
+            kept = [("x1", d), ("x2", d), ("a", ff)]
+            if self.post_norm:
+                kept += [("f1", d), ("f2", d)]
+                for name in ("post_mean1", "post_rstd1", "post_mean2", "post_rstd2"):
+                    c[name] = new(n, F32)
+            for name, cols in kept:
+                if self.act8:
+                    c[name + "_8"] = act8(cols)
+                else:
+                    c[name] = new(n * cols)
+            self.saved.append(c)
+        self.tmp = {name: new(n * d) for name in ("dh", "dctx", "df", "dx", "f")}
+        if self.act8:
+            self.tmp["x"], self.tmp["a"] = new(n * d), new(n * ff)
+        self.tmp["dqkv"], self.tmp["da"] = new(3 * n * d), new(n * ff)
+        self.tmp["logits"], self.tmp["dlogits"] = new(n * V), new(n * V)
+        self.loss = new(1)
+        self._plan_key = (B, T)
+
+    def kept_bytes(self) -> int:
+        """Bytes of what the last step's forward pass left for its backward."""
+        buffers = list(self.h) + [b for c in self.saved for b in c.values()]
+        return sum(b.numel * DTYPE_SIZE[b.dtype] for b in buffers)
+
+    def _step_residual_norm(self, ids, labels, B, T, linear, marks):
+        lib, s, cd = self.lib, self.stream, self.cd
+        n, d, ff, V, H, dh = B * T, self.d, self.ff, self.V, self.H, self.dh
+        scale = 1.0 / math.sqrt(dh)
+        P = lambda buf: buf.data_ptr()
+        t = {k: P(v) for k, v in self.tmp.items()}
+        grad_dtype = F32 if self.deferred else cd
+        at = lambda l, name: self._w(f"blocks.{l}.{name}")
+        g = lambda l, name: self._g(f"blocks.{l}.{name}")
+        post = lambda l, i: [at(l, f"post{i}_g"), at(l, f"post{i}_b")] if self.post_norm else [None, None]
+        post_stats = lambda c, i: [P(c[f"post_mean{i}"]), P(c[f"post_rstd{i}"])] if self.post_norm else [None, None]
+        gate = lambda l, i: at(l, f"gate{i}") if self.post_norm else None
+        x_of = lambda c, name: t["x"] if self.act8 else P(c[name])  # (of one layer at a time, if the rest is in 8 bits)
+        f_of = lambda c, name: P(c[name]) if self.post_norm and not self.act8 else t["f"]
+        kept8 = lambda c, name: P(c[name]) if self.act8 and name in c else None
+
+        # ---- forward
+        lib.mg_gather(self._w("embed"), P(ids), P(self.h[0]), n, V, d, d, 1, ids.dtype, cd, s)
+        c = self.saved[0]
+        lib.mg_layer_norm_fwd_stats(P(self.h[0]), at(0, "ln1_g"), at(0, "ln1_b"), x_of(c, "x1"), P(c["mean1"]), P(c["rstd1"]), n, d,
+                                    self.eps, cd, s)
+        if self.act8:
+            lib.mg_act8_store(t["x"], P(c["x1_8"]), n, d, 0, cd, s)
+        for l in range(self.L):
+            c = self.saved[l]
+            linear(x_of(c, "x1"), at(l, "wq"), P(c["qkv"]), 3 * d, d)
+            lib.mg_flash_attn_fwd_packed(P(c["qkv"]), None, P(c["ctx"]), P(c["lse"]), B, T, H, dh, scale, 1, 0, cd, s)
+            linear(P(c["ctx"]), at(l, "wo"), f_of(c, "f1"), d, d)
+            lib.mg_residual_norm_fwd(f_of(c, "f1"), P(self.h[l]), gate(l, 1), *post(l, 1), at(l, "ln2_g"), at(l, "ln2_b"),
+                                     P(c["h_mid"]), x_of(c, "x2"), *post_stats(c, 1), P(c["mean2"]), P(c["rstd2"]),
+                                     kept8(c, "f1_8"), kept8(c, "x2_8"), n, d, n, self.residual_scale, self.eps, cd, s)
+            a = t["a"] if self.act8 else P(c["a"])
+            lib.mg_matmul_bias_relu_bt(x_of(c, "x2"), at(l, "w1"), at(l, "b1"), a, 1, n, ff, d, d, 1, d, 1, n * d, ff * d, cd, s)
+            if self.act8:
+                lib.mg_act8_store(a, P(c["a_8"]), n, ff, 1, cd, s)
+            linear(a, at(l, "w2"), f_of(c, "f2"), d, ff)
+            nxt = self.saved[l + 1] if l + 1 < self.L else None  # the last block's output meets no norm before the head
+            pre = [at(l + 1, "ln1_g"), at(l + 1, "ln1_b")] if nxt else [None, None]
+            pre_stats = [P(nxt["mean1"]), P(nxt["rstd1"])] if nxt else [None, None]
+            lib.mg_residual_norm_fwd(f_of(c, "f2"), P(c["h_mid"]), gate(l, 2), *post(l, 2), *pre, P(self.h[l + 1]),
+                                     x_of(nxt, "x1") if nxt else None, *post_stats(c, 2), *pre_stats, kept8(c, "f2_8"),
+                                     kept8(nxt, "x1_8") if nxt else None, n, d, n, self.residual_scale, self.eps, cd, s)
+        linear(P(self.h[self.L]), self._w("lm_head"), t["logits"], V, d)
+        lib.mg_cross_entropy_fused_ids(t["logits"], P(labels), None, P(self.loss), t["dlogits"], n, V, cd, labels.dtype, s)
+        if marks:
+            marks("forward")
+
+        # ---- backward
+        def lin_bwd(dy, x, w, dx, dw, db, N, K, relu=0):
+            if self.deferred:
+                lib.mg_linear_bwd_deferred(dy, x, w, dx, dw, db, n, N, K, 0, relu, cd, F32, self.pending, s)
+            else:
+                lib.mg_linear_bwd_fused(dy, x, w, dx, dw, db, n, N, K, 0, relu, cd, s)
+
+        def kept_bwd(dy, c, name, w, dx, dw, db, N, K, relu=0):  # of a layer whose input is one of `kept`
+            if self.act8:
+                lib.mg_linear_bwd_act8(dy, P(c[name + "_8"]), w, dx, dw, db, n, N, K, 0, relu, cd, grad_dtype, s)
+            else:
+                lin_bwd(dy, P(c[name]), w, dx, dw, db, N, K, relu)
+
+        def residual_bwd(l, i, dx, h_out, pre_layer, pre_name, pre_mean, pre_rstd):
+            """df from the gradients dx of the next block's input and `dh` of the stream, which goes one block down in place."""
+            c = self.saved[l]
+            f, f8 = (None, kept8(c, f"f{i}_8")) if self.act8 or not self.post_norm else (P(c[f"f{i}"]), None)
+            gr = lambda layer, *names: [g(layer, name) for name in names]
+            lib.mg_residual_norm_bwd(dx, t["dh"], f, f8, h_out, gate(l, i), *post(l, i), at(pre_layer, pre_name + "_g") if dx else None,
+                                     *post_stats(c, i), pre_mean, pre_rstd, t["df"], t["dh"],
+                                     *(gr(l, f"gate{i}", f"post{i}_g", f"post{i}_b") if self.post_norm else [None] * 3),
+                                     *(gr(pre_layer, pre_name + "_g", pre_name + "_b") if dx else [None] * 2), n, d, n,
+                                     self.residual_scale, cd, grad_dtype, s)
+
+        lin_bwd(t["dlogits"], P(self.h[self.L]), self._w("lm_head"), t["dh"], self._g("lm_head"), None, V, d)
+        for l in reversed(range(self.L)):
+            c = self.saved[l]
+            if l + 1 < self.L:
+                up = self.saved[l + 1]
+                residual_bwd(l, 2, t["dx"], P(self.h[l + 1]), l + 1, "ln1", P(up["mean1"]), P(up["rstd1"]))
+            else:
+                residual_bwd(l, 2, None, None, None, None, None, None)
+            kept_bwd(t["df"], c, "a", at(l, "w2"), t["da"], g(l, "w2"), None, d, ff, relu=1)
+            kept_bwd(t["da"], c, "x2", at(l, "w1"), t["dx"], g(l, "w1"), g(l, "b1"), ff, d)
+            residual_bwd(l, 1, t["dx"], P(c["h_mid"]), l, "ln2", P(c["mean2"]), P(c["rstd2"]))
+            lin_bwd(t["df"], P(c["ctx"]), at(l, "wo"), t["dctx"], g(l, "wo"), None, d, d)
+            lib.mg_flash_attn_bwd_packed(t["dctx"], P(c["ctx"]), P(c["qkv"]), None, P(c["lse"]), t["dqkv"], B, T, H, dh, scale, 1, 0,
+                                         cd, s)
+            kept_bwd(t["dqkv"], c, "x1", at(l, "wq"), t["dx"], g(l, "wq"), None, 3 * d, d)
+        c = self.saved[0]
+        norm = (t["dx"], P(self.h[0]), at(0, "ln1_g"), P(c["mean1"]), P(c["rstd1"]), t["dh"], t["dh"], g(0, "ln1_g"), g(0, "ln1_b"))
+        if self.deferred:
+            lib.mg_layer_norm_bwd_stats_deferred(*norm, n, d, cd, F32, self.pending, s)
+            lib.mg_scatter_add_deferred(P(ids), t["dh"], self._g("embed"), n, V, d, ids.dtype, cd, F32, self.pending, s)
+            lib.mg_finish_deferred(self.pending, s)
+        else:
+            lib.mg_layer_norm_bwd_stats_add(*norm, n, d, cd, s)
+            lib.mg_scatter_add(P(ids), t["dh"], self._g("embed"), n, V, d, ids.dtype, cd, s)
+            lib.mg_cast(P(self.wgrad), P(self.grads), self.total, cd, F32, s)
+        if marks:
+            marks("backward")
+        return self.loss
+
     # ------------------------------------------------------------------ the same step through the rule tables
 
     def graph(self, ids: AnyBuffer, labels: AnyBuffer, B: int, T: int):
@@ -279,6 +438,8 @@ class TinyTransformer:
         cross-entropy on class ids.  Returns (loss node, {parameter name: leaf node})."""
         from .runtime import Layout, Node
 
+        if self._residual_norm():
+            raise MogradError(2, "the rule tables have no node for post_norm, residual_scale or act8: use step()")
         n, d, ff, V, H, dh, cd = B * T, self.d, self.ff, self.V, self.H, self.dh, self.cd
         leaves = {}
 
@@ -387,10 +548,10 @@ class TinyTransformer:
         return linear + self.L * 3.5 * attn_fwd
 
 
-def init_params(rng: np.random.Generator, vocab_size: int, d_model: int, d_ff: int, n_layers: int) -> dict:
+def init_params(rng: np.random.Generator, vocab_size: int, d_model: int, d_ff: int, n_layers: int, post_norm: bool = False) -> dict:
     """Random parameters with the reference's initialisers: Embedding ~ N(0, 1)
     (nn/modules/embedding.mojo:23-29), Linear weight and bias ~ U(+-sqrt(6 / fan_in))
-    (nn/modules/linear.mojo:29-47), LayerNorm gamma 1, beta 0."""
+    (nn/modules/linear.mojo:29-47), LayerNorm gamma 1, beta 0.  post_norm: POST_NORM_PARAMS too, gates of 1."""
     def lin(o, i):
         b = math.sqrt(6.0 / i)
         return rng.uniform(-b, b, size=(o, i)).astype(np.float32)
@@ -405,5 +566,7 @@ def init_params(rng: np.random.Generator, vocab_size: int, d_model: int, d_ff: i
             "w1": lin(ff, d), "b1": rng.uniform(-math.sqrt(6.0 / d), math.sqrt(6.0 / d), ff).astype(np.float32),
             "w2": lin(d, ff),
         })
+        if post_norm:
+            blocks[-1].update({name: (np.zeros if name.endswith("_b") else np.ones)(d, np.float32) for name in POST_NORM_PARAMS})
     return {"embed": rng.standard_normal((vocab_size, d)).astype(np.float32), "lm_head": lin(vocab_size, d),
             "blocks": blocks}

@@ -29,6 +29,7 @@ Pinning (what makes each function trustworthy without running the reference):
   argmax_axis           numpy.argmax on NaN-free input (first occurrence), hand cases
   act8_*                by definition over all steps k (tests/test_act8.py), integers that are their own 8 bits
   residual_norm_*       layer_norm_* above, torch autograd (f64), central differences (tests/test_residual_norm.py)
+  residual_transformer_step  tiny_transformer_step without the options, torch autograd (f64) with (tests/test_residual_transformer.py)
   round_class           tests/test_memory.mojo:18-30 (1000 -> 1024, 1025 -> 1152)
 All of the above are exercised in tests/test_oracle.py, where no other file is named.
 """
@@ -629,6 +630,87 @@ def residual_norm_bwd(dx, dh_out, f, h_out, gate=None, post=None, pre=None, scal
         u = norm_grad(u * gamma, hat, rstd[:, None])
     out["df"] = u
     return out
+
+
+def residual_transformer_step(params, ids, labels, n_heads, scale=1.0, eps=1e-5, store=None, kept=None):
+    """tiny_transformer_step with each block's output joined to the stream by residual_norm_fwd: normalised and gated
+    if the blocks have POST_NORM parameters (post1_g, post1_b, gate1 after attention; post2_g, post2_b, gate2 after the MLP),
+    the stream scaled by `scale`.  `kept(layer, name, value)`, if given, is what the backward sees of the activations
+    x1, x2, a, f1, f2 (rows, cols)."""
+    r = (lambda a: a) if store is None else (lambda a: None if a is None else np.asarray(store(a), dtype=F64))
+    kept = kept or (lambda layer, name, value: value)
+    ids, labels = np.asarray(ids, dtype=np.int64), np.asarray(labels, dtype=np.int64).reshape(-1)
+    B, T = ids.shape
+    blocks, L = params["blocks"], len(params["blocks"])
+    V, d = np.asarray(params["embed"]).shape
+    dh, n = d // n_heads, B * T
+    pair = lambda b, name: (b[name + "_g"], b[name + "_b"])
+
+    def join(b, i, f, h, pre):
+        post, gate = (pair(b, f"post{i}"), np.asarray(b[f"gate{i}"])[None]) if f"gate{i}" in b else (None, None)
+        out = residual_norm_fwd(f, h, gate, post, pre, scale, eps)
+        out["h_out"], out["x"] = r(out["h_out"]), r(out["x"])
+        return out
+
+    h = gather(np.asarray(params["embed"], dtype=F64), ids.reshape(-1))
+    h0 = h
+    x = r(layer_norm_fwd(h, *pair(blocks[0], "ln1"), eps))
+    saved = []
+    for l, b in enumerate(blocks):
+        c = {"x1": x}
+        q, k, v = (r(matmul_bias_bt(x, b[w])).reshape(B, T, n_heads, dh) for w in ("wq", "wk", "wv"))
+        o, _ = sdpa_fwd(q, k, v, causal=True)
+        c["qkv"], c["ctx"] = (q, k, v), r(o).transpose(0, 2, 1, 3).reshape(n, d)
+        c["f1"] = r(matmul_bias_bt(c["ctx"], b["wo"]))
+        c["mid"] = join(b, 1, c["f1"], h, pair(b, "ln2"))
+        c["x2"] = c["mid"]["x"]
+        c["a"] = relu(r(matmul_bias_bt(c["x2"], b["w1"], b["b1"])))
+        c["f2"] = r(matmul_bias_bt(c["a"], b["w2"]))
+        c["end"] = join(b, 2, c["f2"], c["mid"]["h_out"], pair(blocks[l + 1], "ln1") if l + 1 < L else None)
+        h, x = c["end"]["h_out"], c["end"]["x"]
+        for name in ("x1", "x2", "a", "f1", "f2"):
+            c[name] = kept(l, name, c[name])
+        saved.append(c)
+    logits = r(matmul_bias_bt(h, params["lm_head"]))
+    loss = cross_entropy_ids(logits, labels)
+    dlogits = r(cross_entropy_grad_ids(logits, labels, 1.0))
+
+    grads = {"lm_head": r(linear_grad_w(dlogits, h)), "blocks": [dict() for _ in blocks]}
+    state = {"dh": r(linear_grad_x(dlogits, params["lm_head"]))}
+
+    def split(l, i, out, f, dx, pre, into, pre_name):
+        """The gradient of f; `dh` goes on to the stream below."""
+        b = blocks[l]
+        gated = f"gate{i}" in b
+        post = (*pair(b, f"post{i}"), out["post_mean"], out["post_rstd"]) if gated else None
+        got = residual_norm_bwd(dx, state["dh"], f, out["h_out"], np.asarray(b[f"gate{i}"])[None] if gated else None, post,
+                                (*pre, out["pre_mean"], out["pre_rstd"]) if pre else None, scale)
+        if gated:
+            grads["blocks"][l].update({f"gate{i}": r(got["dgate"][0]), f"post{i}_g": r(got["dpost_gamma"]),
+                                       f"post{i}_b": r(got["dpost_beta"])})
+        if pre:
+            grads["blocks"][into].update({pre_name + "_g": r(got["dpre_gamma"]), pre_name + "_b": r(got["dpre_beta"])})
+        state["dh"] = r(got["dh"])
+        return r(got["df"])
+
+    dx = None
+    for l in reversed(range(L)):
+        b, c, g = blocks[l], saved[l], grads["blocks"][l]
+        df = split(l, 2, c["end"], c["f2"], dx, pair(blocks[l + 1], "ln1") if l + 1 < L else None, l + 1, "ln1")
+        g["w2"] = r(linear_grad_w(df, c["a"]))
+        da = relu_grad(c["a"], r(linear_grad_x(df, b["w2"])))
+        g["w1"], g["b1"] = r(linear_grad_w(da, c["x2"])), r(linear_grad_b(da))
+        df = split(l, 1, c["mid"], c["f1"], r(linear_grad_x(da, b["w1"])), pair(b, "ln2"), l, "ln2")
+        g["wo"] = r(linear_grad_w(df, c["ctx"]))
+        do = r(linear_grad_x(df, b["wo"])).reshape(B, T, n_heads, dh).transpose(0, 2, 1, 3)
+        dq, dk, dv = (r(t).reshape(n, d) for t in sdpa_bwd(*c["qkv"], do, causal=True))
+        for name, t in (("wq", dq), ("wk", dk), ("wv", dv)):
+            g[name] = r(linear_grad_w(t, c["x1"]))
+        dx = r(linear_grad_x(dq, b["wq"]) + linear_grad_x(dk, b["wk"]) + linear_grad_x(dv, b["wv"]))
+    din, dg, db = layer_norm_bwd(dx, h0, blocks[0]["ln1_g"], eps)
+    grads["blocks"][0].update({"ln1_g": r(dg), "ln1_b": r(db)})
+    grads["embed"] = r(scatter_add(ids.reshape(-1), r(state["dh"] + r(din)), V))
+    return float(loss), grads
 
 
 # --------------------------------------------------------------------------- #

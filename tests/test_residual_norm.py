@@ -104,7 +104,7 @@ def test_refusals():
             fwd(**bad)
         assert e.value.status == 1 and "residual_norm_fwd" in str(e.value), bad
     for bad in common + [dict(dtype=F16, grads=BF16), dict(grads=I64), dict(dgate=None), dict(gate=None), dict(f8=p), dict(f=None, f8=odd),
-                         dict(df=None), dict(dh=None), dict(h_out=None), dict(dpost=(p, None)), dict(dpre=(None, p)), dict(dx=None),
+                         dict(f=None, post=none4, dpost=(None, None)), dict(df=None), dict(dh=None), dict(h_out=None), dict(dpost=(p, None)), dict(dpre=(None, p)), dict(dx=None),
                          dict(post=none4), dict(pre=(None,) * 3, dx=None, dpre=(None, None), dh_out=None)]:
         with pytest.raises(MogradError) as e:
             bwd(**bad)
@@ -238,8 +238,8 @@ def _check_kept(p, got, dtype):
         assert np.array_equal(got["x8"], O.act8_store(got["x"], KIND[dtype]))
 
 
-def _backward(device, p, saved, dtype, grads, scale, offset=0, in_place=False, act8=False, skip=False):
-    rows, cols = p["f"].shape
+def _backward(device, p, saved, dtype, grads, scale, offset=0, in_place=False, act8=False, skip=False, shape=None):
+    rows, cols = shape or p["f"].shape
     place = _Place(device, offset)
     gates = 0 if p["gate"] is None else len(p["gate"])
     put = lambda a, t=dtype: place.put(a, t)
@@ -374,6 +374,19 @@ def test_rows_do_not_touch_each_other(device, dtype, cols):
         assert np.array_equal(got[n][same], clean[n][same]), n
     assert np.isnan(got["x"][4]).all() and np.isnan(got["x"][9]).all()
     assert np.isfinite(got["x"][12:14]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [33, 384, 70000])
+def test_backward_without_f(device, cols):
+    """Neither a gate nor a post norm: f is not asked for."""
+    p = _inputs(37, 12, cols, 0, 0, 1, F32)
+    saved = _saved(p, F32, 0.5)
+    want = _backward(device, p, saved, F32, F32, 0.5)
+    _check_backward(p, saved, want, F32, F32, 0.5)
+    got = _backward(device, dict(p, f=None), saved, F32, F32, 0.5, shape=(12, cols))
+    for n in want:
+        assert np.array_equal(got[n], want[n]), n
 
 
 @pytest.mark.gpu
