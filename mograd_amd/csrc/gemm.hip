@@ -5,6 +5,8 @@
 #include "gemm_16bit_small.h"
 #include "gemm_f32_direct.h"
 #include "gemm_impl.h"
+#include "linear_act8.h"
+#include "mg_act8.h"
 #include "mg_deferred.h"
 #include "mg_rows.h"
 
@@ -873,6 +875,100 @@ static int linear_bwd_one_launch(const void* dy, const void* x, const void* w, v
   *db_done = groups > 0;
   *done = true;
   return MG_OK;
+}
+
+// Whether the gradients of a layer whose input is kept in 8 bits come from its bytes (act8_dw_block), or from a restored copy of it
+// by the kernels of any Linear backward.  us by the copy | from the bytes, over 200 layers of 64 to 32768 rows and 64 to 8192 columns:
+//   16 bits: the copy takes 2.5 us and M K 3 bytes at 4.6 TB/s, and dW's tiles from bytes are slower than copied ones, so from 2 million
+//     values on, (16384, 384 <- 1536) 89 | 65, (7421, 80 <- 897) 38.5 | 24.8, (4225, 456 <- 2104) 52 | 42, (4096, 1024 <- 1024) 37 | 32, against
+//     (1135, 408 <- 416) 11.3 | 13.8, (1999, 1001 <- 768) 24.6 | 27.3; up to 180 GFLOP, past which 256 x 256 tiles pay for the
+//     copy: (5772, 3568 <- 1768) 239 | 199, (4515, 3288 <- 3800) 269 | 304, (8192, 4096 <- 4096) 444 | 580.  On average 0.6 % more than the better
+//     one for each, the copy always 9 %, the bytes always 11 %.
+//   fp32: three bf16 products at 16 times the rate of an fp32 one, a launch apart from dX's: from 0.8 GFLOP and 128 columns on,
+//     (2048, 512 <- 784) 69 | 52, (1910, 600 <- 632) 66 | 45, (16879, 664 <- 760) 424 | 243, (2048, 4096 <- 4096) 1060 | 740, against
+//     (1202, 629 <- 88) 18.5 | 26, (283, 320 <- 96) 9.4 | 15, (28956, 128 <- 72) 51 | 77.
+// MOGRAD_HIP_ACT8_ROUTE = 0 (the copy) | 1 (the bytes) overrides the choice.
+static bool act8_from_bytes(int64_t M, int64_t N, int64_t K, bool f32) {
+  const double flop = 4.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
+  const bool pays = f32 ? flop >= 8e8 && K >= 128 : static_cast<double>(M) * static_cast<double>(K) >= 2e6 && flop <= 1.8e11;
+  return env_int("MOGRAD_HIP_ACT8_ROUTE", pays) != 0;
+}
+
+// dW (and db) from the bytes of an input in 8 bits: 16-bit layers with dX in the same launch, fp32 ones after a launch of its own for
+// dX, whose mask is the restored input.  The sums over the ranges of rows go out in one launch.
+template <typename T>
+static int linear_act8_one_launch(const void* dy, const uint8_t* q, const uint8_t* e, int64_t ldx, const void* w, void* dx, void* dw,
+                                  void* db, int64_t M, int64_t N, int64_t K, bool dx_accumulate, bool relu, bool grad_f32,
+                                  hipStream_t stream, bool* done) {
+  constexpr bool F32 = sizeof(T) == 4;
+  *done = false;
+  if (M > 0x7fffffffLL || N < WideVec<T>::value || std::max(N, K) + 64 > kGemmDeepMaxLd) return MG_OK;
+  if (!act8_from_bytes(M, N, K, F32)) return MG_OK;
+  // Ranges of rows: a workgroup and a quarter a CU where dX's tiles run beside them, two where dW is alone; of 64 rows at least.
+  const int64_t tiles_n = ceil_div(N, 128), tiles_k = ceil_div(K, 128), tiles = tiles_n * tiles_k, cus = device_info().cu_count;
+  const int64_t wanted = F32 ? std::min<int64_t>(96, 2 * cus / tiles) : (5 * cus / 4 + tiles / 2) / tiles;
+  int splits = static_cast<int>(std::max<int64_t>(1, std::min(wanted, M / 64)));
+  splits = std::max(1, env_int("MOGRAD_HIP_ACT8_SPLITS", splits));
+  const int rows_per_split = static_cast<int>(ceil_div(ceil_div(M, splits), 64) * 64);
+  splits = static_cast<int>(ceil_div(M, rows_per_split));
+  int64_t ldy = N, ldw = K, no_batch = 0;
+  PadCopies<T> pads;
+  if constexpr (!F32) {
+    if (dx) {
+      if (!mult8(N) || !aligned16(dy)) MG_TRY(pads.add(&dy, 1, M, N, &ldy, &no_batch));
+      if (!mult8(K) || !aligned16(w)) MG_TRY(pads.add(&w, 1, N, K, &ldw, &no_batch));
+      MG_TRY(pads.launch(stream));
+    }
+  }
+  Scratch partial, db_part, restored;
+  const int64_t slice = gemm16_partial_floats(N, K, 1, 1);
+  if (splits > 1) MG_TRY(partial.take(splits * slice * static_cast<int64_t>(sizeof(float))));
+  if (db) MG_TRY(db_part.take(splits * N * static_cast<int64_t>(sizeof(float))));
+  Act8Dw<T> pw{static_cast<const T*>(dy), q, e, partial.as<float>(), static_cast<T*>(dw),
+               grad_f32 ? static_cast<float*>(dw) : nullptr, db_part.as<float>(), ldy, ldx, static_cast<int>(M),
+               static_cast<int>(N), static_cast<int>(K), static_cast<int>(tiles_n), static_cast<int>(tiles_k), rows_per_split,
+               splits, false};
+  const int64_t n_dw = splits > 1 ? gemm_split_grid(tiles, splits, 1) : tiles;
+  if constexpr (F32) {
+    if (dx) {
+      GemmArgs g{dy, w, nullptr, dx, 1, M, K, N, N, 1, K, 1, 0, 0, MG_F32};
+      if (relu) {
+        MG_TRY(restored.take(M * K * static_cast<int64_t>(sizeof(T))));
+        MG_TRY(act8_load(q, restored.as<char>(), M, K, MG_F32, stream));
+        g.relu_mask = restored.as<char>();
+      }
+      if (dx_accumulate) g.residual = dx;
+      MG_TRY(gemm_dispatch("linear_bwd_act8(dx)", g, stream));
+    }
+    MG_TRY(launch_linear_act8<T>(pw, nullptr, n_dw, 0, stream));
+  } else {
+    const int x_tiles_m = static_cast<int>(ceil_div(M, 128));
+    Gemm16Problem<T> px{static_cast<const T*>(dy), static_cast<const T*>(w), nullptr, static_cast<T*>(dx), nullptr,
+                        static_cast<int>(M), static_cast<int>(K), static_cast<int>(N), ldy, ldw, K, 0, 0, M * K, x_tiles_m,
+                        static_cast<int>(tiles_k), static_cast<int>(N), 1, 1,
+                        GemmEpilogue<T>{dx_accumulate ? static_cast<const T*>(dx) : nullptr, nullptr, 0}};
+    if (relu) px.mask8 = q, px.mask8_ld = ldx;
+    MG_TRY(launch_linear_act8<T>(pw, &px, n_dw, dx ? x_tiles_m * tiles_k : 0, stream));
+  }
+  *done = true;
+  if (splits == 1 && !db) return MG_OK;
+  DeferredList list;
+  list.out_dtype = grad_f32 || F32 ? MG_F32 : std::is_same_v<T, f16_t> ? MG_F16 : MG_BF16;
+  if (splits > 1)
+    list.push(kDeferSplitK, partial.as<float>(), dw, slice, static_cast<int>(N), static_cast<int>(K), splits, ceil_div(slice / 4, 1024));
+  if (db) list.push(kDeferBiasRows, db_part.as<float>(), db, 0, 0, static_cast<int>(N), splits, ceil_div(ceil_div(N, 64), 4));
+  return mg_finish_deferred(&list, stream);
+}
+
+int linear_bwd_act8_products(const void* dy, const uint8_t* q, const uint8_t* e, int64_t ldx, const void* w, void* dx, void* dw,
+                             void* db, int64_t M, int64_t N, int64_t K, bool dx_accumulate, bool relu, int dtype, int grad_dtype,
+                             hipStream_t stream, bool* done) {
+  auto run = [&](auto zero) {
+    return linear_act8_one_launch<decltype(zero)>(dy, q, e, ldx, w, dx, dw, db, M, N, K, dx_accumulate, relu,
+                                                  grad_dtype == MG_F32 && dtype != MG_F32, stream, done);
+  };
+  if (dtype == MG_F32) return run(float{});
+  return dtype == MG_BF16 ? run(bf16_t{}) : run(f16_t{});
 }
 
 // The same for an fp32 layer small enough for gemm_f32_direct_kernel's tiles: dX, dW and db in one

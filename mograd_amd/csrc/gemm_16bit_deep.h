@@ -47,6 +47,11 @@ struct Gemm16Deep {
   static constexpr int kOccupancy = kWavesPerSimd * 2 / WN < 1 ? 1
                                     : 160 * 1024 / kLds < kWavesPerSimd * 2 / WN ? 160 * 1024 / kLds : kWavesPerSimd * 2 / WN;
   static_assert(kRowsA * 8 % kThreads == 0 && kRowsB0 * 8 % kThreads == 0 && kRowsB1 * 8 % kThreads == 0, "whole requests");
+  static constexpr bool kMask8 = false;  // the output is masked by Gemm16Problem::mask8
+};
+template <class S>
+struct Gemm16DeepMask8 : S {
+  static constexpr bool kMask8 = true;
 };
 // Byte offsets, from the tile's first row and the step's first k, of the 16-byte chunks that this thread
 // requests for one image.  Image row r is row (r / PER_WAVE) * WAVE_ROWS + first + r % PER_WAVE of the
@@ -115,11 +120,11 @@ __device__ __forceinline__ void gemm16_deep_stage(const floatx16 (*acc)[BJ], con
 // Output of a wave's 64 x (32 BJ) values (two rows of accumulator blocks): through the wave's own strip of LDS
 // and out as 16 bytes per lane, whole rows of the strip one after the other.  EARLY (where
 // registers are free): what the epilogue reads is requested before the strip is written.
-template <typename T, bool HAS_BIAS, int BJ, bool EARLY>
+template <typename T, bool HAS_BIAS, int BJ, bool EARLY, bool MASK8 = false>
 __device__ __forceinline__ void gemm16_deep_write(const floatx16 (*acc)[BJ], const float (&bias_v)[BJ],
                                                  uint16_t* __restrict__ mine, T* __restrict__ C, int M, int N, int64_t ldc,
                                                  int row0, int col0, int lane, const T* residual, const T* relu_mask,
-                                                 int relu) {
+                                                 int relu, const uint8_t* mask8 = nullptr, int64_t mask8_ld = 0) {
   constexpr int STRIDE = 32 * BJ + 8;
   constexpr int CPR = 4 * BJ;                                    // 16-byte chunks of a row
   constexpr int PERIOD = CPR % 3 == 0 ? 3 : 1;                   // stores after which the rows of a lane repeat
@@ -139,6 +144,14 @@ __device__ __forceinline__ void gemm16_deep_write(const floatx16 (*acc)[BJ], con
 #pragma unroll
     for (int i = 0; i < CPR; ++i) fetch(i);
   }
+  uint2 m8[MASK8 ? CPR : 1];
+  if constexpr (MASK8) {  // (rows past the edge: the last one; columns past it: the mask has them to the end of a block of 32)
+#pragma unroll
+    for (int i = 0; i < CPR; ++i) {
+      const int r = min(row0 + row[i % PERIOD] + i / PERIOD * ROWS, M - 1), c = col0 + ch[i % PERIOD] * 8;
+      m8[i] = *reinterpret_cast<const uint2*>(mask8 + r * mask8_ld + min(static_cast<int64_t>(c), mask8_ld - 8));
+    }
+  }
   if (relu) gemm16_deep_stage<T, HAS_BIAS, true, BJ>(acc, bias_v, mine, lane);
   else gemm16_deep_stage<T, HAS_BIAS, false, BJ>(acc, bias_v, mine, lane);
   __builtin_amdgcn_wave_barrier();  // the strip is the wave's own: its LDS accesses are in order
@@ -148,7 +161,15 @@ __device__ __forceinline__ void gemm16_deep_write(const floatx16 (*acc)[BJ], con
     const uint16_t* src = mine + rl * STRIDE + ch[i % PERIOD] * 8;
     if (r >= M || c >= N) continue;
     const int64_t at = r * ldc + c;
-    const uint4 v = *reinterpret_cast<const uint4*>(src);
+    uint4 v = *reinterpret_cast<const uint4*>(src);
+    if constexpr (MASK8) {
+      const uint32_t mw[2] = {m8[i].x, m8[i].y};
+      auto keep = [&](uint32_t w, int e) {  // values e and e + 1 of the chunk
+        const bool lo = static_cast<int8_t>(mw[e / 4] >> e % 4 * 8) > 0, hi = static_cast<int8_t>(mw[e / 4] >> (e % 4 + 1) * 8) > 0;
+        return w & ((lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u));
+      };
+      v = make_uint4(keep(v.x, 0), keep(v.y, 2), keep(v.z, 4), keep(v.w, 6));
+    }
     const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
     if (c + 8 > N) {  // the chunk over the right edge, element by element
 #pragma unroll
@@ -565,9 +586,10 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
     uint16_t* mine = reinterpret_cast<uint16_t*>(lds) + wave * 64 * S::kStripStride;
 #pragma unroll
     for (int h = 0; h < AI; ++h) {
-      gemm16_deep_write<T, HAS_BIAS, BJ, AI == 1>(&acc[2 * h], bias_v, mine, pr.C + at, M, N, pr.ldc, row0 + 64 * h, col0, lane,
-                                                 pr.ep.residual ? pr.ep.residual + at : nullptr,
-                                                 pr.ep.relu_mask ? pr.ep.relu_mask + at : nullptr, pr.ep.relu);
+      gemm16_deep_write<T, HAS_BIAS, BJ, AI == 1, S::kMask8>(&acc[2 * h], bias_v, mine, pr.C + at, M, N, pr.ldc, row0 + 64 * h,
+                                                            col0, lane, pr.ep.residual ? pr.ep.residual + at : nullptr,
+                                                            pr.ep.relu_mask ? pr.ep.relu_mask + at : nullptr, pr.ep.relu,
+                                                            pr.mask8, pr.mask8_ld);
       __builtin_amdgcn_wave_barrier();
     }
   }

@@ -767,6 +767,10 @@ struct Gemm16Problem {
   bool partial_stream = false;
   // The output continues as a LayerNorm backward inside the launch (gemm16_deep_ln_bwd).
   Gemm16LayerNormBwd<T> ln;
+  // Where Gemm16Deep::kMask8 is set: C is zero where these signed bytes, rows mask8_ld apart (a multiple of 32, zeros past N), are
+  // not positive; an activation in 8 bits (mg_act8.h) as the mask of the ReLU that it is the output of.
+  const uint8_t* mask8 = nullptr;
+  int64_t mask8_ld = 0;
 };
 
 // How a product's weight gradient is to be left (GemmArgs::deferred, c_f32).

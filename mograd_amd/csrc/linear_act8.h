@@ -1,0 +1,32 @@
+// Arguments of the products with an input in 8 bits (linear_act8_dw.h), shared with their host side (gemm.hip).
+#pragma once
+
+#include "gemm_impl.h"
+
+namespace mg {
+
+template <typename T>
+struct Act8Dw {
+  const T* dy;           // (M, N), rows ldy apart, any address of its elements
+  const uint8_t *q, *e;  // (M, ldx) and (M, ldx / 32)
+  float* partial;        // splits > 1: partial tiles as gemm16_partial_floats says
+  T* dw;                 // splits == 1: the result, of T ...
+  float* dw32;           // ... or, if not null, fp32
+  float* db_part;        // not null: sums of dY over each range of rows, (splits, N)
+  int64_t ldy, ldx;
+  int M, N, K;
+  int tiles_n, tiles_k, rows_per_split, splits;
+  bool partial_stream;  // see Gemm16Problem
+};
+
+// The workgroups of dW, and of dX = dY W behind them (n_dx == 0: none; only for 16-bit types).
+template <typename T>
+int launch_linear_act8(const Act8Dw<T>& dw, const Gemm16Problem<T>* dx, int64_t n_dw, int64_t n_dx, hipStream_t stream);
+
+// gemm.hip: the three gradients from (M, K) bytes q, rows ldx apart, and their exponents e, sums left on `list`.
+// *done = false: not such a layer, nothing launched.
+int linear_bwd_act8_products(const void* dy, const uint8_t* q, const uint8_t* e, int64_t ldx, const void* w, void* dx, void* dw,
+                             void* db, int64_t M, int64_t N, int64_t K, bool dx_accumulate, bool relu, int dtype, int grad_dtype,
+                             hipStream_t stream, bool* done);
+
+}  // namespace mg

@@ -1,4 +1,5 @@
 // The gradients of a Linear layer whose input was kept in 8 bits (format: mg_act8.h).
+#include "linear_act8.h"
 #include "mg_act8.h"
 #include "mg_deferred.h"
 
@@ -22,6 +23,13 @@ int mg_linear_bwd_act8(const void* dy, const void* x8, const void* w, void* dx, 
   }
   MG_TRY(mg::act8_pointer_check(who, x8));
   mg::CaptureHold hold(s);
+  const int64_t ld = mg::act8_ld(K);
+  const uint8_t* const q = static_cast<const uint8_t*>(x8);
+  bool done = false;
+  MG_TRY(mg::linear_bwd_act8_products(dy, q, q + M * ld, ld, w, dx, dw, db, M, N, K, dx_accumulate != 0, x_is_relu_output != 0, dtype,
+                                      grad_dtype, s, &done));
+  if (done) return MG_OK;
+  // The restored input in scratch, and the kernels of a Linear layer's backward.
   mg::Scratch x;
   MG_TRY(x.take(M * K * static_cast<int64_t>(mg::dtype_size(dtype))));
   MG_TRY(mg::act8_load(x8, x.as<char>(), M, K, dtype, s));

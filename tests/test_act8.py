@@ -221,7 +221,11 @@ LINEARS = [(1, 1, 1), (1, 5, 3), (7, 33, 20), (64, 64, 64), (100, 96, 130), (257
 @pytest.mark.parametrize("dtype,grads", [(BF16, BF16), (BF16, F32), (F16, F16), (F16, F32), (F32, F32)])
 @pytest.mark.parametrize("M,N,K", LINEARS)
 @pytest.mark.parametrize("relu", [0, 1])
-def test_linear_gradients(device, M, N, K, dtype, grads, relu):
+@pytest.mark.parametrize("route,splits", [("", ""), ("1", "1"), ("1", "5")])
+def test_linear_gradients(device, monkeypatch, M, N, K, dtype, grads, relu, route, splits):
+    """By the choice that is made for the size, and by the tiles that multiply the bytes, in one range of rows and in several."""
+    monkeypatch.setenv("MOGRAD_HIP_ACT8_ROUTE", route)
+    monkeypatch.setenv("MOGRAD_HIP_ACT8_SPLITS", splits)
     x = _values(21, M, K, dtype)
     if relu:
         x = np.maximum(x, 0)
@@ -271,8 +275,10 @@ def test_linear_of_no_rows(device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", FLOATS)
-def test_what_was_not_finite_shows_in_the_gradient(device, dtype):
+@pytest.mark.parametrize("route", ["0", "1"])
+def test_what_was_not_finite_shows_in_the_gradient(device, monkeypatch, dtype, route):
     """An infinity in the forward's activation: NaN in the columns of dw of its block, the other columns as ever."""
+    monkeypatch.setenv("MOGRAD_HIP_ACT8_ROUTE", route)
     M, N, K = 130, 48, 160
     x = _values(23, M, K, dtype)
     clean = O.act8_load(O.act8_store(x, KIND[dtype]), M, K)
@@ -287,8 +293,52 @@ def test_what_was_not_finite_shows_in_the_gradient(device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("M,N,K", [(64, 8, 32), (190, 131, 129), (130, 256, 96)])
+def test_large_and_infinite_gradients(device, monkeypatch, dtype, M, N, K):
+    """The largest finite dY, tiny ones and an infinity, by the tiles that multiply the bytes: what fp32 products would give."""
+    monkeypatch.setenv("MOGRAD_HIP_ACT8_ROUTE", "1")
+    big = {F32: np.float32(3.4028235e38), BF16: np.float32(3.3895314e38), F16: np.float32(65504)}[dtype]
+    x = np.zeros((M, K), np.float32)
+    x[::7, ::5] = 0.5
+    x[5, 1] = 2.0
+    act8 = O.act8_store(x, KIND[dtype])
+    assert np.array_equal(O.act8_load(act8, M, K), x)
+    dy = np.zeros((M, N), np.float32)
+    dy[7, 0], dy[14, 1], dy[21, 2], dy[28, 3] = big, -big, np.inf, np.float32(2.0 ** -24)
+    dy[5, 4] = np.float32(1 + 2.0 ** -23) if dtype == F32 else 1.0
+    dy = round_to_dtype(dy, dtype)
+    _, dw, db = _linear(device, dy, act8, np.zeros((N, K)), M, N, K, dtype, F32)
+    with np.errstate(invalid="ignore"):
+        want = (dy.astype(np.float64)[:, :, None] * x.astype(np.float64)[:, None, :]).sum(axis=0)
+    np.testing.assert_array_equal(dw, want.astype(np.float32))
+    np.testing.assert_array_equal(db, dy.astype(np.float64).sum(axis=0).astype(np.float32))
+
+
+@pytest.mark.gpu
+def test_routes_agree(device, monkeypatch):
+    """The restored copy and the bytes are the same numbers: the results are, up to the order of the sums."""
+    for dtype in FLOATS:
+        M, N, K = 1500, 264, 200
+        act8 = O.act8_store(np.maximum(_values(25, M, K, dtype), 0), KIND[dtype], True)
+        dy = round_to_dtype(normal(25, 3, (M, N)), dtype)
+        w = round_to_dtype(normal(25, 4, (N, K)), dtype)
+        runs = []
+        for route in ("0", "1"):
+            monkeypatch.setenv("MOGRAD_HIP_ACT8_ROUTE", route)
+            runs.append(_linear(device, dy, act8, w, M, N, K, dtype, F32, relu=1))
+        x8, a = O.act8_load(act8, M, K), np.abs(dy.astype(np.float64))
+        assert (runs[0][0] == 0).sum() == (runs[1][0] == 0).sum() >= (x8 <= 0).sum()
+        for i, mass in ((0, a @ np.abs(w.astype(np.float64))), (1, a.T @ np.abs(x8)), (2, a.sum(0))):
+            bound = _bound(runs[0][i], mass, max(M, N), dtype if i == 0 else F32)
+            assert (np.abs(runs[0][i].astype(np.float64) - runs[1][i]) <= 2 * bound).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_linear_twice_gives_the_same_bits(device, dtype):
+@pytest.mark.parametrize("route", ["0", "1"])
+def test_linear_twice_gives_the_same_bits(device, monkeypatch, dtype, route):
+    monkeypatch.setenv("MOGRAD_HIP_ACT8_ROUTE", route)
     M, N, K = 2000, 96, 160
     act8 = O.act8_store(_values(24, M, K, dtype), KIND[dtype])
     dy = round_to_dtype(normal(24, 3, (M, N)), dtype)
