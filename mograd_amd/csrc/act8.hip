@@ -4,87 +4,112 @@
 
 namespace mg {
 
-// A thread takes 16 columns, half a block: 16 bytes of q, and two (16 bits) or four (fp32) 16-byte chunks of x.  The other
-// half is its neighbouring lane's, so a block's maximum takes one exchange.  One pass, bound by HBM: (s + 33 / 32) bytes a value.
-constexpr int kAct8Unit = 16;
+// A thread takes chunks of 16 bytes of x, neighbouring threads neighbouring ones, so that every access of a wave is one run of
+// memory: (s + 33 / 32) bytes a value in one pass, bound by HBM.  The 4 (16 bits) or 8 (fp32) lanes of a block exchange its maximum.
+// COUNT chunks a thread, a workgroup's width apart, are on their way at once where there are enough to give every CU work.
+// (16384, 1536) bf16 there and back 30.1 us, 5.1 TB/s; (2048, 4096) fp32 16.5 (half a block a thread, 32 or 64 bytes of x side by side:
+// 31.4 and 25.6).
+constexpr int kAct8Threads = 256;
 
-// Row and first column of a unit.
-template <typename Index>
-__device__ __forceinline__ void act8_place(Index unit, uint32_t units_per_row, int64_t& row, int& c) {
-  const Index r = unit / units_per_row;
+// Row and first column of a chunk.
+template <int VEC, typename Index>
+__device__ __forceinline__ void act8_place(Index chunk, uint32_t chunks_per_row, int64_t& row, int& c) {
+  const Index r = chunk / chunks_per_row;
   row = r;
-  c = static_cast<int>(unit - r * units_per_row) * kAct8Unit;
+  c = static_cast<int>(chunk - r * chunks_per_row) * VEC;
 }
 
-template <typename T, bool ANY, typename Index>
-__global__ __launch_bounds__(256) void act8_store_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
-                                                         uint8_t* __restrict__ exponents, int64_t units, int cols,
-                                                         uint32_t units_per_row, int keep_sign) {
-  constexpr int VEC = WideVec<T>::value;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (u >= units) return;  // (units come in pairs, and so do lanes)
-  int64_t row;
-  int c;
-  act8_place<Index>(static_cast<Index>(u), units_per_row, row, c);
-  const T* p = x + row * cols + c;
-  float v[kAct8Unit / VEC][VEC];
-  if (c + kAct8Unit <= cols) {
+template <typename T, bool ANY, typename Index, int COUNT>
+__global__ __launch_bounds__(kAct8Threads) void act8_store_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
+                                                                  uint8_t* __restrict__ exponents, int64_t chunks, int cols,
+                                                                  uint32_t chunks_per_row, int keep_sign) {
+  constexpr int VEC = WideVec<T>::value, LANES = kAct8Block / VEC;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAct8Threads * COUNT) + threadIdx.x;
+  float v[COUNT][VEC];
 #pragma unroll
-    for (int i = 0; i < kAct8Unit / VEC; ++i) {
-      if constexpr (ANY) VecAny<T, VEC>::load(p + i * VEC, v[i]);
-      else VecIO<T, VEC>::load(p + i * VEC, v[i]);
+  for (int k = 0; k < COUNT; ++k) {
+    const int64_t u = first + k * kAct8Threads;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[k][i] = 0.f;
+    if (u >= chunks) continue;
+    int64_t row;
+    int c;
+    act8_place<VEC, Index>(static_cast<Index>(u), chunks_per_row, row, c);
+    const T* const p = x + row * cols + c;
+    if (c + VEC <= cols) {
+      if constexpr (ANY) VecAny<T, VEC>::load(p, v[k]);
+      else VecIO<T, VEC>::load(p, v[k]);
+    } else {  // the row's last values one by one, zeros behind them
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (c + i < cols) v[k][i] = to_float(p[i]);
     }
-  } else {  // the row's last values one by one, zeros behind them
-#pragma unroll
-    for (int i = 0; i < kAct8Unit; ++i) v[i / VEC][i % VEC] = c + i < cols ? to_float(p[i]) : 0.f;
   }
-  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kAct8Unit; ++i) m = max(m, act8_abs_bits(v[i / VEC][i % VEC]));
-  const uint32_t e = act8_exponent<T>(act8_lanes_max<2>(m));
-  const float inverse = act8_inverse(e);
-  uint32_t w[4];
+  for (int k = 0; k < COUNT; ++k) {
+    const int64_t u = first + k * kAct8Threads;
+    if (u >= chunks) return;  // (chunks come in whole blocks, and so do lanes)
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x4[4] = {v[4 * i / VEC][4 * i % VEC], v[4 * i / VEC][4 * i % VEC + 1], v[4 * i / VEC][4 * i % VEC + 2],
-                         v[4 * i / VEC][4 * i % VEC + 3]};
-    w[i] = act8_pack4(x4, inverse, keep_sign != 0);
+    for (int i = 0; i < VEC; ++i) m = max(m, act8_abs_bits(v[k][i]));
+    const uint32_t e = act8_exponent<T>(act8_lanes_max<LANES>(m));
+    const float inverse = act8_inverse(e);
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float x4[4] = {v[k][4 * i], v[k][4 * i + 1], v[k][4 * i + 2], v[k][4 * i + 3]};
+      w[i] = act8_pack4(x4, inverse, keep_sign != 0);
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + u * VEC) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(q + u * VEC) = w[0];
+    if (u % LANES == 0) exponents[u / LANES] = static_cast<uint8_t>(e);
   }
-  *reinterpret_cast<uint4*>(q + u * kAct8Unit) = make_uint4(w[0], w[1], w[2], w[3]);
-  if ((u & 1) == 0) exponents[u / 2] = static_cast<uint8_t>(e);
 }
 
-template <typename T, bool ANY, typename Index>
-__global__ __launch_bounds__(256) void act8_load_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ exponents,
-                                                        T* __restrict__ x, int64_t units, int cols, uint32_t units_per_row) {
-  constexpr int VEC = WideVec<T>::value;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (u >= units) return;
-  int64_t row;
-  int c;
-  act8_place<Index>(static_cast<Index>(u), units_per_row, row, c);
-  const uint4 r = *reinterpret_cast<const uint4*>(q + u * kAct8Unit);
-  const float scale = act8_scale(exponents[u / 2]);
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-  float v[kAct8Unit / VEC][VEC];
+template <typename T, bool ANY, typename Index, int COUNT>
+__global__ __launch_bounds__(kAct8Threads) void act8_load_kernel(const uint8_t* __restrict__ q,
+                                                                 const uint8_t* __restrict__ exponents, T* __restrict__ x,
+                                                                 int64_t chunks, int cols, uint32_t chunks_per_row) {
+  constexpr int VEC = WideVec<T>::value, LANES = kAct8Block / VEC;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAct8Threads * COUNT) + threadIdx.x;
+  uint32_t w[COUNT][VEC / 4], e[COUNT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float x4[4];
-    act8_unpack4(w[i], scale, x4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[4 * i / VEC][4 * i % VEC + j] = x4[j];
-  }
-  T* p = x + row * cols + c;
-  if (c + kAct8Unit <= cols) {
-#pragma unroll
-    for (int i = 0; i < kAct8Unit / VEC; ++i) {
-      if constexpr (ANY) VecAny<T, VEC>::store(p + i * VEC, v[i]);
-      else VecIO<T, VEC>::store(p + i * VEC, v[i]);
+  for (int k = 0; k < COUNT; ++k) {
+    const int64_t u = min(first + k * kAct8Threads, chunks - 1);
+    if constexpr (VEC == 8) {
+      const uint2 r = *reinterpret_cast<const uint2*>(q + u * VEC);
+      w[k][0] = r.x;
+      w[k][1] = r.y;
+    } else {
+      w[k][0] = *reinterpret_cast<const uint32_t*>(q + u * VEC);
     }
-  } else {
+    e[k] = exponents[u / LANES];
+  }
 #pragma unroll
-    for (int i = 0; i < kAct8Unit; ++i)
-      if (c + i < cols) p[i] = from_float<T>(v[i / VEC][i % VEC]);
+  for (int k = 0; k < COUNT; ++k) {
+    const int64_t u = first + k * kAct8Threads;
+    if (u >= chunks) return;
+    int64_t row;
+    int c;
+    act8_place<VEC, Index>(static_cast<Index>(u), chunks_per_row, row, c);
+    const float scale = act8_scale(e[k]);
+    float v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      float x4[4];
+      act8_unpack4(w[k][i], scale, x4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = x4[j];
+    }
+    T* const p = x + row * cols + c;
+    if (c + VEC <= cols) {
+      if constexpr (ANY) VecAny<T, VEC>::store(p, v);
+      else VecIO<T, VEC>::store_stream(p, v);  // (restored for one reader; plain stores 33.2 and 18.6 us)
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (c + i < cols) p[i] = from_float<T>(v[i]);
+    }
   }
 }
 
@@ -94,52 +119,52 @@ static bool act8_aligned(const void* x, int64_t cols) {
   return cols % WideVec<T>::value == 0 && aligned16(x);
 }
 
-template <typename T>
-static int act8_store_typed(const void* x, void* act8, int64_t rows, int64_t cols, bool keep_sign, hipStream_t stream) {
-  const int64_t ld = act8_ld(cols), units = rows * (ld / kAct8Unit);
-  uint8_t* const q = static_cast<uint8_t*>(act8);
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(units, 256))), dim3(256), 0, stream,
-                       static_cast<const T*>(x), q, q + rows * ld, units, static_cast<int>(cols),
-                       static_cast<uint32_t>(ld / kAct8Unit), keep_sign ? 1 : 0);
+// Calls `launch(kernel choice, workgroups)` with what the sizes ask for: chunks at any address or on 16 bytes, 32- or 64-bit division,
+// one chunk a thread or four.
+template <typename T, typename F>
+static int act8_launch(const void* x, int64_t chunks, int64_t cols, F&& launch) {
+  auto indexed = [&](auto any, auto index) {
+    if (chunks >= static_cast<int64_t>(device_info().cu_count) * 4 * kAct8Threads * 4)
+      launch(any, index, std::integral_constant<int, 4>{}, ceil_div(chunks, 4 * kAct8Threads));
+    else launch(any, index, std::integral_constant<int, 1>{}, ceil_div(chunks, kAct8Threads));
   };
-  const bool narrow = units <= 0x7fffffffLL;
-  if (act8_aligned<T>(x, cols)) {
-    if (narrow) launch(act8_store_kernel<T, false, uint32_t>);
-    else launch(act8_store_kernel<T, false, uint64_t>);
-  } else {
-    if (narrow) launch(act8_store_kernel<T, true, uint32_t>);
-    else launch(act8_store_kernel<T, true, uint64_t>);
-  }
+  auto aligned = [&](auto any) {
+    if (chunks <= 0x7fffffffLL) indexed(any, uint32_t{});
+    else indexed(any, uint64_t{});
+  };
+  if (act8_aligned<T>(x, cols)) aligned(std::false_type{});
+  else aligned(std::true_type{});
   MG_LAUNCH_CHECK();
   return MG_OK;
+}
+
+template <typename T>
+static int act8_store_typed(const void* x, void* act8, int64_t rows, int64_t cols, bool keep_sign, hipStream_t stream) {
+  const int64_t ld = act8_ld(cols), per_row = ld / WideVec<T>::value, chunks = rows * per_row;
+  uint8_t* const q = static_cast<uint8_t*>(act8);
+  return act8_launch<T>(x, chunks, cols, [&](auto any, auto index, auto count, int64_t blocks) {
+    hipLaunchKernelGGL((act8_store_kernel<T, decltype(any)::value, decltype(index), decltype(count)::value>),
+                       dim3(static_cast<unsigned>(blocks)), dim3(kAct8Threads), 0, stream, static_cast<const T*>(x), q,
+                       q + rows * ld, chunks, static_cast<int>(cols), static_cast<uint32_t>(per_row), keep_sign ? 1 : 0);
+  });
 }
 
 template <typename T>
 static int act8_load_typed(const void* act8, void* x, int64_t rows, int64_t cols, hipStream_t stream) {
-  const int64_t ld = act8_ld(cols), units = rows * (ld / kAct8Unit);
+  const int64_t ld = act8_ld(cols), per_row = ld / WideVec<T>::value, chunks = rows * per_row;
   const uint8_t* const q = static_cast<const uint8_t*>(act8);
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(ceil_div(units, 256))), dim3(256), 0, stream, q, q + rows * ld,
-                       static_cast<T*>(x), units, static_cast<int>(cols), static_cast<uint32_t>(ld / kAct8Unit));
-  };
-  const bool narrow = units <= 0x7fffffffLL;
-  if (act8_aligned<T>(x, cols)) {
-    if (narrow) launch(act8_load_kernel<T, false, uint32_t>);
-    else launch(act8_load_kernel<T, false, uint64_t>);
-  } else {
-    if (narrow) launch(act8_load_kernel<T, true, uint32_t>);
-    else launch(act8_load_kernel<T, true, uint64_t>);
-  }
-  MG_LAUNCH_CHECK();
-  return MG_OK;
+  return act8_launch<T>(x, chunks, cols, [&](auto any, auto index, auto count, int64_t blocks) {
+    hipLaunchKernelGGL((act8_load_kernel<T, decltype(any)::value, decltype(index), decltype(count)::value>),
+                       dim3(static_cast<unsigned>(blocks)), dim3(kAct8Threads), 0, stream, q, q + rows * ld,
+                       static_cast<T*>(x), chunks, static_cast<int>(cols), static_cast<uint32_t>(per_row));
+  });
 }
 
-// Rows and columns that the format's index arithmetic takes: 2^31 workgroups of 256 units.
+// Rows and columns that the format's index arithmetic takes: 2^31 - 1 workgroups.
 int act8_check(const char* who, int64_t rows, int64_t cols, int dtype) {
   if (!is_float_dtype(dtype)) return fail(MG_ERR_INVALID, "%s: unsupported dtype %s", who, dtype_name(dtype));
   if (rows < 0 || cols <= 0 || cols > 0x3fffffffLL || rows > 0x7fffffffLL ||
-      (rows > 0 && act8_ld(cols) / kAct8Unit > (int64_t{1} << 38) / rows))
+      (rows > 0 && act8_ld(cols) > (int64_t{1} << 40) / rows))
     return fail(MG_ERR_INVALID, "%s: bad shape rows=%lld cols=%lld", who, static_cast<long long>(rows),
                 static_cast<long long>(cols));
   return MG_OK;
