@@ -884,27 +884,47 @@ static int linear_bwd_one_launch(const void* dy, const void* x, const void* w, v
 //     (1135, 408 <- 416) 11.3 | 13.8, (1999, 1001 <- 768) 24.6 | 27.3; up to 180 GFLOP, past which 256 x 256 tiles pay for the
 //     copy: (5772, 3568 <- 1768) 239 | 199, (4515, 3288 <- 3800) 269 | 304, (8192, 4096 <- 4096) 444 | 580.  On average 0.6 % more than the better
 //     one for each, the copy always 9 %, the bytes always 11 %.
-//   fp32: three bf16 products at 16 times the rate of an fp32 one, a launch apart from dX's: from 0.8 GFLOP and 128 columns on,
-//     (2048, 512 <- 784) 69 | 52, (1910, 600 <- 632) 66 | 45, (16879, 664 <- 760) 424 | 243, (2048, 4096 <- 4096) 1060 | 740, against
-//     (1202, 629 <- 88) 18.5 | 26, (283, 320 <- 96) 9.4 | 15, (28956, 128 <- 72) 51 | 77.
+//   fp32: three bf16 products at 16 times the rate of an fp32 one.  With dX in the same launch from 1 GFLOP and 128 columns on, and
+//     from 600 000 values on where they have 256 columns or 0.7 GFLOP: (2048, 512 <- 784) 69 | 43, (1910, 600 <- 632) 72 | 39,
+//     (16384, 1536 <- 384) 422 | 229, (2048, 4096 <- 4096) 1057 | 701, (2945, 56 <- 1064) 45 | 31, against (874, 248 <- 544) 21 | 27,
+//     (1234, 248 <- 136) 14.7 | 23.2, (3094, 996 <- 96) 35 | 44; dW alone from 0.8 GFLOP and 128 columns on: (1910, 601 <- 632) 66 | 45,
+//     against (1202, 629 <- 88) 18.5 | 26, (283, 321 <- 96) 9.4 | 15.
 // MOGRAD_HIP_ACT8_ROUTE = 0 (the copy) | 1 (the bytes) overrides the choice.
-static bool act8_from_bytes(int64_t M, int64_t N, int64_t K, bool f32) {
-  const double flop = 4.0 * static_cast<double>(M) * static_cast<double>(N) * static_cast<double>(K);
-  const bool pays = f32 ? flop >= 8e8 && K >= 128 : static_cast<double>(M) * static_cast<double>(K) >= 2e6 && flop <= 1.8e11;
+static bool act8_from_bytes(int64_t M, int64_t N, int64_t K, bool f32, bool together) {
+  const double values = static_cast<double>(M) * static_cast<double>(K), flop = 4.0 * values * static_cast<double>(N);
+  const bool pays = !f32       ? values >= 2e6 && flop <= 1.8e11
+                    : together ? (flop >= 1e9 && K >= 128) || (values >= 6e5 && (K >= 256 || flop >= 7e8))
+                               : flop >= 8e8 && K >= 128;
   return env_int("MOGRAD_HIP_ACT8_ROUTE", pays) != 0;
 }
 
-// dW (and db) from the bytes of an input in 8 bits: 16-bit layers with dX in the same launch, fp32 ones after a launch of its own for
-// dX, whose mask is the restored input.  The sums over the ranges of rows go out in one launch.
+// The tiles in which an fp32 dX goes beside dW: 128, 64 or 0 (a launch of its own).  Arrays on 16-byte chunks and a tile of 64 for every
+// second CU at least; tiles of 128 from four for every five CUs on, unless their last round is the emptier one by more than the rest of the
+// launch fills.  us by 64 | 128: (5727, 164 <- 1024) 64 | 57, (16384, 1536 <- 384) 244 | 229, (2048, 4096 <- 4096) 761 | 701, against
+// (18195, 1088 <- 192) 134 | 165, (7341, 248 <- 536) 59 | 69, (1024, 1024 <- 1024) 40 | 93.  MOGRAD_HIP_ACT8_XTILE = 0 | 64 | 128 overrides it.
+static int act8_f32_dx_tile(const void* dy, const void* w, int64_t M, int64_t N, int64_t K) {
+  const int64_t cus = device_info().cu_count, blocks128 = ceil_div(M, 128) * ceil_div(K, 128), blocks64 = ceil_div(M, 64) * ceil_div(K, 64);
+  if (!mult4(N) || !mult4(K) || !aligned16(dy) || !aligned16(w) || N < 32 || 2 * blocks64 < cus) return 0;
+  if (env_str("MOGRAD_HIP_ACT8_XTILE")) {
+    const int only = env_int("MOGRAD_HIP_ACT8_XTILE", 0);
+    return only == 64 || only == 128 ? only : 0;
+  }
+  return 5 * blocks128 >= 4 * cus && 4.0 * ceil_div(blocks128, cus) <= 1.4 * ceil_div(blocks64, cus) ? 128 : 64;
+}
+
+// dW (and db) from the bytes of an input in 8 bits, with dX in the same launch, or, where act8_f32_dx_tile says so, after a launch of its
+// own for it, whose mask is the restored input.  The sums over the ranges of rows go out in one launch.
 template <typename T>
 static int linear_act8_one_launch(const void* dy, const uint8_t* q, const uint8_t* e, int64_t ldx, const void* w, void* dx, void* dw,
                                   void* db, int64_t M, int64_t N, int64_t K, bool dx_accumulate, bool relu, bool grad_f32,
                                   hipStream_t stream, bool* done) {
   constexpr bool F32 = sizeof(T) == 4;
   *done = false;
-  if (M > 0x7fffffffLL || N < WideVec<T>::value || std::max(N, K) + 64 > kGemmDeepMaxLd) return MG_OK;
-  if (!act8_from_bytes(M, N, K, F32)) return MG_OK;
-  // Ranges of rows: a workgroup and a quarter a CU where dX's tiles run beside them, two where dW is alone; of 64 rows at least.
+  // (rows in 32 bits, with room for what the ranges' lengths are rounded up by)
+  if (M > 0x7f000000LL || N < WideVec<T>::value || std::max(N, K) + 64 > kGemmDeepMaxLd) return MG_OK;
+  const int x_tile = !F32 ? 128 : dx ? act8_f32_dx_tile(dy, w, M, N, K) : 0;
+  if (!act8_from_bytes(M, N, K, F32, x_tile != 0)) return MG_OK;
+  // Ranges of rows: a workgroup and a quarter a CU where a 16-bit dX's tiles run beside them, two in fp32; of 64 rows at least.
   const int64_t tiles_n = ceil_div(N, 128), tiles_k = ceil_div(K, 128), tiles = tiles_n * tiles_k, cus = device_info().cu_count;
   const int64_t wanted = F32 ? std::min<int64_t>(96, 2 * cus / tiles) : (5 * cus / 4 + tiles / 2) / tiles;
   int splits = static_cast<int>(std::max<int64_t>(1, std::min(wanted, M / 64)));
@@ -929,27 +949,24 @@ static int linear_act8_one_launch(const void* dy, const uint8_t* q, const uint8_
                static_cast<int>(N), static_cast<int>(K), static_cast<int>(tiles_n), static_cast<int>(tiles_k), rows_per_split,
                splits, false};
   const int64_t n_dw = splits > 1 ? gemm_split_grid(tiles, splits, 1) : tiles;
-  if constexpr (F32) {
-    if (dx) {
-      GemmArgs g{dy, w, nullptr, dx, 1, M, K, N, N, 1, K, 1, 0, 0, MG_F32};
-      if (relu) {
-        MG_TRY(restored.take(M * K * static_cast<int64_t>(sizeof(T))));
-        MG_TRY(act8_load(q, restored.as<char>(), M, K, MG_F32, stream));
-        g.relu_mask = restored.as<char>();
-      }
-      if (dx_accumulate) g.residual = dx;
-      MG_TRY(gemm_dispatch("linear_bwd_act8(dx)", g, stream));
+  const int x_tiles_m = static_cast<int>(ceil_div(M, std::max(x_tile, 1))), x_tiles_k = static_cast<int>(ceil_div(K, std::max(x_tile, 1)));
+  Gemm16Problem<T> px{static_cast<const T*>(dy), static_cast<const T*>(w), nullptr, static_cast<T*>(dx), nullptr,
+                      static_cast<int>(M), static_cast<int>(K), static_cast<int>(N), ldy, ldw, K, 0, 0, M * K, x_tiles_m,
+                      x_tiles_k, static_cast<int>(N), 1, 1,
+                      GemmEpilogue<T>{dx_accumulate ? static_cast<const T*>(dx) : nullptr, nullptr, 0}};
+  if (relu) px.mask8 = q, px.mask8_ld = ldx;
+  const int64_t n_dx = dx && x_tile != 0 ? static_cast<int64_t>(x_tiles_m) * x_tiles_k : 0;
+  if (dx && n_dx == 0) {
+    GemmArgs g{dy, w, nullptr, dx, 1, M, K, N, N, 1, K, 1, 0, 0, MG_F32};
+    if (relu) {
+      MG_TRY(restored.take(M * K * static_cast<int64_t>(sizeof(T))));
+      MG_TRY(act8_load(q, restored.as<char>(), M, K, MG_F32, stream));
+      g.relu_mask = restored.as<char>();
     }
-    MG_TRY(launch_linear_act8<T>(pw, nullptr, n_dw, 0, stream));
-  } else {
-    const int x_tiles_m = static_cast<int>(ceil_div(M, 128));
-    Gemm16Problem<T> px{static_cast<const T*>(dy), static_cast<const T*>(w), nullptr, static_cast<T*>(dx), nullptr,
-                        static_cast<int>(M), static_cast<int>(K), static_cast<int>(N), ldy, ldw, K, 0, 0, M * K, x_tiles_m,
-                        static_cast<int>(tiles_k), static_cast<int>(N), 1, 1,
-                        GemmEpilogue<T>{dx_accumulate ? static_cast<const T*>(dx) : nullptr, nullptr, 0}};
-    if (relu) px.mask8 = q, px.mask8_ld = ldx;
-    MG_TRY(launch_linear_act8<T>(pw, &px, n_dw, dx ? x_tiles_m * tiles_k : 0, stream));
+    if (dx_accumulate) g.residual = dx;
+    MG_TRY(gemm_dispatch("linear_bwd_act8(dx)", g, stream));
   }
+  MG_TRY(launch_linear_act8<T>(pw, &px, x_tile, n_dw, n_dx, stream));
   *done = true;
   if (splits == 1 && !db) return MG_OK;
   DeferredList list;

@@ -878,15 +878,19 @@ __device__ __forceinline__ void gemm32_pipe_frag(const char* __restrict__ lds_st
 // SPLIT_K: a work item is (K range, batch, tile); the fp32 partial tiles go to
 // partial[(split * batches + batch), M, N] and gemm_splitk_reduce_kernel adds them up in a
 // fixed order (for outputs with too few tiles to fill the device, e.g. a 10-class head).
-template <bool A_KC, bool B_KC, bool HAS_BIAS, bool SPLIT_K, int TS>
-__global__ __launch_bounds__(kGemmThreads, TS == 128 ? 2 : 4) void gemm_f32_pipe_kernel(
-    const float* __restrict__ A, const float* __restrict__ B, const float* __restrict__ bias, float* __restrict__ C,
-    float* __restrict__ partial, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int64_t bsa, int64_t bsb,
-    int64_t bsc, int tiles_m, int tiles_n, int batches, int k_per_split, int total_work, GemmEpilogue<float> ep_in) {
-  constexpr int OP = TS * kGemmBK * 4;  // bytes of one operand's step
-  constexpr int NT = TS / 64;           // 32 x 32 tiles of a wave along either axis
-  constexpr int NI = TS / 32;           // copy requests per thread, operand and step
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][OP];
+// MASK8: C is zero where these signed bytes, rows mask8_ld apart, are not positive.
+// Work items first, first + stride, ...; `lds` is four times kGemm32PipeOperand<TS> bytes on 1024.
+template <int TS>
+constexpr int kGemm32PipeOperand = TS * kGemmBK * 4;  // bytes of one operand's step
+template <bool A_KC, bool B_KC, bool HAS_BIAS, bool SPLIT_K, int TS, bool MASK8 = false>
+__device__ __forceinline__ void gemm32_pipe_work(
+    char* lds, int first, int stride, const float* __restrict__ A, const float* __restrict__ B, const float* __restrict__ bias,
+    float* __restrict__ C, float* __restrict__ partial, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int64_t bsa,
+    int64_t bsb, int64_t bsc, int tiles_m, int tiles_n, int batches, int k_per_split, int total_work,
+    const GemmEpilogue<float>& ep_in, const uint8_t* __restrict__ mask8 = nullptr, int64_t mask8_ld = 0) {
+  constexpr int OP = kGemm32PipeOperand<TS>;
+  constexpr int NT = TS / 64;  // 32 x 32 tiles of a wave along either axis
+  constexpr int NI = TS / 32;  // copy requests per thread, operand and step
 
   const int tiles = tiles_m * tiles_n;
   const int wave = threadIdx.x / kWave;
@@ -898,7 +902,7 @@ __global__ __launch_bounds__(kGemmThreads, TS == 128 ? 2 : 4) void gemm_f32_pipe
   // The grid holds at most the workgroups that are resident at once; each takes output tiles
   // work, work + gridDim.x, ...  Workgroups that share operand slabs then start every tile
   // together, which keeps their fetches of the shared rows close in time.
-  for (int work = blockIdx.x; work < total_work; work += gridDim.x) {
+  for (int work = first; work < total_work; work += stride) {
     const int split = SPLIT_K ? work / (tiles * batches) : 0;
     const int in_split = SPLIT_K ? work % (tiles * batches) : work;
     const int batch = in_split / tiles;
@@ -930,12 +934,12 @@ __global__ __launch_bounds__(kGemmThreads, TS == 128 ? 2 : 4) void gemm_f32_pipe
     gemm32_pipe_sources<B_KC, TS>(ldb, n0, N, src_b);
     auto request = [&](int step, int copy) {
       if (step == full_steps) {
-        gemm32_pipe_tail<A_KC, TS>(a + step * a_step, src_a, rem, lds[copy][0]);
-        gemm32_pipe_tail<B_KC, TS>(b + step * b_step, src_b, rem, lds[copy][1]);
+        gemm32_pipe_tail<A_KC, TS>(a + step * a_step, src_a, rem, lds + copy * 2 * OP);
+        gemm32_pipe_tail<B_KC, TS>(b + step * b_step, src_b, rem, lds + copy * 2 * OP + OP);
         return;
       }
-      gemm32_pipe_issue<NI>(a + step * a_step, src_a, lds[copy][0]);
-      gemm32_pipe_issue<NI>(b + step * b_step, src_b, lds[copy][1]);
+      gemm32_pipe_issue<NI>(a + step * a_step, src_a, lds + copy * 2 * OP);
+      gemm32_pipe_issue<NI>(b + step * b_step, src_b, lds + copy * 2 * OP + OP);
     };
     request(0, 0);
     for (int it = 0; it < steps; ++it) {
@@ -946,8 +950,8 @@ __global__ __launch_bounds__(kGemmThreads, TS == 128 ? 2 : 4) void gemm_f32_pipe
       MG_WAIT_VMCNT(0);
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       if (it + 1 < steps) request(it + 1, cur ^ 1);
-      const char* la = lds[cur][0];
-      const char* lb = lds[cur][1];
+      const char* la = lds + cur * 2 * OP;
+      const char* lb = lds + cur * 2 * OP + OP;
       // The fragments of k-group g + 1 are requested before the products of group g.
       float fa[2][NT][4], fb[2][NT][4];
       auto frags = [&](int buf, int g) {
@@ -971,7 +975,7 @@ __global__ __launch_bounds__(kGemmThreads, TS == 128 ? 2 : 4) void gemm_f32_pipe
               acc[ti][tj] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[p][ti][j], fb[p][tj][j], acc[ti][tj], 0, 0, 0);
       }
     }
-    // The next tile's first copy goes into lds[0]: every wave must be done reading it.
+    // The next tile's first copy goes into the first one: every wave must be done reading it.
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
     // Accumulator element r of a lane is row (r/4)*8 + (lane/32)*4 + r%4, column lane%32.
@@ -990,12 +994,24 @@ __global__ __launch_bounds__(kGemmThreads, TS == 128 ? 2 : 4) void gemm_f32_pipe
               partial[((static_cast<int64_t>(split) * batches + batch) * M + row) * N + col] = acc[ti][tj][r];
             } else {
               const int64_t at = static_cast<int64_t>(row) * ldc + col;
-              c[at] = gemm_finish<float>(acc[ti][tj][r] + bv, ep, at);
+              float v = acc[ti][tj][r] + bv;
+              if constexpr (MASK8) v = static_cast<int8_t>(mask8[static_cast<int64_t>(row) * mask8_ld + col]) > 0 ? v : 0.f;
+              c[at] = gemm_finish<float>(v, ep, at);
             }
           }
         }
       }
   }  // tiles of this workgroup
+}
+
+template <bool A_KC, bool B_KC, bool HAS_BIAS, bool SPLIT_K, int TS>
+__global__ __launch_bounds__(kGemmThreads, TS == 128 ? 2 : 4) void gemm_f32_pipe_kernel(
+    const float* __restrict__ A, const float* __restrict__ B, const float* __restrict__ bias, float* __restrict__ C,
+    float* __restrict__ partial, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldc, int64_t bsa, int64_t bsb,
+    int64_t bsc, int tiles_m, int tiles_n, int batches, int k_per_split, int total_work, GemmEpilogue<float> ep) {
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kGemm32PipeOperand<TS>];
+  gemm32_pipe_work<A_KC, B_KC, HAS_BIAS, SPLIT_K, TS>(lds, blockIdx.x, gridDim.x, A, B, bias, C, partial, M, N, K, lda, ldb, ldc, bsa,
+                                                      bsb, bsc, tiles_m, tiles_n, batches, k_per_split, total_work, ep);
 }
 
 // out[i] = sum_s partial[s * slice + i] (+ bias[i % N]) for i < numel <= slice, converted to T.  One thread

@@ -19,9 +19,10 @@ struct Act8Dw {
   bool partial_stream;  // see Gemm16Problem
 };
 
-// The workgroups of dW, and of dX = dY W behind them (n_dx == 0: none; only for 16-bit types).
+// The workgroups of dW and those of dX = dY W in one launch (n_dx == 0: dW alone); x_tile: 64 or 128, rows and columns of a tile of an
+// fp32 dX.
 template <typename T>
-int launch_linear_act8(const Act8Dw<T>& dw, const Gemm16Problem<T>* dx, int64_t n_dw, int64_t n_dx, hipStream_t stream);
+int launch_linear_act8(const Act8Dw<T>& dw, const Gemm16Problem<T>* dx, int x_tile, int64_t n_dw, int64_t n_dx, hipStream_t stream);
 
 // gemm.hip: the three gradients from (M, K) bytes q, rows ldx apart, and their exponents e, sums left on `list`.
 // *done = false: not such a layer, nothing launched.

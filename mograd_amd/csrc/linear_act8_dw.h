@@ -312,19 +312,38 @@ __global__ __launch_bounds__(256, 2) void linear_act8_kernel(Act8Dw<T> dw, Gemm1
   else gemm16_deep_block<T, S, true, false, false, false>(lds, blockIdx.x - n_dw, dx);
 }
 
+// The same of an fp32 layer, dX by gemm32_pipe_work's TS x TS tiles.  These run longer and go first: a step of them waits for its
+// copies more than it multiplies, and dW's workgroups use the pipe meanwhile.
+template <int TS, bool RELU>
+__global__ __launch_bounds__(256, 2) void linear_act8_f32_kernel(Act8Dw<float> dw, Gemm16Problem<float> dx, int n_dx) {
+  constexpr int LDS = 4 * kGemm32PipeOperand<TS> > Act8DwShape<float>::kLds ? 4 * kGemm32PipeOperand<TS> : Act8DwShape<float>::kLds;
+  __shared__ __attribute__((aligned(1024))) char lds[LDS];
+  if (static_cast<int>(blockIdx.x) >= n_dx) act8_dw_block<float>(lds, blockIdx.x - n_dx, dw);
+  else
+    gemm32_pipe_work<true, false, false, false, TS, RELU>(lds, blockIdx.x, n_dx, dx.A, dx.B, nullptr, dx.C, nullptr, dx.M, dx.N, dx.K, dx.lda,
+                                                          dx.ldb, dx.ldc, 0, 0, 0, dx.tiles_m, dx.tiles_n, 1, dx.K, n_dx, dx.ep, dx.mask8,
+                                                          dx.mask8_ld);
+}
+
 // n_dx == 0: dW alone.
 template <typename T>
-int launch_linear_act8(const Act8Dw<T>& dw, const Gemm16Problem<T>* dx, int64_t n_dw, int64_t n_dx, hipStream_t stream) {
+int launch_linear_act8(const Act8Dw<T>& dw, const Gemm16Problem<T>* dx, int x_tile, int64_t n_dw, int64_t n_dx, hipStream_t stream) {
   if (n_dw + n_dx > 0x7fffffffLL) return fail(MG_ERR_INVALID, "linear_bwd_act8: too many output tiles");
   if (n_dx == 0) {
     hipLaunchKernelGGL((act8_dw_kernel<T>), dim3(static_cast<unsigned>(n_dw)), dim3(256), 0, stream, dw);
   } else {
+    auto launch = [&](auto kernel, int64_t first) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_dw + n_dx)), dim3(256), 0, stream, dw, *dx, static_cast<int>(first));
+    };
     if constexpr (sizeof(T) == 2) {
-      auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_dw + n_dx)), dim3(256), 0, stream, dw, *dx, static_cast<int>(n_dw));
-      };
-      if (dx->mask8) launch(linear_act8_kernel<T, true>);
-      else launch(linear_act8_kernel<T, false>);
+      if (dx->mask8) launch(linear_act8_kernel<T, true>, n_dw);
+      else launch(linear_act8_kernel<T, false>, n_dw);
+    } else if (x_tile == 128) {
+      if (dx->mask8) launch(linear_act8_f32_kernel<128, true>, n_dx);
+      else launch(linear_act8_f32_kernel<128, false>, n_dx);
+    } else {
+      if (dx->mask8) launch(linear_act8_f32_kernel<64, true>, n_dx);
+      else launch(linear_act8_f32_kernel<64, false>, n_dx);
     }
   }
   MG_LAUNCH_CHECK();

@@ -1,5 +1,5 @@
 // Gradients of f16 Linear layers from an input in 8 bits.
 #include "linear_act8_dw.h"
 namespace mg {
-template int launch_linear_act8<f16_t>(const Act8Dw<f16_t>&, const Gemm16Problem<f16_t>*, int64_t, int64_t, hipStream_t);
+template int launch_linear_act8<f16_t>(const Act8Dw<f16_t>&, const Gemm16Problem<f16_t>*, int, int64_t, int64_t, hipStream_t);
 }  // namespace mg

@@ -250,6 +250,41 @@ def test_linear_gradients(device, monkeypatch, M, N, K, dtype, grads, relu, rout
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(4097, 36, 132), (1000, 100, 580), (2500, 512, 260)])
+@pytest.mark.parametrize("tile", ["0", "64", "128"])
+@pytest.mark.parametrize("relu", [0, 1])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_f32_dx_beside_dw(device, monkeypatch, M, N, K, tile, relu, accumulate):
+    """fp32 arrays on 16-byte chunks: dx in the launch of dw, by either tile, and in one of its own; masked where x is not positive, or
+    was not finite."""
+    monkeypatch.setenv("MOGRAD_HIP_ACT8_ROUTE", "1")
+    monkeypatch.setenv("MOGRAD_HIP_ACT8_XTILE", tile)
+    x = _values(26, M, K, F32)
+    if relu:
+        x = np.maximum(x, 0)
+        x[M // 2, 40] = np.inf
+    act8 = O.act8_store(x, "f32", bool(relu))
+    x8 = O.act8_load(act8, M, K)
+    dy = normal(26, 3, (M, N), std=0.1).astype(np.float32).astype(np.float64)
+    w = normal(26, 4, (N, K), std=K ** -0.5).astype(np.float32).astype(np.float64)
+    before = normal(26, 5, (M, K)).astype(np.float32) if accumulate else None
+    dx, dw, db = _linear(device, dy, act8, w, M, N, K, F32, F32, relu, before)
+    with np.errstate(invalid="ignore"):
+        want = dy @ w * ((x8 > 0) if relu else 1)
+    bound = _bound(want, np.abs(dy) @ np.abs(w), N, F32)
+    if accumulate:
+        want = want + before
+        bound = bound + EPS[F32] / 2 * (np.abs(want) + bound)
+    _check(dx, want, bound, "dx")
+    rest = np.r_[0:32, 64:K] if relu else np.arange(K)
+    if relu:
+        assert (dx[M // 2, 32:64] == (before[M // 2, 32:64] if accumulate else 0)).all() and np.isnan(dw[:, 32:64]).all()
+    want = dy.T @ x8[:, rest]
+    _check(dw[:, rest], want, _bound(want, np.abs(dy).T @ np.abs(x8[:, rest]), M, F32), "dw")
+    _check(db, dy.sum(0), _bound(dy.sum(0), np.abs(dy).sum(0), M, F32), "db")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_linear_without_dx_or_db(device, dtype):
     M, N, K = 300, 72, 200
