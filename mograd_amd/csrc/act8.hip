@@ -1,6 +1,5 @@
 // Activations in 8 bits: putting a tensor away and bringing it back (format: mg_act8.h).
 #include "mg_act8.h"
-#include "mg_rows.h"
 
 namespace mg {
 
@@ -9,15 +8,6 @@ namespace mg {
 // COUNT chunks a thread, a workgroup's width apart, are on their way at once where there are enough to give every CU work.
 // (16384, 1536) bf16 there and back 30.1 us, 5.1 TB/s; (2048, 4096) fp32 16.5 (half a block a thread, 32 or 64 bytes of x side by side:
 // 31.4 and 25.6).
-constexpr int kAct8Threads = 256;
-
-// Row and first column of a chunk.
-template <int VEC, typename Index>
-__device__ __forceinline__ void act8_place(Index chunk, uint32_t chunks_per_row, int64_t& row, int& c) {
-  const Index r = chunk / chunks_per_row;
-  row = r;
-  c = static_cast<int>(chunk - r * chunks_per_row) * VEC;
-}
 
 template <typename T, bool ANY, typename Index, int COUNT>
 __global__ __launch_bounds__(kAct8Threads) void act8_store_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
@@ -70,47 +60,7 @@ template <typename T, bool ANY, typename Index, int COUNT>
 __global__ __launch_bounds__(kAct8Threads) void act8_load_kernel(const uint8_t* __restrict__ q,
                                                                  const uint8_t* __restrict__ exponents, T* __restrict__ x,
                                                                  int64_t chunks, int cols, uint32_t chunks_per_row) {
-  constexpr int VEC = WideVec<T>::value, LANES = kAct8Block / VEC;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAct8Threads * COUNT) + threadIdx.x;
-  uint32_t w[COUNT][VEC / 4], e[COUNT];
-#pragma unroll
-  for (int k = 0; k < COUNT; ++k) {
-    const int64_t u = min(first + k * kAct8Threads, chunks - 1);
-    if constexpr (VEC == 8) {
-      const uint2 r = *reinterpret_cast<const uint2*>(q + u * VEC);
-      w[k][0] = r.x;
-      w[k][1] = r.y;
-    } else {
-      w[k][0] = *reinterpret_cast<const uint32_t*>(q + u * VEC);
-    }
-    e[k] = exponents[u / LANES];
-  }
-#pragma unroll
-  for (int k = 0; k < COUNT; ++k) {
-    const int64_t u = first + k * kAct8Threads;
-    if (u >= chunks) return;
-    int64_t row;
-    int c;
-    act8_place<VEC, Index>(static_cast<Index>(u), chunks_per_row, row, c);
-    const float scale = act8_scale(e[k]);
-    float v[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC / 4; ++i) {
-      float x4[4];
-      act8_unpack4(w[k][i], scale, x4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] = x4[j];
-    }
-    T* const p = x + row * cols + c;
-    if (c + VEC <= cols) {
-      if constexpr (ANY) VecAny<T, VEC>::store(p, v);
-      else VecIO<T, VEC>::store_stream(p, v);  // (restored for one reader; plain stores 33.2 and 18.6 us)
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (c + i < cols) p[i] = from_float<T>(v[i]);
-    }
-  }
+  act8_load_chunks<T, ANY, Index, COUNT>(blockIdx.x, q, exponents, x, chunks, cols, chunks_per_row);
 }
 
 // Every 16-byte chunk of x lies on 16 bytes.
@@ -124,7 +74,7 @@ static bool act8_aligned(const void* x, int64_t cols) {
 template <typename T, typename F>
 static int act8_launch(const void* x, int64_t chunks, int64_t cols, F&& launch) {
   auto indexed = [&](auto any, auto index) {
-    if (chunks >= static_cast<int64_t>(device_info().cu_count) * 4 * kAct8Threads * 4)
+    if (chunks >= act8_many_chunks())
       launch(any, index, std::integral_constant<int, 4>{}, ceil_div(chunks, 4 * kAct8Threads));
     else launch(any, index, std::integral_constant<int, 1>{}, ceil_div(chunks, kAct8Threads));
   };

@@ -101,8 +101,7 @@ struct PadJobs {
   int block_end[3];
 };
 template <typename T>
-__global__ __launch_bounds__(256) void pad_columns_kernel(PadJobs<T> jobs) {
-  const int b = blockIdx.x;
+__device__ __forceinline__ void pad_columns(int b, const PadJobs<T>& jobs) {
   const int which = b < jobs.block_end[0] ? 0 : b < jobs.block_end[1] ? 1 : 2;
   const PadJob<T>& j = jobs.job[which];
   const int64_t i = static_cast<int64_t>(b - (which ? jobs.block_end[which - 1] : 0)) * 256 + threadIdx.x;
@@ -113,6 +112,19 @@ __global__ __launch_bounds__(256) void pad_columns_kernel(PadJobs<T> jobs) {
   const int c0 = static_cast<int>(i - row * per_row) * E;
   const T* src = j.src + row / j.rows * j.batch_stride + row % j.rows * j.ld + c0;
   reinterpret_cast<uint4*>(j.dst)[i] = gemm_gather_chunk(src, j.cols - c0);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void pad_columns_kernel(PadJobs<T> jobs) {
+  pad_columns(blockIdx.x, jobs);
+}
+// The same, and an activation in 8 bits restored by the first workgroups.
+template <typename T>
+__global__ __launch_bounds__(256) void pad_and_restore_kernel(PadJobs<T> jobs, const uint8_t* q, const uint8_t* e, T* x, int64_t chunks,
+                                                              int cols, uint32_t chunks_per_row, int restoring) {
+  static_assert(kAct8Threads == 256, "a workgroup of either");
+  const int b = blockIdx.x;
+  if (b < restoring) act8_load_chunks<T, false, uint32_t, 1>(b, q, e, x, chunks, cols, chunks_per_row);
+  else pad_columns(b - restoring, jobs);
 }
 
 // Collects the operands of one product that need such an image and makes them in one launch.
@@ -144,6 +156,22 @@ struct PadCopies {
     if (count == 0 || blocks == 0) return MG_OK;
     if (blocks > 0x7fffffffLL) return fail(MG_ERR_INVALID, "matmul: operand too large");
     hipLaunchKernelGGL((pad_columns_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, jobs);
+    MG_LAUNCH_CHECK();
+    return MG_OK;
+  }
+  // The copies, and `in` restored to (rows, cols) of T, in one launch where there are copies, none of what is restored, and chunks
+  // few enough for a launch to count: (1999, 768) fp16 and a copy of (1999, 1001) 8.2 us, in two launches 10.0.
+  int launch(const Act8Restore& in, int64_t rows, int64_t cols, bool copies_it, int dtype, hipStream_t stream) {
+    const int64_t ld = act8_ld(cols), per_row = ld / WideVec<T>::value, chunks = rows * per_row;
+    const int64_t restoring = ceil_div(chunks, kAct8Threads);
+    if (count == 0 || copies_it || cols % WideVec<T>::value != 0 || chunks >= act8_many_chunks() || blocks + restoring > 0x7fffffffLL) {
+      MG_TRY(act8_load(in.act8, in.x, rows, cols, dtype, stream));
+      return launch(stream);
+    }
+    const uint8_t* const q = static_cast<const uint8_t*>(in.act8);
+    hipLaunchKernelGGL((pad_and_restore_kernel<T>), dim3(static_cast<unsigned>(restoring + blocks)), dim3(256), 0, stream, jobs, q,
+                       q + rows * ld, static_cast<T*>(in.x), chunks, static_cast<int>(cols), static_cast<uint32_t>(per_row),
+                       static_cast<int>(restoring));
     MG_LAUNCH_CHECK();
     return MG_OK;
   }
@@ -733,7 +761,7 @@ static Choice16 choose_linear_bwd(int64_t M, int64_t N, int64_t K, bool with_dx,
 template <typename T>
 static int linear_bwd_one_launch(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
                                  int64_t N, int64_t K, const void* relu_mask, bool dx_accumulate, hipStream_t stream,
-                                 bool* done, bool* db_done, const LinearBwdLayerNorm* ln) {
+                                 bool* done, bool* db_done, const LinearBwdLayerNorm* ln, const Act8Restore* restore) {
   *done = false;
   *db_done = false;
   if (env_int("MOGRAD_HIP_LINEAR_BWD_ONE_LAUNCH", 1) == 0 || env_str("MOGRAD_HIP_GEMM16_PIPE")) return MG_OK;
@@ -784,7 +812,8 @@ static int linear_bwd_one_launch(const void* dy, const void* x, const void* w, v
     MG_TRY(pads.add(&x, 1, M, K, &ldx, &no_batch));
     if (dx) MG_TRY(pads.add(&w, 1, N, K, &ldw, &no_batch));
   }
-  MG_TRY(pads.launch(stream));
+  if (restore) MG_TRY(pads.launch(*restore, M, K, pad_k && !any, std::is_same_v<T, f16_t> ? MG_F16 : MG_BF16, stream));
+  else MG_TRY(pads.launch(stream));
 
   Scratch partial;
   const int64_t numel = N * K;
@@ -1074,13 +1103,13 @@ static int linear_bwd_bias(const void* dy, void* db, int64_t M, int64_t N, int d
 // *done: dX and dW are on their way; *db_done: so is db (else the caller sums dY's columns).
 int linear_bwd_products(const void* dy, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t N,
                         int64_t K, const void* relu_mask, bool dx_accumulate, int dtype, hipStream_t stream, bool* done,
-                        bool* db_done, const LinearBwdLayerNorm* ln = nullptr) {
+                        bool* db_done, const LinearBwdLayerNorm* ln = nullptr, const Act8Restore* restore = nullptr) {
   *done = false;
   *db_done = false;
   if (dtype == MG_BF16)
-    return linear_bwd_one_launch<bf16_t>(dy, x, w, dx, dw, db, M, N, K, relu_mask, dx_accumulate, stream, done, db_done, ln);
+    return linear_bwd_one_launch<bf16_t>(dy, x, w, dx, dw, db, M, N, K, relu_mask, dx_accumulate, stream, done, db_done, ln, restore);
   if (dtype == MG_F16)
-    return linear_bwd_one_launch<f16_t>(dy, x, w, dx, dw, db, M, N, K, relu_mask, dx_accumulate, stream, done, db_done, ln);
+    return linear_bwd_one_launch<f16_t>(dy, x, w, dx, dw, db, M, N, K, relu_mask, dx_accumulate, stream, done, db_done, ln, restore);
   if (dtype == MG_F32 && !ln)
     return linear_bwd_f32_one_launch(dy, x, w, dx, dw, db, M, N, K, relu_mask, dx_accumulate, stream, done, db_done);
   return MG_OK;
@@ -1223,3 +1252,19 @@ int mg_linear_bwd_layer_norm_bwd(const void* dy, const void* x, const void* w, c
 }
 
 }  // extern "C"
+
+namespace mg {
+
+int linear_bwd_act8_copied(const void* dy, const Act8Restore& restore, const void* w, void* dx, void* dw, void* db, int64_t M,
+                           int64_t N, int64_t K, bool dx_accumulate, bool relu, int dtype, hipStream_t stream) {
+  if (dtype != MG_F32) {
+    bool done = false, db_done = false;
+    MG_TRY(linear_bwd_products(dy, restore.x, w, dx, dw, db, M, N, K, relu ? restore.x : nullptr, dx_accumulate, dtype, stream, &done,
+                               &db_done, nullptr, &restore));
+    if (done) return db && !db_done ? linear_bwd_bias(dy, db, M, N, dtype, stream) : MG_OK;
+  }
+  MG_TRY(act8_load(restore.act8, restore.x, M, K, dtype, stream));
+  return linear_bwd_impl(dy, restore.x, w, dx, dw, db, M, N, K, dx_accumulate, relu, dtype, stream);
+}
+
+}  // namespace mg

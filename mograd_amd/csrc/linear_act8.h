@@ -30,4 +30,13 @@ int linear_bwd_act8_products(const void* dy, const uint8_t* q, const uint8_t* e,
                              void* db, int64_t M, int64_t N, int64_t K, bool dx_accumulate, bool relu, int dtype, int grad_dtype,
                              hipStream_t stream, bool* done);
 
+// An input that the products below read as T and that lies in 8 bits yet: M rows of K columns at `act8`, to be restored into `x`.
+struct Act8Restore {
+  const void* act8;
+  void* x;
+};
+// The same by the kernels of any Linear backward, which read a copy of the input (it is restored into `restore.x`).
+int linear_bwd_act8_copied(const void* dy, const Act8Restore& restore, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t N,
+                           int64_t K, bool dx_accumulate, bool relu, int dtype, hipStream_t stream);
+
 }  // namespace mg

@@ -29,15 +29,19 @@ int mg_linear_bwd_act8(const void* dy, const void* x8, const void* w, void* dx, 
   MG_TRY(mg::linear_bwd_act8_products(dy, q, q + M * ld, ld, w, dx, dw, db, M, N, K, dx_accumulate != 0, x_is_relu_output != 0, dtype,
                                       grad_dtype, s, &done));
   if (done) return MG_OK;
-  // The restored input in scratch, and the kernels of a Linear layer's backward.
   mg::Scratch x;
   MG_TRY(x.take(M * K * static_cast<int64_t>(mg::dtype_size(dtype))));
-  MG_TRY(mg::act8_load(x8, x.as<char>(), M, K, dtype, s));
-  if (grad_dtype == dtype)
-    return mg_linear_bwd_fused(dy, x.as<char>(), w, dx, dw, db, M, N, K, dx_accumulate, x_is_relu_output, dtype, stream);
+  auto run = [&] {
+    return mg::linear_bwd_act8_copied(dy, mg::Act8Restore{x8, x.as<char>()}, w, dx, dw, db, M, N, K, dx_accumulate != 0,
+                                      x_is_relu_output != 0, dtype, s);
+  };
+  if (grad_dtype == dtype) return run();
   mg::DeferredList list;
-  const int rc = mg_linear_bwd_deferred(dy, x.as<char>(), w, dx, dw, db, M, N, K, dx_accumulate, x_is_relu_output, dtype,
-                                        grad_dtype, &list, stream);
+  int rc;
+  {
+    mg::DeferredScope scope(&list, dtype, grad_dtype);
+    rc = run();
+  }
   const int rc2 = mg_finish_deferred(&list, stream);
   return rc != MG_OK ? rc : rc2;
 }

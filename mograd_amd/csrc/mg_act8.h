@@ -17,6 +17,7 @@
 
 #include "mg_device.h"
 #include "mg_internal.h"
+#include "mg_rows.h"
 
 namespace mg {
 
@@ -86,6 +87,66 @@ __device__ __forceinline__ uint32_t act8_lanes_max(uint32_t v) {
   if constexpr (LANES >= 4) v = max(v, move(v, std::integral_constant<int, kDppQuadXor2>{}));
   if constexpr (LANES >= 8) v = max(v, move(v, std::integral_constant<int, kDppRowHalfMirror>{}));
   return v;
+}
+
+constexpr int kAct8Threads = 256;
+// From so many chunks on a thread takes four.
+inline int64_t act8_many_chunks() { return static_cast<int64_t>(device_info().cu_count) * 4 * kAct8Threads * 4; }
+
+// Row and first column of a chunk.
+template <int VEC, typename Index>
+__device__ __forceinline__ void act8_place(Index chunk, uint32_t chunks_per_row, int64_t& row, int& c) {
+  const Index r = chunk / chunks_per_row;
+  row = r;
+  c = static_cast<int>(chunk - r * chunks_per_row) * VEC;
+}
+
+// The work of workgroup `block` of a restoring pass (act8.hip): COUNT chunks of 16 bytes a thread.  ANY: x at any address, rows of any
+// length.
+template <typename T, bool ANY, typename Index, int COUNT>
+__device__ __forceinline__ void act8_load_chunks(int64_t block, const uint8_t* __restrict__ q, const uint8_t* __restrict__ exponents,
+                                                 T* __restrict__ x, int64_t chunks, int cols, uint32_t chunks_per_row) {
+  constexpr int VEC = WideVec<T>::value, LANES = kAct8Block / VEC;
+  const int64_t first = block * (kAct8Threads * COUNT) + threadIdx.x;
+  uint32_t w[COUNT][VEC / 4], e[COUNT];
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) {
+    const int64_t u = min(first + k * kAct8Threads, chunks - 1);
+    if constexpr (VEC == 8) {
+      const uint2 r = *reinterpret_cast<const uint2*>(q + u * VEC);
+      w[k][0] = r.x;
+      w[k][1] = r.y;
+    } else {
+      w[k][0] = *reinterpret_cast<const uint32_t*>(q + u * VEC);
+    }
+    e[k] = exponents[u / LANES];
+  }
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) {
+    const int64_t u = first + k * kAct8Threads;
+    if (u >= chunks) return;
+    int64_t row;
+    int c;
+    act8_place<VEC, Index>(static_cast<Index>(u), chunks_per_row, row, c);
+    const float scale = act8_scale(e[k]);
+    float v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      float x4[4];
+      act8_unpack4(w[k][i], scale, x4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = x4[j];
+    }
+    T* const p = x + row * cols + c;
+    if (c + VEC <= cols) {
+      if constexpr (ANY) VecAny<T, VEC>::store(p, v);
+      else VecIO<T, VEC>::store_stream(p, v);  // (restored for one reader; plain stores 33.2 and 18.6 us)
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (c + i < cols) p[i] = from_float<T>(v[i]);
+    }
+  }
 }
 
 }  // namespace mg

@@ -214,7 +214,7 @@ def _check(got, want, bound, what):
 
 
 LINEARS = [(1, 1, 1), (1, 5, 3), (7, 33, 20), (64, 64, 64), (100, 96, 130), (257, 65, 384), (128, 1001, 77), (999, 40, 32),
-           (513, 256, 300), (3000, 130, 136), (1024, 384, 768), (2048, 512, 2048), (4097, 384, 384)]
+           (513, 256, 300), (3000, 130, 136), (1024, 384, 768), (2048, 512, 2048), (4097, 384, 384), (1999, 1001, 768)]
 
 
 @pytest.mark.gpu
