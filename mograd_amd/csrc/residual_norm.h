@@ -37,9 +37,10 @@ struct ResidualNormBwd {
   // piece_span on or with the gate row.
   int64_t gates, gates_per_group, piece_start, piece_span, row_step;
   uint32_t pieces;
+  int own;  // each of a workgroup's rows in flight has whole gate rows to itself
   // Column sums.  gate_sums [2][gates * pieces][cols]: of d and d fh over each piece of a gate row's rows; pre_sums
   // [2][workgroups][cols]: of dx xh and dx.  Null where nobody asks.
-  float *gate_sums, *pre_sums;
+  float *gate_sums, *pre_sums, *post_sums;  // (post_sums: see ResidualNormFinish)
   float* row_sums;  // (rows, 2), the kernels of wide rows: the two means of the pre norm's gradient
 };
 
@@ -70,7 +71,8 @@ struct ResidualNormFinish {
   const float *gate_sums, *pre_sums;
   const T *gate, *post_gamma, *post_beta;
   void *dgate, *dpost_gamma, *dpost_beta, *dpre_gamma, *dpre_beta;
-  int64_t cols, groups, gates, pieces;
+  float* post_sums;  // of many gate rows, [2][gridDim.z][cols]: the post norm's gradients over gates_per_block each; or null
+  int64_t cols, groups, gates, gates_per_block, pieces;
   int split;  // lanes to a gate row: a power of two, 1 .. 32
   int first;  // the first workgroups' job: 0 the gate and the post norm, 1 the pre norm
   int grad_f32;

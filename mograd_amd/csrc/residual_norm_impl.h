@@ -362,7 +362,8 @@ __global__ __launch_bounds__(WG) void residual_norm_fwd_wide_kernel(const Residu
 // ------------------------------------------------------------------------------------
 // Backward, stage 1: df, dh, and column sums of the workgroup's rows.  A workgroup has either one piece of the rows of one
 // gate row, or several gate rows whole (the partition is the host's, ResidualNormBwd); the sums A and B go out where the gate
-// row changes.  No atomics, fixed orders.
+// row changes.  Many gate rows of few rows (a gate a token) go to the rows in flight, which write A and B from their registers.
+// No atomics, fixed orders.
 // ------------------------------------------------------------------------------------
 
 template <typename T, int TPR, int VPT, int WG, bool ANY, bool F8, bool POST, bool PRE>
@@ -391,8 +392,8 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_kernel(const ResidualNor
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sums[k][i][e] = 0.f;
   // Sums k and k + 1 over the workgroup's rows to `out` and, `set` floats on, to the second one's place; back to zero.
-  auto flush = [&](int k, float* out, int64_t set) {
-    if constexpr (RPW == 1) {
+  auto flush = [&](int k, float* out, int64_t set, bool from_registers) {
+    if (RPW == 1 || from_registers) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int c = Row::col(i, t);
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_kernel(const ResidualNor
           }
         }
       }
-    } else {
+    } else if constexpr (RPW > 1) {
       // The rows of the workgroup hold sums for the same columns: added through LDS, after those that share a wave.
       const int mine = TPR < kWave ? static_cast<int>(threadIdx.x / kWave) : sub;
       __syncthreads();  // (the sums before these have been read)
@@ -460,10 +461,11 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_kernel(const ResidualNor
   const uint32_t piece = blockIdx.x, group = blockIdx.y * gridDim.x + blockIdx.x;
   const int64_t first = static_cast<int64_t>(blockIdx.y) * a.gates_per_group;
   const int64_t last = min(first + a.gates_per_group, a.gates);
-  for (int64_t gate_row = first; gate_row < last; ++gate_row) {
+  const bool own = RPW > 1 && a.own;
+  for (int64_t gate_row = first + (own ? sub : 0); gate_row < last; gate_row += own ? RPW : 1) {
     const int64_t base = gate_row * static_cast<int64_t>(a.gate_rows) + piece * a.piece_start;
     const int64_t end = min((gate_row + 1) * static_cast<int64_t>(a.gate_rows), base + a.piece_span);
-    int64_t row = base + sub;
+    int64_t row = base + (own ? 0 : sub);
 
     Row dx, dh, h, dx_next, dh_next, h_next;
     FRow f, f_next;
@@ -603,10 +605,10 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_kernel(const ResidualNor
       }
     }
     const int64_t item = gate_row * a.pieces + piece;
-    if (POST || a.gate) flush(0, a.gate_sums + item * cols, a.gates * a.pieces * cols);
+    if (POST || a.gate) flush(0, a.gate_sums + item * cols, a.gates * a.pieces * cols, own);
   }
   const int64_t groups = gridDim.x * gridDim.y;
-  if constexpr (PRE) flush(2, a.pre_sums + static_cast<int64_t>(group) * cols, groups * cols);
+  if constexpr (PRE) flush(2, a.pre_sums + static_cast<int64_t>(group) * cols, groups * cols, false);
 }
 
 // The backward of rows that registers do not hold, a workgroup a row: df and dh.  f in the type T.
@@ -690,8 +692,9 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_columns_kernel(const Res
 }
 
 // Stage 2: from the workgroups' column sums to the parameters' gradients, in a fixed order.  A workgroup has 32 columns and
-// 32 lanes for each; blockIdx.y: 0 the gate and the post norm, 1 the pre norm.  The lanes are `split` to a gate row, whose
-// pieces they share, so that many gate rows are walked side by side, and the pieces of one are.
+// 32 lanes for each; blockIdx.y: 0 the gate and the post norm, 1 the pre norm; blockIdx.z: a block of gate rows.  The lanes are
+// `split` to a gate row, whose pieces they share, so that many gate rows are walked side by side, and the pieces of one are; whole
+// gate rows go eight to a lane at once.
 template <typename T>
 __global__ __launch_bounds__(1024) void residual_norm_finish_kernel(const ResidualNormFinish<T> a) {
   __shared__ float tile[2][32][33];
@@ -756,6 +759,7 @@ __global__ __launch_bounds__(1024) void residual_norm_finish_kernel(const Residu
     else static_cast<T*>(out)[at] = from_float<T>(v);
   };
   if (a.first + blockIdx.y == 1) {
+    if (blockIdx.z > 0) return;
     float g, b;
     walk(a.pre_sums + c, a.pre_sums + a.groups * cols + c, ly, a.groups, 32, g, b);
     add_all(g, b);
@@ -770,27 +774,53 @@ __global__ __launch_bounds__(1024) void residual_norm_finish_kernel(const Residu
   const int at_once = 32 / a.split;  // gate rows
   const int64_t second = a.gates * a.pieces * cols;
   float sg = 0.f, sb = 0.f;
-  for (int64_t gate0 = 0; gate0 < a.gates; gate0 += at_once) {
-    const int64_t gate_row = gate0 + ly / a.split;
-    const bool here = gate_row < a.gates;
-    float d, df;
-    const float* const p = a.gate_sums + gate_row * a.pieces * cols + c;
-    walk(p, p + second, ly % a.split, here ? a.pieces : 0, a.split, d, df);
-    if (a.split == 32) add_all(d, df);  // (of the one gate row)
-    else if (a.split > 1) add_lanes(a.split, d, df);
-    if (here && mine && ly % a.split == 0) {
-      float g = 1.f;
-      if (a.gate) {
-        put(a.dgate, gate_row * cols + c, pg * df + pb * d);
-        g = to_float(a.gate[gate_row * cols + c]);
+  const int64_t gate_first = static_cast<int64_t>(blockIdx.z) * a.gates_per_block;
+  const int64_t gate_last = min(gate_first + a.gates_per_block, a.gates);
+  if (a.pieces == 1) {
+    for (int64_t gate0 = gate_first + ly; mine && gate0 < gate_last; gate0 += 8 * 32) {
+      float d[8], df[8], g[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {  // (past the last gate row the last one again, to no effect)
+        const int64_t at = min(gate0 + 32 * k, gate_last - 1) * cols + c;
+        d[k] = a.gate_sums[at];
+        df[k] = a.gate_sums[second + at];
+        g[k] = a.gate ? to_float(a.gate[at]) : 1.f;
       }
-      sg += g * df;
-      sb += g * d;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (gate0 + 32 * k >= gate_last) continue;
+        if (a.gate) put(a.dgate, (gate0 + 32 * k) * cols + c, pg * df[k] + pb * d[k]);
+        sg += g[k] * df[k];
+        sb += g[k] * d[k];
+      }
+    }
+  } else {
+    for (int64_t gate0 = gate_first; gate0 < gate_last; gate0 += at_once) {
+      const int64_t gate_row = gate0 + ly / a.split;
+      const bool here = gate_row < gate_last;
+      float d, df;
+      const float* const p = a.gate_sums + gate_row * a.pieces * cols + c;
+      walk(p, p + second, ly % a.split, here ? a.pieces : 0, a.split, d, df);
+      if (a.split == 32) add_all(d, df);  // (of the one gate row)
+      else if (a.split > 1) add_lanes(a.split, d, df);
+      if (here && mine && ly % a.split == 0) {
+        float g = 1.f;
+        if (a.gate) {
+          put(a.dgate, gate_row * cols + c, pg * df + pb * d);
+          g = to_float(a.gate[gate_row * cols + c]);
+        }
+        sg += g * df;
+        sb += g * d;
+      }
     }
   }
   if (!a.post_gamma) return;
-  if (a.split < 32) add_all(sg, sb);
-  if (ly == 0 && mine) {
+  if (a.split < 32 || a.pieces == 1) add_all(sg, sb);
+  if (ly != 0 || !mine) return;
+  if (a.post_sums) {
+    a.post_sums[blockIdx.z * cols + c] = sg;
+    a.post_sums[(gridDim.z + blockIdx.z) * cols + c] = sb;
+  } else {
     put(a.dpost_gamma, c, sg);
     put(a.dpost_beta, c, sb);
   }
@@ -900,13 +930,17 @@ struct ResidualNormOps {
   // Splits the rows over at most `most` workgroups of `rows_at_once` rows: fewer gate rows than workgroups are cut into
   // pieces, more are dealt out whole.
   static int64_t partition(ResidualNormBwd<T>& a, int64_t most, int rows_at_once, bool interleave) {
+    a.own = 0;
     const int64_t per_gate = std::max<int64_t>(1, std::min(most / a.gates, ceil_div(a.gate_rows, rows_at_once)));
     a.gates_per_group = ceil_div(a.gates, most);
     if (a.gates_per_group > 1 || per_gate == 1) {
       a.pieces = 1;
       a.piece_start = 0;
       a.piece_span = a.gate_rows;
-      a.row_step = rows_at_once;
+      // (us by workgroups | rows in flight, 384 columns of 16384 rows in bf16, a gate row for every 64 rows, which leaves seven of eight
+      // with nothing, 22.9 | 58.4, for every 16, half of them, 28.3 | 27.6, for every 4 50.8 | 34.5, for each 161 | 61)
+      a.own = rows_at_once > 1 && a.gates * (a.gate_rows < rows_at_once ? 8 : 2) >= most * rows_at_once;
+      a.row_step = a.own ? 1 : rows_at_once;
       return ceil_div(a.gates, a.gates_per_group);
     }
     a.gates_per_group = 1;
@@ -922,12 +956,21 @@ struct ResidualNormOps {
   static int take_sums(ResidualNormBwd<T>& a, int64_t groups, Scratch& scratch) {
     const int64_t gate = a.post_gamma || a.gate ? 2 * a.gates * a.pieces * a.cols : 0;
     const int64_t pre = a.pre_gamma ? 2 * groups * a.cols : 0;
+    const int64_t post = a.post_gamma && finish_blocks(a) > 1 ? 2 * finish_blocks(a) * a.cols : 0;
     // (the second array starts where float4s may)
     const int64_t at = ceil_div(gate, 4) * 4;
-    MG_TRY(scratch.take(std::max<int64_t>(1, at + pre) * static_cast<int64_t>(sizeof(float))));
+    MG_TRY(scratch.take(std::max<int64_t>(1, at + pre + post) * static_cast<int64_t>(sizeof(float))));
     a.gate_sums = gate ? scratch.as<float>() : nullptr;
     a.pre_sums = pre ? scratch.as<float>() + at : nullptr;
+    a.post_sums = post ? scratch.as<float>() + at + pre : nullptr;
     return MG_OK;
+  }
+
+  // Blocks of gate rows that the second stage is dealt out in; pieces are summed in one.
+  // (one block: 640 us of (16384, 384) with a gate a token instead of 61)
+  static constexpr int64_t kGatesPerBlock = 256;
+  static int64_t finish_blocks(const ResidualNormBwd<T>& a) {
+    return a.pieces == 1 ? std::min<int64_t>(65535, ceil_div(a.gates, kGatesPerBlock)) : 1;
   }
 
   static int finish(const ResidualNormBwd<T>& a, int64_t groups, void* const (&out)[4], hipStream_t stream) {
@@ -946,14 +989,25 @@ struct ResidualNormOps {
     f.cols = a.cols;
     f.groups = groups;
     f.gates = a.gates;
+    f.gates_per_block = ceil_div(a.gates, finish_blocks(a));
+    f.post_sums = a.post_sums;
     f.pieces = a.pieces;
     f.grad_f32 = a.grad_f32;
     f.split = 32;
     while (f.split > 1 && (32 / f.split) < a.gates) f.split /= 2;
     f.first = a.gate_sums ? 0 : 1;
-    const unsigned jobs = (a.gate_sums ? 1u : 0u) + (a.pre_sums ? 1u : 0u);
-    hipLaunchKernelGGL((residual_norm_finish_kernel<T>), dim3(static_cast<unsigned>(ceil_div(a.cols, 32)), jobs), dim3(1024), 0,
-                       stream, f);
+    const unsigned jobs = (a.gate_sums ? 1u : 0u) + (a.pre_sums ? 1u : 0u), blocks = static_cast<unsigned>(finish_blocks(a));
+    const unsigned columns = static_cast<unsigned>(ceil_div(a.cols, 32));
+    hipLaunchKernelGGL((residual_norm_finish_kernel<T>), dim3(columns, jobs, a.gate_sums ? blocks : 1u), dim3(1024), 0, stream, f);
+    MG_LAUNCH_CHECK();
+    if (!a.post_sums) return MG_OK;
+    // The post norm's gradients from the blocks', as the pre norm's come from the workgroups'.
+    f.pre_sums = a.post_sums;
+    f.groups = blocks;
+    f.dpre_gamma = out[0];
+    f.dpre_beta = out[1];
+    f.first = 1;
+    hipLaunchKernelGGL((residual_norm_finish_kernel<T>), dim3(columns), dim3(1024), 0, stream, f);
     MG_LAUNCH_CHECK();
     return MG_OK;
   }

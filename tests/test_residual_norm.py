@@ -345,6 +345,25 @@ def test_backward(device, rows, cols, gates, post, pre, dtype, grads):
         _check_backward(p, saved, got, dtype, grads, 1.25, **kw)
 
 
+# rows, cols, gates: more gate rows than workgroups, and than rows in flight at once, of every layout
+MANY_GATES = [(9100, 40, 4550), (4400, 200, 2200), (2400, 500, 1200), (2210, 1001, 1105), (1600, 384, 400), (700, 130, 350), (300, 4096, 300),
+              (2100, 3, 2100), (520, 8200, 260)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,grads", [(F32, F32), (F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("rows,cols,gates", MANY_GATES)
+@pytest.mark.parametrize("post,pre", [(1, 1), (0, 1), (1, 0)])
+def test_backward_of_many_gate_rows(device, rows, cols, gates, post, pre, dtype, grads):
+    p = _inputs(36, rows, cols, gates, post, pre, dtype)
+    saved = _saved(p, dtype, 1.25)
+    for kw, run in ((dict(), dict()), (dict(act8=True), dict(offset=1))):
+        got = _backward(device, p, saved, dtype, grads, 1.25, **kw, **run)
+        _check_backward(p, saved, got, dtype, grads, 1.25, **kw)
+        again = _backward(device, p, saved, dtype, grads, 1.25, **kw, **run)
+        assert all(np.array_equal(got[n], again[n]) for n in got)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_first_column_far_from_the_others(device, dtype):
