@@ -22,28 +22,30 @@ int mg_linear_bwd_act8(const void* dy, const void* x8, const void* w, void* dx, 
     return MG_OK;
   }
   MG_TRY(mg::act8_pointer_check(who, x8));
-  mg::CaptureHold hold(s);
-  const int64_t ld = mg::act8_ld(K);
-  const uint8_t* const q = static_cast<const uint8_t*>(x8);
-  bool done = false;
-  MG_TRY(mg::linear_bwd_act8_products(dy, q, q + M * ld, ld, w, dx, dw, db, M, N, K, dx_accumulate != 0, x_is_relu_output != 0, dtype,
-                                      grad_dtype, s, &done));
-  if (done) return MG_OK;
-  mg::Scratch x;
-  MG_TRY(x.take(M * K * static_cast<int64_t>(mg::dtype_size(dtype))));
-  auto run = [&] {
-    return mg::linear_bwd_act8_copied(dy, mg::Act8Restore{x8, x.as<char>()}, w, dx, dw, db, M, N, K, dx_accumulate != 0,
-                                      x_is_relu_output != 0, dtype, s);
-  };
-  if (grad_dtype == dtype) return run();
-  mg::DeferredList list;
-  int rc;
-  {
-    mg::DeferredScope scope(&list, dtype, grad_dtype);
-    rc = run();
-  }
-  const int rc2 = mg_finish_deferred(&list, stream);
-  return rc != MG_OK ? rc : rc2;
+  return mg::without_exceptions(who, [&]() -> int {
+    mg::CaptureHold hold(s);
+    const int64_t ld = mg::act8_ld(K);
+    const uint8_t* const q = static_cast<const uint8_t*>(x8);
+    bool done = false;
+    MG_TRY(mg::linear_bwd_act8_products(dy, q, q + M * ld, ld, w, dx, dw, db, M, N, K, dx_accumulate != 0, x_is_relu_output != 0, dtype,
+                                        grad_dtype, s, &done));
+    if (done) return MG_OK;
+    mg::Scratch x;
+    MG_TRY(x.take(M * K * static_cast<int64_t>(mg::dtype_size(dtype))));
+    auto run = [&] {
+      return mg::linear_bwd_act8_copied(dy, mg::Act8Restore{x8, x.as<char>()}, w, dx, dw, db, M, N, K, dx_accumulate != 0,
+                                        x_is_relu_output != 0, dtype, s);
+    };
+    if (grad_dtype == dtype) return run();
+    mg::DeferredList list;
+    int rc;
+    {
+      mg::DeferredScope scope(&list, dtype, grad_dtype);
+      rc = run();
+    }
+    const int rc2 = mg_finish_deferred(&list, stream);
+    return rc != MG_OK ? rc : rc2;
+  });
 }
 
 }  // extern "C"

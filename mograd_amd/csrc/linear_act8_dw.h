@@ -320,9 +320,9 @@ __global__ __launch_bounds__(256, 2) void linear_act8_f32_kernel(Act8Dw<float> d
   __shared__ __attribute__((aligned(1024))) char lds[LDS];
   if (static_cast<int>(blockIdx.x) >= n_dx) act8_dw_block<float>(lds, blockIdx.x - n_dx, dw);
   else
-    gemm32_pipe_work<true, false, false, false, TS, RELU>(lds, blockIdx.x, n_dx, dx.A, dx.B, nullptr, dx.C, nullptr, dx.M, dx.N, dx.K, dx.lda,
-                                                          dx.ldb, dx.ldc, 0, 0, 0, dx.tiles_m, dx.tiles_n, 1, dx.K, n_dx, dx.ep, dx.mask8,
-                                                          dx.mask8_ld);
+    gemm32_pipe_work<true, false, false, false, TS, RELU>(lds, blockIdx.x, n_dx, dx.A, dx.B, nullptr, dx.C, nullptr, dx.M, dx.N, dx.K,
+                                                          dx.lda, dx.ldb, dx.ldc, 0, 0, 0, dx.tiles_m, dx.tiles_n, 1, dx.K, n_dx, dx.ep,
+                                                          dx.mask8, dx.mask8_ld);
 }
 
 // n_dx == 0: dW alone.

@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
+#include <exception>
 #include <string>
 
 #include "mograd_hip.h"
@@ -74,6 +75,17 @@ class CaptureHold {
   bool on_ = false;
   hipStreamCaptureMode mode_ = hipStreamCaptureModeRelaxed;
 };
+
+// The part of an entry point that allocates host memory (the pool's books, lists of pending sums): what that throws becomes an
+// error code, C callers have no frames for it.
+template <typename F>
+int without_exceptions(const char* who, F&& body) {
+  try {
+    return body();
+  } catch (const std::exception& e) {
+    return fail(MG_ERR_OOM, "%s: host memory: %s", who, e.what());
+  }
+}
 
 // A view of up to kMaxRank dimensions: extents and element strides, passed to kernels by
 // value.

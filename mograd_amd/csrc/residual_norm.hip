@@ -121,7 +121,7 @@ int mg_residual_norm_bwd(const void* dx, const void* dh_out, const void* f, cons
     a.gate_rows = static_cast<uint32_t>(gate ? gate_rows : rows);
     a.gates = rows / a.gate_rows;
     a.scale = residual_scale;
-    return mg::residual_norm_bwd<T>(a, out, dtype, s);
+    return mg::without_exceptions(who, [&] { return mg::residual_norm_bwd<T>(a, out, dtype, s); });
   };
   switch (dtype) {
     case MG_F32: return run(float{});
