@@ -907,23 +907,22 @@ static int linear_bwd_one_launch(const void* dy, const void* x, const void* w, v
 }
 
 // Whether the gradients of a layer whose input is kept in 8 bits come from its bytes (act8_dw_block), or from a restored copy of it
-// by the kernels of any Linear backward.  us by the copy | from the bytes, over 200 layers of 64 to 32768 rows and 64 to 8192 columns:
-//   16 bits: the copy takes 2.5 us and M K 3 bytes at 4.6 TB/s, and dW's tiles from bytes are slower than copied ones, so from 2 million
-//     values on, (16384, 384 <- 1536) 89 | 65, (7421, 80 <- 897) 38.5 | 24.8, (4225, 456 <- 2104) 52 | 42, (4096, 1024 <- 1024) 37 | 32, against
-//     (1135, 408 <- 416) 11.3 | 13.8, (1999, 1001 <- 768) 24.6 | 27.3; up to 180 GFLOP, past which 256 x 256 tiles pay for the
-//     copy: (5772, 3568 <- 1768) 239 | 199, (4515, 3288 <- 3800) 269 | 304, (8192, 4096 <- 4096) 444 | 580.  On average 0.6 % more than the better
-//     one for each, the copy always 9 %, the bytes always 11 %.
-//   fp32: three bf16 products at 16 times the rate of an fp32 one.  With dX in the same launch from 1 GFLOP and 128 columns on, and
-//     from 600 000 values on where they have 256 columns or 0.7 GFLOP: (2048, 512 <- 784) 69 | 43, (1910, 600 <- 632) 72 | 39,
-//     (16384, 1536 <- 384) 422 | 229, (2048, 4096 <- 4096) 1057 | 701, (2945, 56 <- 1064) 45 | 31, against (874, 248 <- 544) 21 | 27,
-//     (1234, 248 <- 136) 14.7 | 23.2, (3094, 996 <- 96) 35 | 44; dW alone from 0.8 GFLOP and 128 columns on: (1910, 601 <- 632) 66 | 45,
-//     against (1202, 629 <- 88) 18.5 | 26, (283, 321 <- 96) 9.4 | 15.
+// by the kernels of any Linear backward.  us by the copy | from the bytes:
+//   16 bits: the copy takes 2.5 us and M K 3 bytes at 4.6 TB/s, and dW's tiles from bytes are slower than copied ones, so from 1.6 million
+//     values and 128 columns on, (16384, 384 <- 1536) 89 | 65, (2863, 192 <- 5908) 76 | 46, (3387, 712 <- 584) 29 | 24, against
+//     (1999, 1001 <- 768) 24.1 | 27.3, (554, 7976 <- 968) 47 | 86, (30224, 80 <- 63) 24 | 57; up to 180 GFLOP, past which 256 x 256 tiles
+//     pay for the copy: (4515, 3288 <- 3800) 269 | 304, (8192, 4096 <- 4096) 444 | 572.  Over 330 layers of 16 to 32768 rows and 32
+//     to 8192 columns 3 % more than the better one for each, the copy always 9 %, the bytes always 14 %.
+//   fp32: three bf16 products at 16 times the rate of an fp32 one.  With dX in the same launch from 0.2 GFLOP on: (2048, 512 <- 784)
+//     69 | 43, (16384, 1536 <- 384) 422 | 229, (2048, 4096 <- 4096) 1057 | 701, against (12982, 96 <- 32) 17 | 27 (1.3 %; the copy always 29 %,
+//     the bytes always 2 %).  dW alone for weights of 400 000 values, and from 1.2 GFLOP and 64 columns on: (24, 4056 <- 3975) 165 | 56,
+//     (457, 7944 <- 109) 116 | 52, (1910, 601 <- 632) 66 | 45, against (233, 768 <- 240) 11 | 23, (4875, 657 <- 48) 28 | 37 (2.8 %, 19 % and 16 %).
 // MOGRAD_HIP_ACT8_ROUTE = 0 (the copy) | 1 (the bytes) overrides the choice.
 static bool act8_from_bytes(int64_t M, int64_t N, int64_t K, bool f32, bool together) {
   const double values = static_cast<double>(M) * static_cast<double>(K), flop = 4.0 * values * static_cast<double>(N);
-  const bool pays = !f32       ? values >= 2e6 && flop <= 1.8e11
-                    : together ? (flop >= 1e9 && K >= 128) || (values >= 6e5 && (K >= 256 || flop >= 7e8))
-                               : flop >= 8e8 && K >= 128;
+  const bool pays = !f32       ? values >= 1.6e6 && K >= 128 && flop <= 1.8e11
+                    : together ? flop >= 2e8
+                               : static_cast<double>(N) * static_cast<double>(K) >= 4e5 || (flop >= 1.2e9 && K >= 64);
   return env_int("MOGRAD_HIP_ACT8_ROUTE", pays) != 0;
 }
 
