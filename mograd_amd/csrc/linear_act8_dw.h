@@ -36,7 +36,7 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
   using S = Act8DwShape<T>;
   using E = typename S::E;
   constexpr int VEC = 16 / sizeof(T), CPR = 128 / VEC;                  // 16-byte chunks of a row of dY
-  constexpr int NA = S::kRows * CPR / 256, NB = S::kRows * 8 / 256;     // 16-byte requests of a thread and step: dY, q
+  constexpr int NA = S::kRows * CPR / 256, NB = S::kRows * 16 / 256;    // requests of a thread and step: 16 bytes of dY, 8 of q
   int tile, split = 0, batch;
   if (p.splits > 1) {
     if (!gemm_split_work(bid, p.tiles_n * p.tiles_k, p.splits, 1, tile, split, batch)) return;
@@ -54,15 +54,16 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
   const bool with_db = p.db_part != nullptr && tk == 0;
 
   struct Staged {
-    uint4 a[NA], b[NB];
+    uint4 a[NA];
+    uint2 b[NB];
     uint32_t e[NB];
   };
   // Requests: byte offsets from a step's first row, which is a scalar.  Columns past an array are read from its last ones: those of
   // dY are put in their places in `put`, and what belongs to no column of the result is not stored.
   const int ac = t % CPR, acol = min(n0 + ac * VEC, p.N - VEC), past = n0 + ac * VEC - acol;
-  const int bcol = min(k0 + t % 8 * 16, static_cast<int>(p.ldx) - 16);
+  const int bcol = min(k0 + t % 16 * 8, static_cast<int>(p.ldx) - 8);
   const uint32_t a_row = static_cast<uint32_t>(p.ldy * sizeof(T)), b_row = static_cast<uint32_t>(p.ldx), e_row = b_row / kAct8Block;
-  const int ar = t / CPR, br = t / 8;  // the thread's first rows of a step
+  const int ar = t / CPR, br = t / 16;  // the thread's first rows of a step
   uint32_t a_at[NA], b_at[NB], e_at[NB];
   auto places = [&](int last) {  // of a step whose last row is `last`: rows past the range repeat it, and become zeros in `put`
 #pragma unroll
@@ -70,7 +71,7 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
       a_at[i] = static_cast<uint32_t>(min(ar + i * (256 / CPR), last)) * a_row + acol * static_cast<int>(sizeof(T));
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const uint32_t row = static_cast<uint32_t>(min(br + i * 32, last));
+      const uint32_t row = static_cast<uint32_t>(min(br + i * 16, last));
       b_at[i] = row * b_row + bcol;
       e_at[i] = row * e_row + bcol / kAct8Block;
     }
@@ -90,7 +91,7 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      r.b[i] = *reinterpret_cast<const uint4*>(b0 + b_at[i]);
+      r.b[i] = *reinterpret_cast<const uint2*>(b0 + b_at[i]);
       r.e[i] = e0[e_at[i]];
     }
   };
@@ -123,7 +124,7 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
         if (ar + i * (256 / CPR) >= left) r.a[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < NB; ++i)
-        if (br + i * 32 >= left) r.b[i] = make_uint4(0, 0, 0, 0), r.e[i] = 7;
+        if (br + i * 16 >= left) r.b[i] = make_uint2(0, 0), r.e[i] = 7;
     }
     if (n0 + 128 > p.N) {
 #pragma unroll
@@ -140,7 +141,7 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
       }
     }
   };
-  // Request i of dY, and half h of the requests of q, into copy `copy` of LDS.  Chunk c of row r stands at c ^ gemm16_tr_swizzle(r).
+  // Request i of dY, and of q, into copy `copy` of LDS.  Chunk c of row r stands at c ^ gemm16_tr_swizzle(r).
   auto put_a = [&](const Staged& r, int i, int copy) {
     char* const at = lds + copy * S::kStep;
     const int row = ar + i * (256 / CPR);
@@ -163,11 +164,10 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
       }
     }
   };
-  auto put_b = [&](const Staged& r, int h, int copy) {
-    const int i = h / 2, row = br + i * 32;
-    const bool upper = (h + row) % 2;  // (odd rows the other way round: sixteen lanes then write to all banks)
+  auto put_b = [&](const Staged& r, int i, int copy) {
+    const int row = br + i * 16, c = t % 16;
     const float scale = act8_scale(r.e[i]);
-    const uint32_t q[2] = {upper ? r.b[i].z : r.b[i].x, upper ? r.b[i].w : r.b[i].y};
+    const uint32_t q[2] = {r.b[i].x, r.b[i].y};
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -176,7 +176,6 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
       w[2 * j] = gemm16_pack2<E>(x[0], x[1]);
       w[2 * j + 1] = gemm16_pack2<E>(x[2], x[3]);
     }
-    const int c = t % 8 * 2 + upper;
     *reinterpret_cast<uint4*>(lds + copy * S::kStep + S::kTerms * S::kImage + row * 256 + (c ^ gemm16_tr_swizzle<128>(row)) * 16) =
         make_uint4(w[0], w[1], w[2], w[3]);
   };
@@ -191,7 +190,7 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
   // Step in `copy` multiplied, the staged one put into the other copy meanwhile: between the matrix instructions of one group,
   // which occupy their pipe for 128 clocks, goes a part of the conversions, and the reads of the next group's fragments before.
   constexpr int GROUPS = S::kRows / 16 * S::kTerms;  // four matrix instructions each: (16 rows, term)
-  static_assert(S::kF32 ? NA + 2 * NB <= GROUPS : NA <= GROUPS && 2 * NB <= GROUPS, "a part of the work to each group");
+  static_assert(S::kF32 ? NA + NB <= GROUPS : NA <= GROUPS && NB <= GROUPS, "a part of the work to each group");
   auto multiply = [&](int copy, const Staged& r) {
     const char* const at = lds + copy * S::kStep;
     uint4 fa[2][2], fb[2][2];
@@ -215,9 +214,9 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
         for (int j = 0; j < 2; ++j) acc[i][j] = GemmMma16<E>::run(fa[g % 2][i], fb[g / S::kTerms % 2][j], acc[i][j]);
       if (g < NA) put_a(r, g, copy ^ 1);
       if constexpr (S::kF32) {
-        if (g >= NA && g - NA < 2 * NB) put_b(r, g - NA, copy ^ 1);
+        if (g >= NA && g - NA < NB) put_b(r, g - NA, copy ^ 1);
       } else {
-        if (g < 2 * NB) put_b(r, g, copy ^ 1);
+        if (g < NB) put_b(r, g, copy ^ 1);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -230,7 +229,7 @@ __device__ __forceinline__ void act8_dw_block(char* lds, int bid, const Act8Dw<T
 #pragma unroll
   for (int i = 0; i < NA; ++i) put_a(r0, i, 0);
 #pragma unroll
-  for (int h = 0; h < 2 * NB; ++h) put_b(r0, h, 0);
+  for (int h = 0; h < NB; ++h) put_b(r0, h, 0);
   request(2, r0);
   __syncthreads();
   // Step s is in copy s % 2; r1, r0 hold steps s + 1 and s + 2 before an even step.  (An odd number of steps ends on one of
