@@ -305,17 +305,15 @@ __global__ __launch_bounds__(WG) void residual_norm_fwd_kernel(const ResidualNor
 }
 
 // Rows of fewer columns than a chunk has, or of more than registers hold: a workgroup a row, which is read again from the
-// caches for every sum.  (Neither is a width that transformers have.)
+// caches for every sum.  (Neither is a width that transformers have.)  Past kWideGroups rows a workgroup takes several: a launch
+// counts its threads in 32 bits.
+constexpr int64_t kWideGroups = 1 << 16;
 template <typename T, int WG>
 __global__ __launch_bounds__(WG) void residual_norm_fwd_wide_kernel(const ResidualNormFwd<T> a) {
   __shared__ float slots[2 * (WG / kWave)];
   int phase = 0;
-  const int64_t row = blockIdx.x;
   const int cols = a.cols;
   const float inv_n = 1.0f / static_cast<float>(cols);
-  const T* const f = a.f + row * cols;
-  const T* const h = a.h + row * cols;
-  const T* const gate = a.gate ? a.gate + static_cast<int64_t>(static_cast<uint32_t>(row) / a.gate_rows) * cols : nullptr;
   auto moments = [&](auto&& value, float& mean, float& rstd) {
     float s[1] = {0.f};
     for (int c = threadIdx.x; c < cols; c += WG) s[0] += value(c);
@@ -331,32 +329,37 @@ __global__ __launch_bounds__(WG) void residual_norm_fwd_wide_kernel(const Residu
     phase ^= 1;
     rstd = rsqrtf(s[0] * inv_n + a.eps);
   };
-  float f_mean = 0.f, f_rstd = 1.f;
-  if (a.post_gamma) {
-    moments([&](int c) { return to_float(f[c]); }, f_mean, f_rstd);
-    if (threadIdx.x == 0) {
-      a.post_mean[row] = f_mean;
-      a.post_rstd[row] = f_rstd;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* const f = a.f + row * cols;
+    const T* const h = a.h + row * cols;
+    const T* const gate = a.gate ? a.gate + static_cast<int64_t>(static_cast<uint32_t>(row) / a.gate_rows) * cols : nullptr;
+    float f_mean = 0.f, f_rstd = 1.f;
+    if (a.post_gamma) {
+      moments([&](int c) { return to_float(f[c]); }, f_mean, f_rstd);
+      if (threadIdx.x == 0) {
+        a.post_mean[row] = f_mean;
+        a.post_rstd[row] = f_rstd;
+      }
     }
-  }
-  auto stream = [&](int c) {
-    float z = to_float(f[c]);
-    if (a.post_gamma) z = (z - f_mean) * f_rstd * to_float(a.post_gamma[c]) + to_float(a.post_beta[c]);
-    if (gate) z *= to_float(gate[c]);
-    return fmaf(a.scale, to_float(h[c]), z);
-  };
-  if (a.pre_gamma) {
-    float mean, rstd;
-    moments(stream, mean, rstd);
-    if (threadIdx.x == 0) {
-      a.pre_mean[row] = mean;
-      a.pre_rstd[row] = rstd;
+    auto stream = [&](int c) {
+      float z = to_float(f[c]);
+      if (a.post_gamma) z = (z - f_mean) * f_rstd * to_float(a.post_gamma[c]) + to_float(a.post_beta[c]);
+      if (gate) z *= to_float(gate[c]);
+      return fmaf(a.scale, to_float(h[c]), z);
+    };
+    if (a.pre_gamma) {
+      float mean, rstd;
+      moments(stream, mean, rstd);
+      if (threadIdx.x == 0) {
+        a.pre_mean[row] = mean;
+        a.pre_rstd[row] = rstd;
+      }
+      for (int c = threadIdx.x; c < cols; c += WG)
+        a.x[row * cols + c] = from_float<T>((stream(c) - mean) * rstd * to_float(a.pre_gamma[c]) + to_float(a.pre_beta[c]));
     }
-    for (int c = threadIdx.x; c < cols; c += WG)
-      a.x[row * cols + c] = from_float<T>((stream(c) - mean) * rstd * to_float(a.pre_gamma[c]) + to_float(a.pre_beta[c]));
+    // (last: h_out may be h, of which each value is read and written by one thread)
+    for (int c = threadIdx.x; c < cols; c += WG) a.h_out[row * cols + c] = from_float<T>(stream(c));
   }
-  // (last: h_out may be h, of which each value is read and written by one thread)
-  for (int c = threadIdx.x; c < cols; c += WG) a.h_out[row * cols + c] = from_float<T>(stream(c));
 }
 
 // ------------------------------------------------------------------------------------
@@ -611,46 +614,49 @@ __global__ __launch_bounds__(WG) void residual_norm_bwd_kernel(const ResidualNor
   if constexpr (PRE) flush(2, a.pre_sums + static_cast<int64_t>(group) * cols, groups * cols, false);
 }
 
-// The backward of rows that registers do not hold, a workgroup a row: df and dh.  f in the type T.
+// The backward of rows that registers do not hold, a workgroup a row at a time: df and dh.  f in the type T.
 template <typename T, int WG>
 __global__ __launch_bounds__(WG) void residual_norm_bwd_wide_kernel(const ResidualNormBwd<T> a) {
   __shared__ float slots[2 * 2 * (WG / kWave)];
   int phase = 0;
-  const int64_t row = blockIdx.x, at = row * a.cols;
   const int cols = a.cols;
   const float inv_n = 1.0f / static_cast<float>(cols);
-  const T* const gate = a.gate ? a.gate + row / a.gate_rows * cols : nullptr;
-  const ResidualNormRow<T> r(a, row);
-  float c[2] = {0.f, 0.f};
-  if (a.pre_gamma) {
-    for (int i = threadIdx.x; i < cols; i += WG) {
-      const float dg = to_float(a.dx[at + i]) * to_float(a.pre_gamma[i]);
-      c[0] += dg;
-      c[1] += dg * r.pre_hat(i);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t at = row * cols;
+    const T* const gate = a.gate ? a.gate + row / a.gate_rows * cols : nullptr;
+    const ResidualNormRow<T> r(a, row);
+    float c[2] = {0.f, 0.f};
+    if (a.pre_gamma) {
+      for (int i = threadIdx.x; i < cols; i += WG) {
+        const float dg = to_float(a.dx[at + i]) * to_float(a.pre_gamma[i]);
+        c[0] += dg;
+        c[1] += dg * r.pre_hat(i);
+      }
+      block_allreduce<SumOp, WG / kWave, 2>(c, slots, phase);
+      phase ^= 1;
     }
-    block_allreduce<SumOp, WG / kWave, 2>(c, slots, phase);
-    phase ^= 1;
-  }
-  const float c0 = c[0] * inv_n, c1 = c[1] * inv_n;
-  float s[2] = {0.f, 0.f};
-  if (a.post_gamma) {
-    for (int i = threadIdx.x; i < cols; i += WG) {
-      const float u = r.stream(i, c0, c1) * (gate ? to_float(gate[i]) : 1.f) * to_float(a.post_gamma[i]);
-      s[0] += u;
-      s[1] += u * r.post_hat(i);
+    const float c0 = c[0] * inv_n, c1 = c[1] * inv_n;
+    float s[2] = {0.f, 0.f};
+    if (a.post_gamma) {
+      for (int i = threadIdx.x; i < cols; i += WG) {
+        const float u = r.stream(i, c0, c1) * (gate ? to_float(gate[i]) : 1.f) * to_float(a.post_gamma[i]);
+        s[0] += u;
+        s[1] += u * r.post_hat(i);
+      }
+      block_allreduce<SumOp, WG / kWave, 2>(s, slots, phase);
+      phase ^= 1;
     }
-    block_allreduce<SumOp, WG / kWave, 2>(s, slots, phase);
-  }
-  if (threadIdx.x == 0) {
-    a.row_sums[2 * row] = c0;
-    a.row_sums[2 * row + 1] = c1;
-  }
-  // dh last: it may be dh_out, of which each value is read and written by one thread ...
-  for (int i = threadIdx.x; i < cols; i += WG) {
-    const float d = r.stream(i, c0, c1);
-    float u = d * (gate ? to_float(gate[i]) : 1.f);
-    if (a.post_gamma) u = r.post_rstd * (u * to_float(a.post_gamma[i]) - s[0] * inv_n - r.post_hat(i) * (s[1] * inv_n));
-    a.df[at + i] = from_float<T>(u);
+    if (threadIdx.x == 0) {
+      a.row_sums[2 * row] = c0;
+      a.row_sums[2 * row + 1] = c1;
+    }
+    // dh last: it may be dh_out, of which each value is read and written by one thread ...
+    for (int i = threadIdx.x; i < cols; i += WG) {
+      const float d = r.stream(i, c0, c1);
+      float u = d * (gate ? to_float(gate[i]) : 1.f);
+      if (a.post_gamma) u = r.post_rstd * (u * to_float(a.post_gamma[i]) - s[0] * inv_n - r.post_hat(i) * (s[1] * inv_n));
+      a.df[at + i] = from_float<T>(u);
+    }
   }
 }
 
@@ -921,7 +927,8 @@ struct ResidualNormOps {
       return dispatch_fwd<true>(s, a, stream);
     }
     if (a.f8) MG_TRY(act8_store(a.f, a.f8, a.rows, a.cols, false, dtype, stream));
-    hipLaunchKernelGGL((residual_norm_fwd_wide_kernel<T, 1024>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((residual_norm_fwd_wide_kernel<T, 1024>), dim3(static_cast<unsigned>(std::min(a.rows, kWideGroups))), dim3(1024), 0,
+                       stream, a);
     MG_LAUNCH_CHECK();
     if (a.x8) MG_TRY(act8_store(a.x, a.x8, a.rows, a.cols, false, dtype, stream));
     return MG_OK;
@@ -1062,7 +1069,8 @@ struct ResidualNormOps {
     }
     MG_TRY(sums.take(2 * a.rows * static_cast<int64_t>(sizeof(float))));
     a.row_sums = sums.as<float>();
-    hipLaunchKernelGGL((residual_norm_bwd_wide_kernel<T, 1024>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((residual_norm_bwd_wide_kernel<T, 1024>), dim3(static_cast<unsigned>(std::min(a.rows, kWideGroups))), dim3(1024), 0,
+                       stream, a);
     MG_LAUNCH_CHECK();
     const int64_t blocks = ceil_div(a.cols, 256);
     const int64_t most = std::max<int64_t>(1, ceil_div(static_cast<int64_t>(device_info().cu_count) * 4, blocks));

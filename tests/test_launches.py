@@ -1,0 +1,83 @@
+"""What the library asks of the HIP runtime, without a GPU: its host code runs over tests/host_cpp/stub_hip.cpp, in a process of its
+own, which writes launches down and refuses those of 2^32 threads along an axis, as the runtime does."""
+import json
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
+
+PRELUDE = """
+import ctypes as C, json, sys
+sys.path.insert(0, sys.argv[2])
+stub = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)  # before the library, whose calls it takes
+stub.stub_launches.restype = stub.stub_mallocs.restype = C.c_int64
+stub.stub_launches.argtypes = [C.c_char_p, C.c_int64]
+stub.stub_capture.argtypes = [C.c_ulonglong]
+import mograd_amd
+from mograd_amd import BF16, F16, F32, MogradError
+lib = mograd_amd.load()
+p, p16 = C.c_void_p(1 << 20), C.c_void_p((1 << 20) + 2)
+
+def launches():
+    n = stub.stub_launches(None, 0)
+    text = C.create_string_buffer(n + 1)
+    stub.stub_launches(text, n + 1)
+    stub.stub_reset()
+    return [list(map(int, line.split())) for line in text.value.decode().splitlines()]
+
+def norm_fwd(rows, cols, gate_rows=1, dtype=BF16, post=True, pre=True, keep=None, stream=None):
+    o, n = (p if post else None), (p if pre else None)
+    lib.mg_residual_norm_fwd(p, p, p, o, o, n, n, p, n, o, o, n, n, keep, keep, rows, cols, gate_rows, 1.0, 1e-5, dtype, stream)
+
+def norm_bwd(rows, cols, gate_rows=1, dtype=BF16, post=True, pre=True, f8=False, stream=None):
+    o, n = (p if post else None), (p if pre else None)
+    lib.mg_residual_norm_bwd(n, p, None if f8 else p, p if f8 else None, p, p, o, o, n, o, o, n, n, p, p, p, o, o, n, n, rows, cols,
+                             gate_rows, 1.0, dtype, F32, stream)
+
+def linear(M, N, K, dtype=BF16, dx=True, relu=1, stream=None):
+    lib.mg_linear_bwd_act8(p, p, p, p if dx else None, p, p, M, N, K, 0, relu, dtype, F32, stream)
+
+out = []
+"""
+
+
+@pytest.fixture(scope="module")
+def stub_hip(tmp_path_factory):
+    out = tmp_path_factory.mktemp("stub") / "libstub_hip.so"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    str(ROOT / "tests" / "host_cpp" / "stub_hip.cpp"), "-o", str(out)], check=True)
+    return out
+
+
+@pytest.fixture
+def over_stub(stub_hip):
+    def run(code):
+        """`code` over the stub; what it puts into `out`."""
+        child = subprocess.run([sys.executable, "-c", PRELUDE + code + "\nprint(json.dumps(out))", str(stub_hip), str(ROOT)],
+                               capture_output=True, text=True, timeout=300)
+        assert child.returncode == 0, child.stderr[-2000:]
+        return json.loads(child.stdout.splitlines()[-1])
+
+    return run
+
+
+def test_the_stub_takes_the_calls(over_stub):
+    got = over_stub("norm_fwd(128, 64); out = launches()")
+    assert len(got) == 1 and got[0][3:6] == [256, 1, 1]
+
+
+def test_residual_norm_of_many_narrow_or_wide_rows(over_stub):
+    """Fewer columns than a chunk, or more than registers hold, where a workgroup has a row at a time: any number of rows."""
+    got = over_stub("""
+for rows in (3, 1 << 22, (1 << 31) - 1):
+    for cols, dtype in ((7, BF16), (1, F32), (3, F16), (20001, BF16)):
+        for keep in (None, p):
+            if rows * cols < 1 << 34:
+                norm_fwd(rows, cols, rows, dtype, keep=keep if rows < 1 << 23 else None)
+                norm_bwd(rows, cols, rows, dtype)
+                out.append(len(launches()))
+""")
+    assert got and min(got) >= 3
