@@ -73,6 +73,7 @@ struct ResidualNormFinish {
   void *dgate, *dpost_gamma, *dpost_beta, *dpre_gamma, *dpre_beta;
   float* post_sums;  // of many gate rows, [2][gridDim.z][cols]: the post norm's gradients over gates_per_block each; or null
   int64_t cols, groups, gates, gates_per_block, pieces;
+  int64_t first_column;  // of the launch's columns
   int split;  // lanes to a gate row: a power of two, 1 .. 32
   int first;  // the first workgroups' job: 0 the gate and the post norm, 1 the pre norm
   int grad_f32;

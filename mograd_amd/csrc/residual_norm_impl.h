@@ -705,7 +705,7 @@ template <typename T>
 __global__ __launch_bounds__(1024) void residual_norm_finish_kernel(const ResidualNormFinish<T> a) {
   __shared__ float tile[2][32][33];
   const int cx = threadIdx.x % 32, ly = threadIdx.x / 32;
-  const int64_t cols = a.cols, c = static_cast<int64_t>(blockIdx.x) * 32 + cx;
+  const int64_t cols = a.cols, c = a.first_column + static_cast<int64_t>(blockIdx.x) * 32 + cx;
   const bool mine = c < cols;
   // The sums of two arrays' rows first, first + step, ...: eight loads on their way at once, those past the end repeating the
   // last row, to no effect.
@@ -1004,9 +1004,8 @@ struct ResidualNormOps {
     while (f.split > 1 && (32 / f.split) < a.gates) f.split /= 2;
     f.first = a.gate_sums ? 0 : 1;
     const unsigned jobs = (a.gate_sums ? 1u : 0u) + (a.pre_sums ? 1u : 0u), blocks = static_cast<unsigned>(finish_blocks(a));
-    const unsigned columns = static_cast<unsigned>(ceil_div(a.cols, 32));
-    hipLaunchKernelGGL((residual_norm_finish_kernel<T>), dim3(columns, jobs, a.gate_sums ? blocks : 1u), dim3(1024), 0, stream, f);
-    MG_LAUNCH_CHECK();
+    const dim3 both(1, jobs, a.gate_sums ? blocks : 1u);
+    MG_TRY(launch_finish(f, both, stream));
     if (!a.post_sums) return MG_OK;
     // The post norm's gradients from the blocks', as the pre norm's come from the workgroups'.
     f.pre_sums = a.post_sums;
@@ -1014,8 +1013,16 @@ struct ResidualNormOps {
     f.dpre_gamma = out[0];
     f.dpre_beta = out[1];
     f.first = 1;
-    hipLaunchKernelGGL((residual_norm_finish_kernel<T>), dim3(columns), dim3(1024), 0, stream, f);
-    MG_LAUNCH_CHECK();
+    return launch_finish(f, dim3(1), stream);
+  }
+  // A workgroup of 1024 threads for 32 columns.  A launch counts its threads in 32 bits, so 2^25 columns a launch.
+  static int launch_finish(ResidualNormFinish<T> f, dim3 grid, hipStream_t stream) {
+    constexpr int64_t kColumns = 1 << 25;
+    for (f.first_column = 0; f.first_column < f.cols; f.first_column += kColumns) {
+      grid.x = static_cast<unsigned>(ceil_div(std::min(f.cols - f.first_column, kColumns), 32));
+      hipLaunchKernelGGL((residual_norm_finish_kernel<T>), grid, dim3(1024), 0, stream, f);
+      MG_LAUNCH_CHECK();
+    }
     return MG_OK;
   }
 

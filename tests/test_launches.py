@@ -81,3 +81,16 @@ for rows in (3, 1 << 22, (1 << 31) - 1):
                 out.append(len(launches()))
 """)
     assert got and min(got) >= 3
+
+
+def test_residual_norm_backward_of_the_widest_rows(over_stub):
+    """The second stage has 1024 threads for 32 columns; every column of 2^30 - 1 is covered."""
+    got = over_stub("""
+for cols in (20001, (1 << 27) - 1, 1 << 27, (1 << 30) - 1):
+    for post, pre in ((True, True), (False, True)):
+        norm_bwd(2, cols, 1, BF16, post, pre)
+        stage2 = [l for l in launches() if l[3] == 1024][1:]  # (the first has the rows)
+        out.append((cols, sum(l[0] for l in stage2)))
+""")
+    for cols, groups in got:
+        assert groups == -(-cols // 32), cols
