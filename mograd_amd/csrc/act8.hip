@@ -12,9 +12,9 @@ namespace mg {
 template <typename T, bool ANY, typename Index, int COUNT>
 __global__ __launch_bounds__(kAct8Threads) void act8_store_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                                   uint8_t* __restrict__ exponents, int64_t chunks, int cols,
-                                                                  uint32_t chunks_per_row, int keep_sign) {
+                                                                  uint32_t chunks_per_row, int keep_sign, int64_t first_block) {
   constexpr int VEC = WideVec<T>::value, LANES = kAct8Block / VEC;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kAct8Threads * COUNT) + threadIdx.x;
+  const int64_t first = (first_block + blockIdx.x) * (kAct8Threads * COUNT) + threadIdx.x;
   float v[COUNT][VEC];
 #pragma unroll
   for (int k = 0; k < COUNT; ++k) {
@@ -59,8 +59,9 @@ __global__ __launch_bounds__(kAct8Threads) void act8_store_kernel(const T* __res
 template <typename T, bool ANY, typename Index, int COUNT>
 __global__ __launch_bounds__(kAct8Threads) void act8_load_kernel(const uint8_t* __restrict__ q,
                                                                  const uint8_t* __restrict__ exponents, T* __restrict__ x,
-                                                                 int64_t chunks, int cols, uint32_t chunks_per_row) {
-  act8_load_chunks<T, ANY, Index, COUNT>(blockIdx.x, q, exponents, x, chunks, cols, chunks_per_row);
+                                                                 int64_t chunks, int cols, uint32_t chunks_per_row,
+                                                                 int64_t first_block) {
+  act8_load_chunks<T, ANY, Index, COUNT>(first_block + blockIdx.x, q, exponents, x, chunks, cols, chunks_per_row);
 }
 
 // Every 16-byte chunk of x lies on 16 bytes.
@@ -69,33 +70,39 @@ static bool act8_aligned(const void* x, int64_t cols) {
   return cols % WideVec<T>::value == 0 && aligned16(x);
 }
 
-// Calls `launch(kernel choice, workgroups)` with what the sizes ask for: chunks at any address or on 16 bytes, 32- or 64-bit division,
-// one chunk a thread or four.
+// Calls `launch(kernel choice, first workgroup, workgroups)` with what the sizes ask for: chunks at any address or on 16 bytes, 32- or
+// 64-bit division, one chunk a thread or four.  A launch counts its threads in 32 bits: 2^23 workgroups of 256 each time.
 template <typename T, typename F>
 static int act8_launch(const void* x, int64_t chunks, int64_t cols, F&& launch) {
+  auto counted = [&](auto any, auto index, auto count) -> int {
+    constexpr int64_t kBlocks = 1 << 23;
+    const int64_t blocks = ceil_div(chunks, decltype(count)::value * kAct8Threads);
+    for (int64_t first = 0; first < blocks; first += kBlocks) {
+      launch(any, index, count, first, std::min(blocks - first, kBlocks));
+      MG_LAUNCH_CHECK();
+    }
+    return MG_OK;
+  };
   auto indexed = [&](auto any, auto index) {
-    if (chunks >= act8_many_chunks())
-      launch(any, index, std::integral_constant<int, 4>{}, ceil_div(chunks, 4 * kAct8Threads));
-    else launch(any, index, std::integral_constant<int, 1>{}, ceil_div(chunks, kAct8Threads));
+    if (chunks >= act8_many_chunks()) return counted(any, index, std::integral_constant<int, 4>{});
+    return counted(any, index, std::integral_constant<int, 1>{});
   };
   auto aligned = [&](auto any) {
-    if (chunks <= 0x7fffffffLL) indexed(any, uint32_t{});
-    else indexed(any, uint64_t{});
+    if (chunks <= 0x7fffffffLL) return indexed(any, uint32_t{});
+    return indexed(any, uint64_t{});
   };
-  if (act8_aligned<T>(x, cols)) aligned(std::false_type{});
-  else aligned(std::true_type{});
-  MG_LAUNCH_CHECK();
-  return MG_OK;
+  if (act8_aligned<T>(x, cols)) return aligned(std::false_type{});
+  return aligned(std::true_type{});
 }
 
 template <typename T>
 static int act8_store_typed(const void* x, void* act8, int64_t rows, int64_t cols, bool keep_sign, hipStream_t stream) {
   const int64_t ld = act8_ld(cols), per_row = ld / WideVec<T>::value, chunks = rows * per_row;
   uint8_t* const q = static_cast<uint8_t*>(act8);
-  return act8_launch<T>(x, chunks, cols, [&](auto any, auto index, auto count, int64_t blocks) {
+  return act8_launch<T>(x, chunks, cols, [&](auto any, auto index, auto count, int64_t first, int64_t blocks) {
     hipLaunchKernelGGL((act8_store_kernel<T, decltype(any)::value, decltype(index), decltype(count)::value>),
                        dim3(static_cast<unsigned>(blocks)), dim3(kAct8Threads), 0, stream, static_cast<const T*>(x), q,
-                       q + rows * ld, chunks, static_cast<int>(cols), static_cast<uint32_t>(per_row), keep_sign ? 1 : 0);
+                       q + rows * ld, chunks, static_cast<int>(cols), static_cast<uint32_t>(per_row), keep_sign ? 1 : 0, first);
   });
 }
 
@@ -103,14 +110,14 @@ template <typename T>
 static int act8_load_typed(const void* act8, void* x, int64_t rows, int64_t cols, hipStream_t stream) {
   const int64_t ld = act8_ld(cols), per_row = ld / WideVec<T>::value, chunks = rows * per_row;
   const uint8_t* const q = static_cast<const uint8_t*>(act8);
-  return act8_launch<T>(x, chunks, cols, [&](auto any, auto index, auto count, int64_t blocks) {
+  return act8_launch<T>(x, chunks, cols, [&](auto any, auto index, auto count, int64_t first, int64_t blocks) {
     hipLaunchKernelGGL((act8_load_kernel<T, decltype(any)::value, decltype(index), decltype(count)::value>),
                        dim3(static_cast<unsigned>(blocks)), dim3(kAct8Threads), 0, stream, q, q + rows * ld,
-                       static_cast<T*>(x), chunks, static_cast<int>(cols), static_cast<uint32_t>(per_row));
+                       static_cast<T*>(x), chunks, static_cast<int>(cols), static_cast<uint32_t>(per_row), first);
   });
 }
 
-// Rows and columns that the format's index arithmetic takes: 2^31 - 1 workgroups.
+// Rows and columns that the index arithmetic takes: both in 32 bits, the bytes of q in 40.
 int act8_check(const char* who, int64_t rows, int64_t cols, int dtype) {
   if (!is_float_dtype(dtype)) return fail(MG_ERR_INVALID, "%s: unsupported dtype %s", who, dtype_name(dtype));
   if (rows < 0 || cols <= 0 || cols > 0x3fffffffLL || rows > 0x7fffffffLL ||

@@ -94,3 +94,18 @@ for cols in (20001, (1 << 27) - 1, 1 << 27, (1 << 30) - 1):
 """)
     for cols, groups in got:
         assert groups == -(-cols // 32), cols
+
+
+def test_act8_of_more_chunks_than_a_launch_counts(over_stub):
+    """(2^31 - 1, 1): 2^31 - 1 blocks of 32, four threads' worth or eight each. Every chunk of 16 bytes has its thread."""
+    got = over_stub("""
+for rows, cols in ((5, 40), ((1 << 29) - 1, 1), ((1 << 31) - 1, 1), ((1 << 31) - 1, 512), (1 << 20, 1 << 20)):
+    for dtype in (F32, BF16):
+        chunks = rows * -(-cols // 32) * (8 if dtype == F32 else 4)
+        each = 4 if chunks >= 1 << 20 else 1
+        for call in (lib.mg_act8_store, lib.mg_act8_load):
+            call(p, p, rows, cols, *([0] if call is lib.mg_act8_store else []), dtype, None)
+            out.append((rows, cols, chunks, each * sum(l[0] * l[3] for l in launches())))
+""")
+    for rows, cols, chunks, places in got:
+        assert 0 <= places - chunks < 4 * 256, (rows, cols)
