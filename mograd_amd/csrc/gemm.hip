@@ -164,7 +164,8 @@ struct PadCopies {
   int launch(const Act8Restore& in, int64_t rows, int64_t cols, bool copies_it, int dtype, hipStream_t stream) {
     const int64_t ld = act8_ld(cols), per_row = ld / WideVec<T>::value, chunks = rows * per_row;
     const int64_t restoring = ceil_div(chunks, kAct8Threads);
-    if (count == 0 || copies_it || cols % WideVec<T>::value != 0 || chunks >= act8_many_chunks() || blocks + restoring > 0x7fffffffLL) {
+    if (count == 0 || copies_it || cols % WideVec<T>::value != 0 || chunks >= act8_many_chunks() ||
+        blocks + restoring > 0xffffffffLL / 256) {
       MG_TRY(act8_load(in.act8, in.x, rows, cols, dtype, stream));
       return launch(stream);
     }
@@ -930,9 +931,10 @@ static bool act8_from_bytes(int64_t M, int64_t N, int64_t K, bool f32, bool toge
 // second CU at least; tiles of 128 from four for every five CUs on, unless their last round is the emptier one by more than the rest of the
 // launch fills.  us by 64 | 128: (5727, 164 <- 1024) 64 | 57, (16384, 1536 <- 384) 244 | 229, (2048, 4096 <- 4096) 761 | 701, against
 // (18195, 1088 <- 192) 134 | 165, (7341, 248 <- 536) 59 | 69, (1024, 1024 <- 1024) 40 | 93.  MOGRAD_HIP_ACT8_XTILE = 0 | 64 | 128 overrides it.
+// A launch counts its threads in 32 bits, so past 2^23 tiles dX has its own, whose workgroups take several.
 static int act8_f32_dx_tile(const void* dy, const void* w, int64_t M, int64_t N, int64_t K) {
   const int64_t cus = device_info().cu_count, blocks128 = ceil_div(M, 128) * ceil_div(K, 128), blocks64 = ceil_div(M, 64) * ceil_div(K, 64);
-  if (!mult4(N) || !mult4(K) || !aligned16(dy) || !aligned16(w) || N < 32 || 2 * blocks64 < cus) return 0;
+  if (!mult4(N) || !mult4(K) || !aligned16(dy) || !aligned16(w) || N < 32 || 2 * blocks64 < cus || blocks64 > 1 << 23) return 0;
   if (env_str("MOGRAD_HIP_ACT8_XTILE")) {
     const int only = env_int("MOGRAD_HIP_ACT8_XTILE", 0);
     return only == 64 || only == 128 ? only : 0;

@@ -327,7 +327,7 @@ __global__ __launch_bounds__(256, 2) void linear_act8_f32_kernel(Act8Dw<float> d
 // n_dx == 0: dW alone.
 template <typename T>
 int launch_linear_act8(const Act8Dw<T>& dw, const Gemm16Problem<T>* dx, int x_tile, int64_t n_dw, int64_t n_dx, hipStream_t stream) {
-  if (n_dw + n_dx > 0x7fffffffLL) return fail(MG_ERR_INVALID, "linear_bwd_act8: too many output tiles");
+  if (n_dw + n_dx > 0xffffffffLL / 256) return fail(MG_ERR_INVALID, "linear_bwd_act8: too many output tiles");
   if (n_dx == 0) {
     hipLaunchKernelGGL((act8_dw_kernel<T>), dim3(static_cast<unsigned>(n_dw)), dim3(256), 0, stream, dw);
   } else {

@@ -109,3 +109,14 @@ for rows, cols in ((5, 40), ((1 << 29) - 1, 1), ((1 << 31) - 1, 1), ((1 << 31) -
 """)
     for rows, cols, chunks, places in got:
         assert 0 <= places - chunks < 4 * 256, (rows, cols)
+
+
+def test_act8_linear_of_more_tiles_than_a_launch_counts(over_stub):
+    """fp32 dX in tiles of 64 rows beside dW: 2^24 of them are 2^32 threads."""
+    got = over_stub("""
+for M in (1 << 20, (1 << 30) - 64, 1 << 30, 0x7f000000):
+    for N, K in ((32, 4), (32, 32), (64, 64)):
+        linear(M, N, K, F32)
+        out.append(len(launches()))
+""")
+    assert got and min(got) >= 1
