@@ -23,7 +23,8 @@ int mg_linear_bwd_act8(const void* dy, const void* x8, const void* w, void* dx, 
   }
   MG_TRY(mg::act8_pointer_check(who, x8));
   return mg::without_exceptions(who, [&]() -> int {
-    mg::CaptureHold hold(s);
+    mg::CaptureHold hold;
+    MG_TRY(hold.begin(s));
     const int64_t ld = mg::act8_ld(K);
     const uint8_t* const q = static_cast<const uint8_t*>(x8);
     bool done = false;

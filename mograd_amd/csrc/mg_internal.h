@@ -66,8 +66,9 @@ class Scratch {
 // the midst of the capture.  (No effect on other streams.)
 class CaptureHold {
  public:
-  explicit CaptureHold(hipStream_t stream);
+  CaptureHold() = default;
   ~CaptureHold();
+  int begin(hipStream_t stream);  // before anything is taken or launched; an error code where it cannot be kept
   CaptureHold(const CaptureHold&) = delete;
   CaptureHold& operator=(const CaptureHold&) = delete;
 

@@ -93,7 +93,8 @@ int mg_residual_norm_bwd(const void* dx, const void* dh_out, const void* f, cons
     MG_TRY(mg::act8_check(who, rows, cols, dtype));
     MG_TRY(mg::act8_pointer_check(who, f8));
   }
-  mg::CaptureHold hold(s);
+  mg::CaptureHold hold;
+  MG_TRY(hold.begin(s));
   void* const out[4] = {dpost_gamma, dpost_beta, dpre_gamma, dpre_beta};
   auto run = [&](auto zero) {
     using T = decltype(zero);

@@ -160,16 +160,20 @@ static std::string summary_locked(Pool& pool) {
 // Set while a CaptureHold of this thread is in force: what is released stays taken.
 static thread_local bool t_hold_released = false;
 
-CaptureHold::CaptureHold(hipStream_t stream) {
+int CaptureHold::begin(hipStream_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (stream == nullptr || t_hold_released) return;  // (the default stream cannot be captured)
-  if (hipStreamIsCapturing(stream, &status) != hipSuccess) {
+  if (stream == nullptr || t_hold_released) return MG_OK;  // (the default stream cannot be captured)
+  if (const hipError_t e = hipStreamIsCapturing(stream, &status); e != hipSuccess) {
     (void)hipGetLastError();
-    return;
+    return fail(MG_ERR_HIP, "whether the stream is captured is not known: %s", hipGetErrorString(e));
   }
-  if (status != hipStreamCaptureStatusActive) return;
-  on_ = hipThreadExchangeStreamCaptureMode(&mode_) == hipSuccess;
-  t_hold_released = on_;
+  if (status != hipStreamCaptureStatusActive) return MG_OK;
+  if (const hipError_t e = hipThreadExchangeStreamCaptureMode(&mode_); e != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(MG_ERR_HIP, "scratch cannot be kept for the graph: %s", hipGetErrorString(e));
+  }
+  on_ = t_hold_released = true;
+  return MG_OK;
 }
 
 CaptureHold::~CaptureHold() {

@@ -120,3 +120,26 @@ for M in (1 << 20, (1 << 30) - 64, 1 << 30, 0x7f000000):
         out.append(len(launches()))
 """)
     assert got and min(got) >= 1
+
+
+def test_a_recorded_call_that_cannot_keep_its_scratch_is_refused(over_stub):
+    """Scratch is kept for the graph under a capture mode of the call's own; without it nothing is taken and nothing launched."""
+    got = over_stub("""
+stream = C.c_void_p(1 << 16)
+stub.stub_capture(7)
+norm_bwd(64, 64, 64, stream=stream)
+linear(64, 64, 64, stream=stream)
+launches()
+took = stub.stub_mallocs()
+stub.stub_exchange_fails(1)
+for call in (lambda: norm_bwd(512, 640, 512, stream=stream), lambda: linear(1024, 640, 512, stream=stream)):
+    try:
+        call()
+        out.append(0)
+    except MogradError as e:
+        out.append(e.status)
+out += [len(launches()), stub.stub_mallocs() - took]
+norm_bwd(64, 64, 64)  # (the default stream is never captured)
+out.append(len(launches()))
+""")
+    assert got[:4] == [3, 3, 0, 0] and got[4] > 0
