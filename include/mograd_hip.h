@@ -132,6 +132,11 @@ int mg_pool_free(void* ptr);
  * (memory.mojo:353-362). */
 int mg_pool_empty_cache(void);
 
+/* Returns the scratch that recorded calls keep (mg_residual_norm_bwd and mg_linear_bwd_act8, see there) to the free lists of the
+ * current device's pool.  For a program that has destroyed its graphs of such calls, and is capturing none.  No counterpart in the
+ * reference. */
+int mg_pool_free_recorded(void);
+
 /* memory_stats, memory.mojo:377-382. */
 int mg_pool_get_stats(mg_pool_stats* out);
 
@@ -598,7 +603,8 @@ int mg_residual_norm_bwd(const void* dx, const void* dh_out, const void* f, cons
                          int64_t gate_rows, float residual_scale, int dtype, int grad_dtype, mg_stream stream);
 
 /* mg_linear_bwd_act8 and mg_residual_norm_bwd take scratch from the pool.  Recorded into a HIP graph they keep it: what such a
- * call took is in no later call's hands for as long as the process runs, so graphs and eager calls never share it. */
+ * call took goes only to calls that are recorded on the same stream in the same capture, so that graphs, the branches of a graph, and
+ * eager calls never share it.  It stays so, also where the capture fails, until mg_pool_free_recorded. */
 
 #ifdef __cplusplus
 }

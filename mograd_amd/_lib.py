@@ -78,6 +78,7 @@ PROTOTYPES = {
     "mg_pool_alloc": (_i, [C.POINTER(_p), _l], True),
     "mg_pool_free": (_i, [_p], True),
     "mg_pool_empty_cache": (_i, [], True),
+    "mg_pool_free_recorded": (_i, [], True),
     "mg_pool_get_stats": (_i, [C.POINTER(PoolStats)], True),
     "mg_pool_summary": (_l, [C.c_char_p, _l], False),
     "mg_layer_norm_fwd": (_i, [_p, _p, _p, _p, _l, _l, _f, _i, _p], True),

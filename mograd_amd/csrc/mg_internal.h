@@ -61,9 +61,10 @@ class Scratch {
   void* ptr_ = nullptr;
 };
 
-// For the length of an entry point's call on a stream that is being captured into a graph: what the call takes from the pool is
-// never handed to another call, since every replay of the graph writes it again, and the pool may ask the driver for memory in
-// the midst of the capture.  (No effect on other streams.)
+// For the length of an entry point's call on a stream that is being captured into a graph: what the call takes from the pool goes
+// only to calls that are recorded on the same stream in the same capture, which run behind it in every replay, since every replay
+// writes it again; mg_pool_free_recorded ends that.  The pool may ask the driver for memory in the midst of the capture.  (No effect
+// on other streams.)
 class CaptureHold {
  public:
   CaptureHold() = default;

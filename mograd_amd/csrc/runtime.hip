@@ -1,6 +1,7 @@
 // Library plumbing: error state, device properties, streams and the caching pool.
 #include <cstdlib>
 #include <cstring>
+#include <map>
 #include <mutex>
 #include <unordered_map>
 #include <vector>
@@ -85,8 +86,12 @@ static int64_t round_class(int64_t nbytes) {
   return ((nbytes + step - 1) / step) * step;
 }
 
+using FreeLists = std::unordered_map<int64_t, std::vector<void*>>;  // by the value in Pool::live
+using Recording = std::pair<unsigned long long, hipStream_t>;        // a capture's id, and one of its streams
+
 struct Pool {
-  std::unordered_map<int64_t, std::vector<void*>> free_lists;
+  FreeLists free_lists;
+  std::map<Recording, FreeLists> recorded;  // (the blocks are still in `live`)
   std::unordered_map<void*, int64_t> live;  // ptr -> class bytes (pooled) or -nbytes (unpooled)
   mg_pool_stats stats{};
 };
@@ -157,13 +162,15 @@ static std::string summary_locked(Pool& pool) {
   return out;
 }
 
-// Set while a CaptureHold of this thread is in force: what is released stays taken.
-static thread_local bool t_hold_released = false;
+// What a CaptureHold of this thread is for, while one is in force.
+static thread_local bool t_holding = false;
+static thread_local Recording t_recording;
 
 int CaptureHold::begin(hipStream_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (stream == nullptr || t_hold_released) return MG_OK;  // (the default stream cannot be captured)
-  if (const hipError_t e = hipStreamIsCapturing(stream, &status); e != hipSuccess) {
+  unsigned long long id = 0;
+  if (stream == nullptr || t_holding) return MG_OK;  // (the default stream cannot be captured)
+  if (const hipError_t e = hipStreamGetCaptureInfo(stream, &status, &id); e != hipSuccess) {
     (void)hipGetLastError();
     return fail(MG_ERR_HIP, "whether the stream is captured is not known: %s", hipGetErrorString(e));
   }
@@ -172,13 +179,14 @@ int CaptureHold::begin(hipStream_t stream) {
     (void)hipGetLastError();
     return fail(MG_ERR_HIP, "scratch cannot be kept for the graph: %s", hipGetErrorString(e));
   }
-  on_ = t_hold_released = true;
+  on_ = t_holding = true;
+  t_recording = {id, stream};
   return MG_OK;
 }
 
 CaptureHold::~CaptureHold() {
   if (!on_) return;
-  t_hold_released = false;
+  t_holding = false;
   (void)hipThreadExchangeStreamCaptureMode(&mode_);
 }
 
@@ -188,19 +196,28 @@ int pool_take(void** out, int64_t nbytes) {
   *out = nullptr;
   std::lock_guard<std::mutex> lock(g_pool_mu);
   Pool& pool = current_pool();
-  if (!pool_enabled_env()) {
+  const int64_t cls = pool_enabled_env() ? round_class(nbytes) : -std::max<int64_t>(nbytes, 1);
+  if (t_holding) {
+    if (auto rec = pool.recorded.find(t_recording); rec != pool.recorded.end()) {
+      if (auto it = rec->second.find(cls); it != rec->second.end() && !it->second.empty()) {
+        *out = it->second.back();
+        it->second.pop_back();
+        return MG_OK;
+      }
+    }
+  }
+  if (cls < 0) {
     void* p = nullptr;
-    int64_t n = nbytes > 0 ? nbytes : 1;
+    const int64_t n = -cls;
     hipError_t e = hipMalloc(&p, static_cast<size_t>(n));
     if (e != hipSuccess) {
       (void)hipGetLastError();
       return fail(MG_ERR_OOM, "mograd: out of device memory allocating %s", fmt_bytes(n).c_str());
     }
-    pool.live[p] = -n;
+    pool.live[p] = cls;
     *out = p;
     return MG_OK;
   }
-  const int64_t cls = round_class(nbytes);
   void* p = nullptr;
   auto it = pool.free_lists.find(cls);
   if (it != pool.free_lists.end() && !it->second.empty()) {
@@ -234,13 +251,17 @@ int pool_take(void** out, int64_t nbytes) {
   return MG_OK;
 }
 
-int pool_release(void* ptr) {
-  if (!ptr || t_hold_released) return MG_OK;
-  std::lock_guard<std::mutex> lock(g_pool_mu);
-  Pool& pool = current_pool();
+static int release_locked(Pool& pool, void* ptr) {
   auto it = pool.live.find(ptr);
   if (it == pool.live.end()) return fail(MG_ERR_INVALID, "pool_free: pointer %p was not allocated by this pool", ptr);
   const int64_t cls = it->second;
+  if (t_holding) {
+    try {
+      pool.recorded[t_recording][cls].push_back(ptr);
+    } catch (const std::exception&) {  // (no memory for the list: the block stays the graph's)
+    }
+    return MG_OK;
+  }
   pool.live.erase(it);
   if (cls < 0) {  // unpooled: plain release (hipFree waits for the device)
     (void)hipFree(ptr);
@@ -249,6 +270,26 @@ int pool_release(void* ptr) {
   pool.free_lists[cls].push_back(ptr);
   pool.stats.allocated_bytes -= cls;
   pool.stats.free_count += 1;
+  return MG_OK;
+}
+
+int pool_release(void* ptr) {
+  if (!ptr) return MG_OK;
+  std::lock_guard<std::mutex> lock(g_pool_mu);
+  return release_locked(current_pool(), ptr);
+}
+
+static int free_recorded() {
+  std::lock_guard<std::mutex> lock(g_pool_mu);
+  Pool& pool = current_pool();
+  for (auto& recording : pool.recorded)
+    for (auto& list : recording.second)
+      while (!list.second.empty()) {
+        void* const p = list.second.back();
+        list.second.pop_back();
+        MG_TRY(release_locked(pool, p));
+      }
+  pool.recorded.clear();
   return MG_OK;
 }
 
@@ -380,6 +421,10 @@ int mg_pool_empty_cache(void) {
   std::lock_guard<std::mutex> lock(mg::g_pool_mu);
   mg::empty_cache_locked(mg::current_pool());
   return MG_OK;
+}
+
+int mg_pool_free_recorded(void) {
+  return mg::without_exceptions("pool_free_recorded", [] { return mg::free_recorded(); });
 }
 
 int mg_pool_get_stats(mg_pool_stats* out) {

@@ -143,3 +143,42 @@ norm_bwd(64, 64, 64)  # (the default stream is never captured)
 out.append(len(launches()))
 """)
     assert got[:4] == [3, 3, 0, 0] and got[4] > 0
+
+
+def test_recorded_calls_share_scratch_within_a_stream_of_a_capture(over_stub):
+    """A replay runs them in order, so the second takes what the first had; another stream, another capture and eager calls do not, until
+    the program has destroyed its graphs and says so."""
+    got = over_stub("""
+from mograd_amd._lib import PoolStats
+streams = C.c_void_p(1 << 16), C.c_void_p(1 << 17)
+
+def both(stream):
+    norm_bwd(512, 640, 512, stream=stream)
+    linear(1024, 640, 512, stream=stream)
+
+def taken():
+    stats = PoolStats()
+    lib.mg_pool_get_stats(stats)
+    return stats.allocated_bytes
+
+def during(capture, stream):
+    stub.stub_capture(capture)
+    before = taken()
+    both(stream)
+    out.append(taken() - before)
+
+during(0, streams[0])
+for capture, stream in ((7, 0), (7, 0), (7, 1), (7, 0), (8, 0), (8, 0), (0, 0)):
+    during(capture, streams[stream])
+out.append(taken())
+stub.stub_capture(0)
+lib.mg_pool_free_recorded()
+out.append(taken())
+mallocs = stub.stub_mallocs()
+both(streams[0])
+out += [taken(), stub.stub_mallocs() - mallocs, stub.stub_mode()]
+""")
+    eager, first, again, other_stream, back, other_capture, again2, between, held, *rest = got
+    assert eager == again == back == again2 == between == 0
+    assert first == other_stream == other_capture > 0 and held == 3 * first
+    assert rest == [0, 0, 0, 0]
