@@ -294,7 +294,7 @@ class TinyTransformer:
 
     def _residual_norm(self) -> bool:
         """Whether the blocks' outputs join the stream by mg_residual_norm_fwd."""
-        return self.post_norm or self.act8 or self.residual_scale != 1.0
+        return self.L > 0 and (self.post_norm or self.act8 or self.residual_scale != 1.0)
 
     def _plan_residual_norm(self, B: int, T: int, new) -> None:
         n, d, ff, V = B * T, self.d, self.ff, self.V

@@ -85,6 +85,15 @@ hipError_t hipMalloc(void** p, size_t n) {
   return hipSuccess;
 }
 hipError_t hipFree(void*) { return hipSuccess; }
+hipError_t hipSetDevice(int) { return hipSuccess; }
+hipError_t hipGetSymbolAddress(void** p, const void*) { return hipMalloc(p, 4096); }
+hipError_t hipMemcpyAsync(void*, const void*, size_t, hipMemcpyKind, hipStream_t) { return hipSuccess; }
+hipError_t hipStreamCreate(hipStream_t* stream) {
+  *stream = reinterpret_cast<hipStream_t>(g_next.fetch_add(4096));
+  return hipSuccess;
+}
+hipError_t hipStreamDestroy(hipStream_t) { return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
 hipError_t hipDeviceSynchronize(void) { return hipSuccess; }
 hipError_t hipStreamIsCapturing(hipStream_t stream, hipStreamCaptureStatus* status) {
   *status = stream && g_capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;

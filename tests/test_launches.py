@@ -182,3 +182,22 @@ out += [taken(), stub.stub_mallocs() - mallocs, stub.stub_mode()]
     assert eager == again == back == again2 == between == 0
     assert first == other_stream == other_capture > 0 and held == 3 * first
     assert rest == [0, 0, 0, 0]
+
+
+def test_a_transformer_without_blocks_takes_the_options(over_stub):
+    """Embedding and head alone: there is nothing that the options change."""
+    got = over_stub("""
+import numpy as np
+from mograd_amd import AnyBuffer, Device
+from mograd_amd.tiny_transformer import TinyTransformer
+device = Device()
+ids = AnyBuffer.from_numpy(device, np.zeros((2, 8), np.int32))
+for options in (dict(), dict(post_norm=True), dict(act8=True), dict(residual_scale=0.5)):
+    model = TinyTransformer(device, 17, 32, 64, 0, 2, **options)
+    launches()
+    model.step(ids, ids, 2, 8)
+    out.append((launches(), model.kept_bytes()))
+for l in out:
+    l[0][:] = [v[:6] for v in l[0]]
+""")
+    assert len(got[0][0]) > 0 and all(g == got[0] for g in got)
