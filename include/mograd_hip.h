@@ -9,15 +9,17 @@
  *     errors in the same situations; a binding re-raises from the message.
  *   - All data pointers are DEVICE pointers unless a parameter is documented as host.
  *   - The caller owns inputs and outputs.  Outputs need no initialisation.  Scratch is
- *     taken from the library's pool and returned before the call returns; this is safe
- *     because all work of one call is enqueued on the one stream passed in, and the pool
- *     hands memory back out only to later calls (the reference's single in-order-stream
- *     contract, mograd/memory.mojo:27-31).  This makes the library a one-stream-per-device
- *     library: every entry point that takes scratch (the LayerNorm, cross-entropy, Linear
- *     and attention backward entries, split products, mg_sum_axis, mg_scatter_add and the
- *     `_deferred` forms) returns its blocks to the pool while its kernels are still queued,
- *     untagged by stream, so calls issued on two streams of one device that overlap in
- *     time may be handed the same block.  Use one stream per device, or order the streams
+ *     taken from the library's pool and returned before the call returns (mg_linear_bwd_act8
+ *     and mg_residual_norm_bwd on a stream that is being captured keep it for the graph, see
+ *     mg_pool_free_recorded); this is safe because all work of one call is enqueued on the
+ *     one stream passed in, and the pool hands memory back out only to later calls (the
+ *     reference's single in-order-stream contract, mograd/memory.mojo:27-31).  This makes
+ *     the library a one-stream-per-device library: every entry point that takes scratch
+ *     (the LayerNorm, cross-entropy, Linear and attention backward entries,
+ *     mg_residual_norm_bwd, mg_linear_bwd_act8, split products, mg_sum_axis, mg_scatter_add
+ *     and the `_deferred` forms) returns its blocks to the pool while its kernels are still
+ *     queued, untagged by stream, so calls issued on two streams of one device that overlap
+ *     in time may be handed the same block.  Use one stream per device, or order the streams
  *     with events so that such calls never overlap.
  *   - `stream` is a hipStream_t passed as void*; NULL is the default stream.  No function
  *     synchronises the host unless its comment says so.

@@ -201,3 +201,27 @@ for l in out:
     l[0][:] = [v[:6] for v in l[0]]
 """)
     assert len(got[0][0]) > 0 and all(g == got[0] for g in got)
+
+
+def test_the_header_names_the_entries_that_take_scratch(over_stub):
+    """Calls of these that overlap in time on two streams write into each other's scratch; the header's conventions say which."""
+    got = over_stub("""
+from mograd_amd._lib import PoolStats
+
+def asked():
+    stats = PoolStats()
+    lib.mg_pool_get_stats(stats)
+    return stats.hit_count + stats.miss_count
+
+for name, call in (("mg_act8_store", lambda: lib.mg_act8_store(p, p, 64, 64, 0, BF16, None)),
+                   ("mg_act8_load", lambda: lib.mg_act8_load(p, p, 64, 64, BF16, None)),
+                   ("mg_linear_bwd_act8", lambda: linear(64, 64, 64)), ("mg_residual_norm_fwd", lambda: norm_fwd(64, 3, 64, keep=p)),
+                   ("mg_residual_norm_bwd", lambda: norm_bwd(64, 64, 64))):
+    before = asked()
+    call()
+    out.append((name, asked() > before))
+""")
+    text = (ROOT / "include" / "mograd_hip.h").read_text()
+    conventions = text[text.index("every entry point that takes scratch"):text.index("returns its blocks")]
+    for name, takes in got:
+        assert (name in conventions) == takes, name
