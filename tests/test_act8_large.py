@@ -4,6 +4,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import test_act8 as A
 from mograd_amd import F32, I32, AnyBuffer
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +44,11 @@ def test_more_chunks_than_32_bits_count_and_a_launch_holds(device):
     assert np.array_equal(np.where(value(0) == 0, 7, np.frexp(value(0))[1] + 126), e[0])  # 2^E <= |x| < 2^(E + 1): k = E - 6
     del x, back, act8, one
     lib.mg_pool_empty_cache()
+
+
+@pytest.mark.parametrize("dtype", A.FLOATS)
+@pytest.mark.parametrize("rows,cols", [(-1, 1024), (0, 1024), (1, 1024), (37, 1001), (5, 993)])
+def test_four_chunks_a_thread(device, dtype, rows, cols):
+    """Tensors of a million chunks of 16 bytes on the way there: one row fewer, just as many, and more, the last workgroup not full."""
+    rows += (1 << 20) * (4 if dtype == F32 else 8) // 1024
+    A.test_store_and_load(device, dtype, rows, cols, keep_sign=rows % 2)
