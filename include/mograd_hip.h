@@ -573,6 +573,7 @@ int mg_act8_load(const void* act8, void* x, int64_t rows, int64_t cols, int dtyp
  *   dw(N,K) = dY^T X'
  *   db(N)   = column sums of dY (NULL to skip).
  * `x8` was stored from a tensor of `dtype`.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the unrounded fp32 sums.
+ * fp32: of a dY of less than 2^-110, dw may leave out what lies below 2^-133.
  * M == 0: dw and db are zeros. */
 int mg_linear_bwd_act8(const void* dy, const void* x8, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t N,
                        int64_t K, int dx_accumulate, int x_is_relu_output, int dtype, int grad_dtype, mg_stream stream);

@@ -6,9 +6,10 @@
 // tensor to the bit, without the tensor: 33 / 32 bytes a value are read instead of one pass that writes two and another that
 // reads them.  A conversion, a multiplication and half a packing a value, done once for the 128 columns of dY that meet it.
 //
-// fp32 dY is cut into three bf16 terms of 8 significant bits each, dY = a + b + c without a remainder (truncation, so that the
-// largest finite values do not round to infinity), and X' is exact in bf16, so three products accumulate in fp32 what one of
-// fp32 operands would, at 16 / 3 times the rate of the fp32 matrix instructions.
+// fp32 dY is cut into three bf16 terms of 8 significant bits each, dY = a + b + c without a remainder from |dY| = 2^-110 on, and
+// to bf16's least number, 2^-133, below (truncation, so that the largest finite values do not round to infinity; the matrix
+// instructions multiply subnormal numbers as they are), and X' is exact in bf16, so three products accumulate in fp32 what one of fp32
+// operands would, at 16 / 3 times the rate of the fp32 matrix instructions.
 //
 // Steps of 64 rows (fp32: 32), two copies in LDS, 64 KB: two workgroups a CU.  The rows of the step after next are requested
 // into registers while the present step is multiplied, those of the next one converted and written.
