@@ -850,6 +850,9 @@ struct ResidualNormOps {
   //  - backward, 65 to 128 chunks, one wave: no barriers, and a workgroup's rows share their column sums (bf16 1024 columns, two
   //    waves | one: 2048 rows 20.4 | 16.0, 16384 rows 51.0 | 50.1)
   //  - past 512 chunks two to a thread: 1024 threads have too few registers each (bf16 (2048, 8192) backward 58.0 | 54.8).
+  // Past 1024 chunks nothing is left but two to each of 1024 threads, whose 128 registers do not hold a row of the backward with both
+  // norms: bf16 spills 320 to 364 bytes a lane (off the chunks 472 to 532), fp32 none to 44 (172 to 192), the bf16 forward 52 to 168.
+  // bf16 (2048, 12288) forward 52 us, with f8 and x8 95, backward 273, of 41, 51 and 61 by its bytes; fp32 (2048, 6144) backward 70 of 61.
   static bool pick_shape(bool forward, int64_t rows, int64_t chunks, Shape* s) {
     const bool two = forward ? rows >= 8192 : false;
     if (chunks <= 16) *s = {16, 1};
@@ -935,7 +938,9 @@ struct ResidualNormOps {
   }
 
   // Splits the rows over at most `most` workgroups of `rows_at_once` rows: fewer gate rows than workgroups are cut into
-  // pieces, more are dealt out whole.
+  // pieces, more are dealt out whole.  (Counts between do not fill the device: 129 to 255 gate rows are a workgroup each, 257 are
+  // two to a workgroup.  us a million values, bf16 (gates 512, 384) with 128 | 129 | 200 | 256 | 257 | 300 gate rows 2.8 | 3.6 | 2.7 |
+  // 2.7 | 3.4 | 3.1; pieces are whole multiples of rows_at_once, so (2587, 1001) with 13 gate rows of 199 is 169 workgroups.)
   static int64_t partition(ResidualNormBwd<T>& a, int64_t most, int rows_at_once, bool interleave) {
     a.own = 0;
     const int64_t per_gate = std::max<int64_t>(1, std::min(most / a.gates, ceil_div(a.gate_rows, rows_at_once)));
