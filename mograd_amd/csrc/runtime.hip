@@ -3,6 +3,8 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <thread>
+#include <tuple>
 #include <unordered_map>
 #include <vector>
 
@@ -87,7 +89,8 @@ static int64_t round_class(int64_t nbytes) {
 }
 
 using FreeLists = std::unordered_map<int64_t, std::vector<void*>>;  // by the value in Pool::live
-using Recording = std::pair<unsigned long long, hipStream_t>;        // a capture's id, and one of its streams
+// A capture's id, and one of its streams; the thread, because hipStreamPerThread names a stream of each.
+using Recording = std::tuple<unsigned long long, hipStream_t, std::thread::id>;
 
 struct Pool {
   FreeLists free_lists;
@@ -180,7 +183,7 @@ int CaptureHold::begin(hipStream_t stream) {
     return fail(MG_ERR_HIP, "scratch cannot be kept for the graph: %s", hipGetErrorString(e));
   }
   on_ = t_holding = true;
-  t_recording = {id, stream};
+  t_recording = {id, stream, std::this_thread::get_id()};
   return MG_OK;
 }
 

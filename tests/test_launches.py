@@ -184,6 +184,29 @@ out += [taken(), stub.stub_mallocs() - mallocs, stub.stub_mode()]
     assert rest == [0, 0, 0, 0]
 
 
+def test_recorded_calls_on_the_streams_of_two_threads(over_stub):
+    """hipStreamPerThread is a stream of each thread by one name: as branches of one capture they do not share scratch."""
+    got = over_stub("""
+import threading
+from mograd_amd._lib import PoolStats
+
+def record():
+    before, after = PoolStats(), PoolStats()
+    lib.mg_pool_get_stats(before)
+    linear(1024, 640, 512, stream=C.c_void_p(2))
+    lib.mg_pool_get_stats(after)
+    out.append(after.allocated_bytes - before.allocated_bytes)
+
+stub.stub_capture(7)
+record()
+record()
+other = threading.Thread(target=record)
+other.start()
+other.join()
+""")
+    assert got[0] > 0 and got == [got[0], 0, got[0]]
+
+
 def test_a_transformer_without_blocks_takes_the_options(over_stub):
     """Embedding and head alone: there is nothing that the options change."""
     got = over_stub("""
