@@ -9,15 +9,16 @@
  *     errors in the same situations; a binding re-raises from the message.
  *   - All data pointers are DEVICE pointers unless a parameter is documented as host.
  *   - The caller owns inputs and outputs.  Outputs need no initialisation.  Scratch is
- *     taken from the library's pool and returned before the call returns (mg_linear_bwd_act8
- *     and mg_residual_norm_bwd on a stream that is being captured keep it for the graph, see
+ *     taken from the library's pool and returned before the call returns (mg_linear_bwd_act8,
+ *     mg_residual_norm_bwd, mg_gated_linear_fwd, mg_gated_linear_bwd, mg_grad_norm and
+ *     mg_clip_grads on a stream that is being captured keep it for the graph, see
  *     mg_pool_free_recorded); this is safe because all work of one call is enqueued on the
  *     one stream passed in, and the pool hands memory back out only to later calls (the
  *     reference's single in-order-stream contract, mograd/memory.mojo:27-31).  This makes
  *     the library a one-stream-per-device library: every entry point that takes scratch
  *     (the LayerNorm, cross-entropy, Linear and attention backward entries,
- *     mg_residual_norm_bwd, mg_linear_bwd_act8, split products, mg_sum_axis, mg_scatter_add
- *     and the `_deferred` forms) returns its blocks to the pool while its kernels are still
+ *     mg_residual_norm_bwd, mg_linear_bwd_act8, mg_gated_linear_fwd and _bwd, mg_grad_norm,
+ *     mg_clip_grads, split products, mg_sum_axis, mg_scatter_add and the `_deferred` forms) returns its blocks to the pool while its kernels are still
  *     queued, untagged by stream, so calls issued on two streams of one device that overlap
  *     in time may be handed the same block.  Use one stream per device, or order the streams
  *     with events so that such calls never overlap.
@@ -134,7 +135,7 @@ int mg_pool_free(void* ptr);
  * (memory.mojo:353-362). */
 int mg_pool_empty_cache(void);
 
-/* Returns the scratch that recorded calls keep (mg_residual_norm_bwd and mg_linear_bwd_act8, see there) to the free lists of the
+/* Returns the scratch that recorded calls keep (mg_residual_norm_bwd, mg_linear_bwd_act8 and others, see there) to the free lists of the
  * current device's pool.  For a program that has destroyed its graphs of such calls, and is capturing none.  No counterpart in the
  * reference. */
 int mg_pool_free_recorded(void);
@@ -432,6 +433,26 @@ int mg_adam_step(void* w, const void* g, void* m, void* v, int64_t n, float lr, 
 /* w = w - g * lr.  Replaces mograd/nn/optim/sgd.mojo:24-45. */
 int mg_sgd_step(void* w, const void* g, int64_t n, float lr, mg_stream stream);
 
+/* The same updates from gradients that are scaled down to a largest global norm on their way in: g is taken as
+ * g * (norm[0] > max_norm ? max_norm / norm[0] : 1), each operation rounded to fp32; g itself stays as it is.  `norm`: one fp32 number
+ * on the device, as mg_grad_norm leaves it.  max_norm >= 0.  No counterpart in the reference. */
+int mg_adam_step_clipped(void* w, const void* g, void* m, void* v, int64_t n, float lr, float beta1, float beta2, float eps,
+                         float weight_decay, int64_t t, int decoupled_weight_decay, const float* norm, float max_norm,
+                         mg_stream stream);
+int mg_sgd_step_clipped(void* w, const void* g, int64_t n, float lr, const float* norm, float max_norm, mg_stream stream);
+
+/* norm[0] (fp32, on the device) = the square root of the sum of the squares of all elements of `count` tensors: their device
+ * addresses, numbers of elements and dtypes (F32, F16, BF16, in any mixture) in HOST arrays of `count` entries, which are free again
+ * when the call returns.  A tensor may start at any address of its elements, and be empty (its address is not looked at).  Squares and
+ * sums in 64 bits, always added in the same order.  No tensors, or none with an element: 0.  No counterpart in the reference. */
+int mg_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int64_t count, float* norm, mg_stream stream);
+
+/* The norm as above (`norm` may be NULL), and out[i] = grads[i] * (norm > max_norm ? max_norm / norm : 1), in fp32, rounded once to the
+ * tensor's dtype.  out[i] may be grads[i]; no other overlap.  max_norm >= 0.  So gradients of a norm that is not a number stay as they
+ * are, and those of an infinite norm become zeros, and NaN where they are infinite.  No counterpart in the reference. */
+int mg_clip_grads(const void* const* grads, void* const* out, const int64_t* numels, const int* dtypes, int64_t count, float max_norm,
+                  float* norm, mg_stream stream);
+
 /* ------------------------------------------------------------------------------------ */
 /* Deferred second-stage reductions.  No counterpart in the reference, which runs every   */
 /* reduction where its graph node is evaluated.                                           */
@@ -605,8 +626,62 @@ int mg_residual_norm_bwd(const void* dx, const void* dh_out, const void* f, cons
                          void* dpost_gamma, void* dpost_beta, void* dpre_gamma, void* dpre_beta, int64_t rows, int64_t cols,
                          int64_t gate_rows, float residual_scale, int dtype, int grad_dtype, mg_stream stream);
 
-/* mg_linear_bwd_act8 and mg_residual_norm_bwd take scratch from the pool.  Recorded into a HIP graph they keep it: what such a
- * call took goes only to calls that are recorded on the same stream in the same capture, so that graphs, the branches of a graph, and
+/* ------------------------------------------------------------------------------------ */
+/* Gated Linear layers and rotary positions.  No counterpart in the reference, whose       */
+/* blocks have a ReLU between two Linear layers and no positions                          */
+/* (examples/tinyshakespear/model.mojo:62-64,88-121).                                     */
+/* ------------------------------------------------------------------------------------ */
+
+/* What a gate is passed through: silu(g) = g sigmoid(g); gelu(g) = g Phi(g); gelu with sigmoid(2 sqrt(2/pi) (g + 0.044715 g^3)) for
+ * Phi (the tanh form); sigmoid(g); max(g, 0). */
+typedef enum mg_gate {
+  MG_GATE_SILU = 0,
+  MG_GATE_GELU = 1,
+  MG_GATE_GELU_TANH = 2,
+  MG_GATE_SIGMOID = 3,
+  MG_GATE_RELU = 4
+} mg_gate;
+
+/* y (M,F) = act(x Wg^T + bg) * (x Wu^T + bu) for x (M,K), all contiguous.  w (2F,K) holds Wg's rows, then Wu's; bias (2F) bg, then bu
+ * (NULL for none).  gu (M,2F): where the two projections g | u of each row are left for the backward (NULL: nowhere).  `gate`: an
+ * mg_gate.  Products and act in fp32, y from the projections before they are rounded.  Any M, F and K from 1, any address of an
+ * element; 16-bit tensors: K at most 2^22 - 64.  Nothing overlaps. */
+int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y, void* gu, int64_t M, int64_t F, int64_t K, int gate,
+                        int dtype, mg_stream stream);
+
+/* Its gradients, from dy (M,F) and the kept gu:  with dg = dy u act'(g) and du = dy act(g), rounded to `dtype`,
+ *   dx(M,K) = dg Wg + du Wu     (NULL to skip; dx_accumulate != 0: added to dx)
+ *   dw(2F,K) = dg^T x | du^T x
+ *   db(2F)  = column sums of dg | du (NULL to skip).
+ * act'(0) of max(g, 0) is 0.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the unrounded fp32 sums.  M == 0: dw and db
+ * are zeros. */
+int mg_gated_linear_bwd(const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t F,
+                        int64_t K, int dx_accumulate, int gate, int dtype, int grad_dtype, mg_stream stream);
+/* The same with the sums of dw and db deferred (see mg_deferred). */
+int mg_gated_linear_bwd_deferred(const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
+                                 int64_t F, int64_t K, int dx_accumulate, int gate, int dtype, int grad_dtype, mg_deferred list,
+                                 mg_stream stream);
+
+/* Queries or keys turned by their positions: y = x, but in each head of each token the pairs of columns (a, b) of the first `rotated`
+ * ones (even, at most 512) become
+ *   y_a = x_a cos t - x_b sin t,  y_b = x_a sin t + x_b cos t,  t = positions(pair_axis[i], b, s) * inv_freq[i],  0 <= i < rotated / 2
+ * for pair i = columns (i, i + rotated / 2), or with neighbours != 0 columns (2 i, 2 i + 1).  inverse != 0: t is taken as -t, which is
+ * the gradient (of y, to that of x).
+ *   x, y        (B,S,H,D) with element strides of batch, token and head in HOST arrays of three; a head's D columns lie side by side.
+ *               y may be x (with the same strides: in place, and then only the pairs are touched); no other overlap.  Queries and keys
+ *               of a (B,S,3,H,D) projection are one call of 2 H heads.
+ *   positions   int32 or int64 (pos_dtype) on the device, (axes,B,S) with element strides pos_strides (HOST, three; 0: shared).
+ *               NULL: 0 .. S-1 in every sequence; axes, pos_strides, pos_dtype and pair_axis are then not looked at.
+ *   pair_axis   HOST, rotated / 2 entries below `axes` (at most 255), which of a token's positions a pair goes by: time, height and
+ *               width of a patch of a video.  NULL where there is one axis.
+ *   inv_freq    fp32 on the device, rotated / 2 entries.
+ * Strides >= 0, H D at most 2^22.  Angles in 64 bits, the turn in fp32, each output rounded once. */
+int mg_rotary(const void* x, void* y, const void* positions, const float* inv_freq, const int32_t* pair_axis, int64_t B, int64_t S,
+              int64_t H, int64_t D, int64_t rotated, const int64_t* x_strides, const int64_t* y_strides, const int64_t* pos_strides,
+              int axes, int pos_dtype, int neighbours, int inverse, int dtype, mg_stream stream);
+
+/* mg_linear_bwd_act8, mg_residual_norm_bwd, mg_gated_linear_fwd, mg_gated_linear_bwd, mg_grad_norm and mg_clip_grads take scratch from
+ * the pool.  Recorded into a HIP graph they keep it: what such a call took goes only to calls that are recorded on the same stream in the same capture, so that graphs, the branches of a graph, and
  * eager calls never share it.  It stays so, also where the capture fails, until mg_pool_free_recorded. */
 
 #ifdef __cplusplus

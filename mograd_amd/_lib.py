@@ -21,6 +21,8 @@ LIB_NAME = "libmograd_hip.so"
 
 # mg_dtype
 F32, F16, BF16, I32, I64 = 0, 1, 2, 3, 4
+# mg_gate
+GATE_SILU, GATE_GELU, GATE_GELU_TANH, GATE_SIGMOID, GATE_RELU = range(5)
 DTYPE_NAMES = {F32: "float32", F16: "float16", BF16: "bfloat16", I32: "int32", I64: "int64"}
 DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2, I32: 4, I64: 8}
 
@@ -139,6 +141,14 @@ PROTOTYPES = {
     "mg_linear_bwd_act8": (_i, [_p] * 6 + [_l, _l, _l, _i, _i, _i, _i, _p], True),
     "mg_residual_norm_fwd": (_i, [_p] * 15 + [_l, _l, _l, _f, _f, _i, _p], True),
     "mg_residual_norm_bwd": (_i, [_p] * 20 + [_l, _l, _l, _f, _i, _i, _p], True),
+    "mg_gated_linear_fwd": (_i, [_p] * 5 + [_l, _l, _l, _i, _i, _p], True),
+    "mg_gated_linear_bwd": (_i, [_p] * 7 + [_l, _l, _l, _i, _i, _i, _i, _p], True),
+    "mg_gated_linear_bwd_deferred": (_i, [_p] * 7 + [_l, _l, _l, _i, _i, _i, _i, _p, _p], True),
+    "mg_rotary": (_i, [_p, _p, _p, _p, C.POINTER(C.c_int32)] + [_l] * 5 + [_pl] * 3 + [_i, _i, _i, _i, _i, _p], True),
+    "mg_grad_norm": (_i, [C.POINTER(_p), _pl, C.POINTER(_i), _l, _p, _p], True),
+    "mg_clip_grads": (_i, [C.POINTER(_p), C.POINTER(_p), _pl, C.POINTER(_i), _l, _f, _p, _p], True),
+    "mg_adam_step_clipped": (_i, [_p, _p, _p, _p, _l, _f, _f, _f, _f, _f, _l, _i, _p, _f, _p], True),
+    "mg_sgd_step_clipped": (_i, [_p, _p, _l, _f, _p, _f, _p], True),
     "mg_flash_attn_bwd_packed": (_i, [_p] * 6 + [_l, _l, _l, _l, _f, _i, _i, _i, _p], True),
 }
 

@@ -1,0 +1,90 @@
+// A gated Linear layer: g = x Wg^T + bg, u = x Wu^T + bu, y = act(g) u, with W = [Wg; Wu] one (2 F, K) array and b = [bg; bu].
+//
+// Gradients, from dy and the kept g and u:
+//   dg = dy u act'(g),  du = dy act(g);   dx = [dg du] W,  dW = [dg du]^T x,  db = column sums of [dg du]
+#pragma once
+
+#include "gemm_impl.h"
+
+namespace mg {
+
+// A product's arguments: B the weights, N the columns F of y, C y (M, F) without gaps.
+template <typename T>
+struct GatedProblem : Gemm16Problem<T> {
+  T* gu = nullptr;  // (M, 2 F): g and u, rounded; may be null
+  int gate = 0;
+};
+
+// Calls f with `gate` (an mg_gate) as a compile-time number.
+template <typename F>
+__host__ __device__ __forceinline__ void gated_with(int gate, F&& f) {
+  switch (gate) {
+    case MG_GATE_SILU: return f(std::integral_constant<int, MG_GATE_SILU>{});
+    case MG_GATE_GELU: return f(std::integral_constant<int, MG_GATE_GELU>{});
+    case MG_GATE_GELU_TANH: return f(std::integral_constant<int, MG_GATE_GELU_TANH>{});
+    case MG_GATE_SIGMOID: return f(std::integral_constant<int, MG_GATE_SIGMOID>{});
+    default: return f(std::integral_constant<int, MG_GATE_RELU>{});
+  }
+}
+
+// s = 1 / (1 + e^-z) and t = 1 - s, either to a few units in its own last place: from e^-|z|, which neither overflows nor leaves
+// anything to cancel.  FAST: e^z as 2^(z log2 e) with the hardware's exponential and reciprocal, |z| 2^-24 and 2^-23 off, which
+// 16 bits do not see; fp32 takes the exact ones.
+template <bool FAST>
+__device__ __forceinline__ void gated_sigmoid(float z, float& s, float& t) {
+  float e, r;
+  if constexpr (FAST) {
+    e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(z));
+    r = __builtin_amdgcn_rcpf(1.f + e);
+  } else {
+    e = expf(-fabsf(z));
+    r = 1.f / (1.f + e);
+  }
+  const float small = e * r;
+  s = z >= 0.f ? r : small;
+  t = z >= 0.f ? small : r;
+  if (z != z) s = t = z;
+}
+
+// The normal distribution's Phi(g): through erfc, whose tail keeps its digits.
+__device__ __forceinline__ float gated_phi(float g) { return 0.5f * erfcf(-0.70710678f * g); }
+
+constexpr float kGeluTanh2C = 1.59576912f;  // 2 sqrt(2 / pi): 1/2 (1 + tanh(c v)) = sigmoid(2 c v)
+
+// act(g)
+template <bool FAST, int GATE>
+__device__ __forceinline__ float gated_act(float g) {
+  if constexpr (GATE == MG_GATE_RELU) return g > 0.f ? g : g != g ? g : 0.f;
+  else if constexpr (GATE == MG_GATE_GELU) return g * gated_phi(g);
+  else {
+    float s, t;
+    gated_sigmoid<FAST>(GATE == MG_GATE_GELU_TANH ? kGeluTanh2C * g * (1.f + 0.044715f * g * g) : g, s, t);
+    return GATE == MG_GATE_SIGMOID ? s : g * s;
+  }
+}
+
+// act(g) and act'(g)
+template <bool FAST, int GATE>
+__device__ __forceinline__ void gated_act_slope(float g, float& act, float& slope) {
+  if constexpr (GATE == MG_GATE_RELU) {
+    act = gated_act<FAST, GATE>(g);
+    slope = g > 0.f ? 1.f : g != g ? g : 0.f;
+  } else if constexpr (GATE == MG_GATE_GELU) {
+    const float phi = gated_phi(g);
+    act = g * phi;
+    slope = phi + g * 0.39894228f * (FAST ? __builtin_amdgcn_exp2f(-0.72134752f * g * g) : expf(-0.5f * g * g));
+  } else {
+    float s, t;
+    gated_sigmoid<FAST>(GATE == MG_GATE_GELU_TANH ? kGeluTanh2C * g * (1.f + 0.044715f * g * g) : g, s, t);
+    const float st = s * t;
+    if constexpr (GATE == MG_GATE_SIGMOID) act = s, slope = st;
+    else if constexpr (GATE == MG_GATE_SILU) act = g * s, slope = s + g * st;
+    else act = g * s, slope = s + g * st * kGeluTanh2C * (1.f + 0.134145f * fminf(g * g, 1e30f));  // (st is zero by then)
+  }
+}
+
+// gemm_deep_*.hip: the products and y in one launch, operands on 16-byte chunks, `tile` kTile128 or kTile256 (64 and 128 columns of y).
+template <typename T>
+int launch_gated_deep(const GatedProblem<T>& pr, Gemm16Tile tile, hipStream_t stream);
+
+}  // namespace mg

@@ -2,6 +2,7 @@
 // a k-step ahead.
 #pragma once
 
+#include "gated_linear.h"
 #include "gemm_impl.h"
 
 namespace mg {
@@ -48,10 +49,19 @@ struct Gemm16Deep {
                                     : 160 * 1024 / kLds < kWavesPerSimd * 2 / WN ? 160 * 1024 / kLds : kWavesPerSimd * 2 / WN;
   static_assert(kRowsA * 8 % kThreads == 0 && kRowsB0 * 8 % kThreads == 0 && kRowsB1 * 8 % kThreads == 0, "whole requests");
   static constexpr bool kMask8 = false;  // the output is masked by Gemm16Problem::mask8
+  static constexpr bool kGated = false;  // the problem is a GatedProblem
 };
 template <class S>
 struct Gemm16DeepMask8 : S {
   static constexpr bool kMask8 = true;
+};
+// A gated Linear layer: part B0 of a wave's columns is multiplied by rows of the gate's weights, part B1 by the same rows of the
+// other ones, so that a lane holds both projections of an output and the product needs no exchange.  A tile has kTN / 2 columns of
+// the output.
+template <class S>
+struct Gemm16DeepGated : S {
+  static_assert(S::BJ0 == S::BJ1, "the same columns of both projections");
+  static constexpr bool kGated = true;
 };
 // Byte offsets, from the tile's first row and the step's first k, of the 16-byte chunks that this thread
 // requests for one image.  Image row r is row (r / PER_WAVE) * WAVE_ROWS + first + r % PER_WAVE of the
@@ -333,6 +343,67 @@ __device__ __forceinline__ void gemm16_deep_ln_bwd(const floatx16 (&acc)[2][S::B
   }
 }
 
+// Rows of a wave's strip (64 x 32 BJ rounded values) to C, 16 bytes per lane, whole rows one after the other.
+template <typename T, int BJ>
+__device__ __forceinline__ void gemm16_strip_out(const uint16_t* __restrict__ mine, T* __restrict__ C, int64_t ldc, int M, int N,
+                                                 int row0, int col0, int lane) {
+  constexpr int STRIDE = 32 * BJ + 8, CPR = 4 * BJ;
+  static_assert(64 % CPR == 0, "a lane keeps its chunk");
+  const int r0 = lane / CPR, ch = lane % CPR, c = col0 + ch * 8;
+  if (c >= N) return;
+#pragma unroll
+  for (int i = 0; i < CPR; ++i) {
+    const int rl = r0 + i * (64 / CPR), r = row0 + rl;
+    if (r >= M) return;
+    const uint4 v = *reinterpret_cast<const uint4*>(mine + rl * STRIDE + ch * 8);
+    T* const at = C + static_cast<int64_t>(r) * ldc + c;
+    if (c + 8 > N) {  // the chunk over the right edge, element by element
+      const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (c + e < N) at[e] = __builtin_bit_cast(T, static_cast<uint16_t>(vw[e / 2] >> (e % 2 * 16)));
+      continue;
+    }
+    const gemm_u4_any out = {v.x, v.y, v.z, v.w};
+    *reinterpret_cast<gemm_u4_any*>(at) = out;
+  }
+}
+
+// Output of a wave's 64 rows of a gated layer: y = act(g) u from the unrounded projections, and these where they are kept.
+template <typename T, int BJ0>
+__device__ __forceinline__ void gemm16_deep_gated_write(const floatx16 (*acc)[2 * BJ0], const float (&bias_v)[2 * BJ0],
+                                                       uint16_t* __restrict__ mine, const GatedProblem<T>& pr, int row0, int col0,
+                                                       int lane) {
+  floatx16 part[2][BJ0];
+  const float none[BJ0] = {};
+  gated_with(pr.gate, [&](auto gate) {
+#pragma unroll
+    for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+      for (int tj = 0; tj < BJ0; ++tj)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          part[ti][tj][r] = gated_act<true, decltype(gate)::value>(acc[ti][tj][r] + bias_v[tj]) * (acc[ti][BJ0 + tj][r] + bias_v[BJ0 + tj]);
+  });
+  gemm16_deep_stage<T, false, false, BJ0>(part, none, mine, lane);
+  __builtin_amdgcn_wave_barrier();  // the strip is the wave's own: its LDS accesses are in order
+  gemm16_strip_out<T, BJ0>(mine, pr.C, pr.N, pr.M, pr.N, row0, col0, lane);
+  if (!pr.gu) return;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+      for (int tj = 0; tj < BJ0; ++tj)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[ti][tj][r] = acc[ti][half * BJ0 + tj][r] + bias_v[half * BJ0 + tj];
+    gemm16_deep_stage<T, false, false, BJ0>(part, none, mine, lane);
+    __builtin_amdgcn_wave_barrier();
+    gemm16_strip_out<T, BJ0>(mine, pr.gu + half * pr.N, 2 * static_cast<int64_t>(pr.N), pr.M, pr.N, row0, col0, lane);
+  }
+}
+
 // The work of workgroup `bid` of a launch for one product; `lds` is S::kLds bytes, aligned to 1024.
 // pr.tiles_m, pr.tiles_n count tiles of S::kTM x S::kTN.  COLSUM: the sums of A over k as well (see Gemm16Problem).  LN_BWD: see gemm16_deep_ln_bwd.
 // OUT_F32: the result goes to pr.c32.
@@ -352,7 +423,7 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
   // (the divisions ran on the vector unit: back into scalars, which the requests' base addresses are made of)
   tm = __builtin_amdgcn_readfirstlane(tm), tn = __builtin_amdgcn_readfirstlane(tn);
   split = __builtin_amdgcn_readfirstlane(split), batch = __builtin_amdgcn_readfirstlane(batch);
-  const int m0 = tm * S::kTM, n0 = tn * S::kTN;
+  const int m0 = tm * S::kTM, n0 = tn * (S::kGated ? S::kTN / 2 : S::kTN);
   const int k_begin = SPLIT_K ? split * pr.k_per_split : 0;
   const int k_end = SPLIT_K ? min(pr.K, k_begin + pr.k_per_split) : pr.K;
   // A reduction of fewer steps than there are copies ends on steps of zeros.
@@ -362,6 +433,8 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
   const int64_t b_step = B_KC ? S::kBK : S::kBK * ldb;
   const uint16_t* a16 = reinterpret_cast<const uint16_t*>(pr.A) + batch * pr.bsa + (A_KC ? m0 * lda + k_begin : m0 + k_begin * lda);
   const uint16_t* b16 = reinterpret_cast<const uint16_t*>(pr.B) + batch * pr.bsb + (B_KC ? n0 * ldb + k_begin : n0 + k_begin * ldb);
+  const uint16_t* b16_1 = b16;  // of part B1
+  if constexpr (S::kGated) b16_1 += N * ldb;
 
   const int wave = threadIdx.x / kWave;
   const int lane = threadIdx.x % kWave;
@@ -382,8 +455,9 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
   uint32_t src_a0[RA], src_a1[RA], src_b0[RB0], src_b1[RB1];
   gemm16_deep_sources<A_KC, S::kRowsA, NT, 32 * AI, S::kWaveM>(lda, m0, M, 0, src_a0);
   gemm16_deep_sources<A_KC, S::kRowsA, NT, 32 * AI, S::kWaveM>(lda, m0, M, 32 * AI, src_a1);
-  gemm16_deep_sources<B_KC, S::kRowsB0, NT, 32 * BJ0, S::kWaveN>(ldb, n0, N, 0, src_b0);
-  gemm16_deep_sources<B_KC, S::kRowsB1, NT, 32 * BJ1, S::kWaveN>(ldb, n0, N, 32 * BJ0, src_b1);
+  constexpr int kColumns = S::kGated ? 32 * BJ0 : S::kWaveN;  // of a wave
+  gemm16_deep_sources<B_KC, S::kRowsB0, NT, 32 * BJ0, kColumns>(ldb, n0, N, 0, src_b0);
+  gemm16_deep_sources<B_KC, S::kRowsB1, NT, 32 * BJ1, kColumns>(ldb, n0, N, S::kGated ? 0 : 32 * BJ0, src_b1);
   using lds_ptr = __attribute__((address_space(3))) char*;
   const uint32_t lds_wave = __builtin_amdgcn_readfirstlane(
       static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)lds)) + wave * 1024);
@@ -395,7 +469,7 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
     if constexpr (IM == 0) gemm16_deep_issue(a16 + step * a_step, src_a0[i], dst);
     if constexpr (IM == 1) gemm16_deep_issue(a16 + step * a_step, src_a1[i], dst);
     if constexpr (IM == 2) gemm16_deep_issue(b16 + step * b_step, src_b0[i], dst);
-    if constexpr (IM == 3) gemm16_deep_issue(b16 + step * b_step, src_b1[i], dst);
+    if constexpr (IM == 3) gemm16_deep_issue(b16_1 + step * b_step, src_b1[i], dst);
   };
   auto request_short = [&](auto image, int i, int step, int copy, int left) {
     constexpr int IM = decltype(image)::value;
@@ -403,7 +477,7 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
     if constexpr (IM == 0) gemm16_deep_issue_short<A_KC, S::kRowsA, NT>(a16 + step * a_step, src_a0[i], i, left, dst);
     if constexpr (IM == 1) gemm16_deep_issue_short<A_KC, S::kRowsA, NT>(a16 + step * a_step, src_a1[i], i, left, dst);
     if constexpr (IM == 2) gemm16_deep_issue_short<B_KC, S::kRowsB0, NT>(b16 + step * b_step, src_b0[i], i, left, dst);
-    if constexpr (IM == 3) gemm16_deep_issue_short<B_KC, S::kRowsB1, NT>(b16 + step * b_step, src_b1[i], i, left, dst);
+    if constexpr (IM == 3) gemm16_deep_issue_short<B_KC, S::kRowsB1, NT>(b16_1 + step * b_step, src_b1[i], i, left, dst);
   };
 
   uint4 fa[2][AI][4], fb0[BJ0][4], fb1[BJ1][4];  // fragments [block of 32 rows][k-slice of 16]
@@ -500,8 +574,13 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
     if constexpr (HAS_BIAS && !SPLIT_K && LEFT == 0) {  // arrives under the last three phases
 #pragma unroll
       for (int j = 0; j < BJ; ++j) {
-        const int col = n0 + wc * S::kWaveN + j * 32 + lane % 32;
-        bias_v[j] = col < N ? to_float(pr.bias[col]) : 0.f;
+        if constexpr (S::kGated) {
+          const int col = n0 + wc * kColumns + j % BJ0 * 32 + lane % 32;
+          bias_v[j] = col < N ? to_float(pr.bias[j / BJ0 * N + col]) : 0.f;
+        } else {
+          const int col = n0 + wc * S::kWaveN + j * 32 + lane % 32;
+          bias_v[j] = col < N ? to_float(pr.bias[col]) : 0.f;
+        }
       }
     }
     phase(A0{}, B1{}, A1{}, copy, QB0{}, it + 2, copy, is_short, no_sync);
@@ -584,6 +663,15 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
       return;
     }
     uint16_t* mine = reinterpret_cast<uint16_t*>(lds) + wave * 64 * S::kStripStride;
+    if constexpr (S::kGated) {
+#pragma unroll
+      for (int h = 0; h < AI; ++h) {
+        gemm16_deep_gated_write<T, BJ0>(&acc[2 * h], bias_v, mine, static_cast<const GatedProblem<T>&>(pr), row0 + 64 * h,
+                                        n0 + wc * kColumns, lane);
+        __builtin_amdgcn_wave_barrier();
+      }
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < AI; ++h) {
       gemm16_deep_write<T, HAS_BIAS, BJ, AI == 1, S::kMask8>(&acc[2 * h], bias_v, mine, pr.C + at, M, N, pr.ldc, row0 + 64 * h,
@@ -599,6 +687,13 @@ template <typename T, class S, bool A_KC, bool B_KC, bool HAS_BIAS, bool SPLIT_K
 __global__ __launch_bounds__(S::kThreads, S::kOccupancy * S::WN / 2) void gemm_16bit_deep_kernel(Gemm16Problem<T> pr) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
   gemm16_deep_block<T, S, A_KC, B_KC, HAS_BIAS, SPLIT_K, false, false, OUT_F32>(lds, blockIdx.x, pr);
+}
+
+// Both projections of a gated layer and their product.
+template <typename T, class S, bool HAS_BIAS>
+__global__ __launch_bounds__(S::kThreads, S::kOccupancy * S::WN / 2) void gated_deep_kernel(GatedProblem<T> pr) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+  gemm16_deep_block<T, Gemm16DeepGated<S>, true, true, HAS_BIAS, false>(lds, blockIdx.x, pr);
 }
 
 // Both products of a Linear layer's backward in one launch: workgroups [0, n_dw) take the K ranges of
@@ -676,6 +771,26 @@ int launch_linear_bwd_deep(const Gemm16Problem<T>& pw, const Gemm16Problem<T>& p
   else return fail(MG_ERR_INVALID, "linear_bwd: no such tile");
   MG_LAUNCH_CHECK();
   return MG_OK;
+}
+
+template <typename T>
+int launch_gated_deep(const GatedProblem<T>& pr_in, Gemm16Tile tile, hipStream_t stream) {
+  GatedProblem<T> pr = pr_in;
+  auto launch = [&](auto shape) -> int {
+    using S = decltype(shape);
+    const int64_t tiles_m = ceil_div(pr.M, S::kTM), tiles_n = ceil_div(pr.N, S::kTN / 2), grid = tiles_m * tiles_n;
+    // (a launch counts its threads in 32 bits, and a tile's number has 31)
+    if (grid > 0xffffffffLL / S::kThreads) return fail(MG_ERR_INVALID, "gated_linear_fwd: too many output tiles");
+    pr.tiles_m = static_cast<int>(tiles_m), pr.tiles_n = static_cast<int>(tiles_n);
+    const dim3 blocks(static_cast<unsigned>(grid));
+    if (pr.bias) hipLaunchKernelGGL((gated_deep_kernel<T, S, true>), blocks, dim3(S::kThreads), 0, stream, pr);
+    else hipLaunchKernelGGL((gated_deep_kernel<T, S, false>), blocks, dim3(S::kThreads), 0, stream, pr);
+    MG_LAUNCH_CHECK();
+    return MG_OK;
+  };
+  if (tile == kTile256) return launch(Gemm16Deep<2, 2, 2>{});
+  if (tile == kTile128) return launch(Gemm16Deep<1, 1, 1>{});
+  return fail(MG_ERR_INVALID, "gated_linear_fwd: no such tile");
 }
 
 }  // namespace mg

@@ -290,4 +290,7 @@ __device__ __forceinline__ void group_allreduce(float (&v)[K], float* slots, int
   }
 }
 
+// What gradients of a global norm are multiplied by so that it is at most `most`: 1 where it is, or where it is not a number.
+__device__ __forceinline__ float clip_scale(float norm, float most) { return norm > most ? __fdiv_rn(most, norm) : 1.f; }
+
 }  // namespace mg

@@ -82,7 +82,8 @@ PyObject* g_fallbacks = nullptr;      // name -> ctypes wrapper
   X(mg_finish_deferred) X(mg_linear_bwd_deferred) X(mg_layer_norm_bwd_stats_deferred) X(mg_linear_bwd_layer_norm_bwd)     \
   X(mg_scatter_add_deferred) X(mg_flash_attn_fwd) X(mg_flash_attn_bwd) X(mg_flash_attn_fwd_bshd)                          \
   X(mg_flash_attn_bwd_bshd) X(mg_flash_attn_fwd_packed) X(mg_flash_attn_bwd_packed) X(mg_act8_store) X(mg_act8_load)       \
-  X(mg_linear_bwd_act8) X(mg_residual_norm_fwd) X(mg_residual_norm_bwd)
+  X(mg_linear_bwd_act8) X(mg_residual_norm_fwd) X(mg_residual_norm_bwd) X(mg_gated_linear_fwd) X(mg_gated_linear_bwd)      \
+  X(mg_gated_linear_bwd_deferred) X(mg_adam_step_clipped) X(mg_sgd_step_clipped)
 
 struct Lib {
 #define X(f) decltype(&::f) f = nullptr;

@@ -718,6 +718,78 @@ def residual_transformer_step(params, ids, labels, n_heads, scale=1.0, eps=1e-5,
 # --------------------------------------------------------------------------- #
 
 
+# --------------------------------------------------------------------------- #
+# Gated Linear layers, rotary positions, the global norm of gradients
+# --------------------------------------------------------------------------- #
+
+GATES = ("silu", "gelu", "gelu_tanh", "sigmoid", "relu")
+
+
+def gate_act(g, gate):
+    """act(g) and act'(g) in float64."""
+    from scipy.special import erfc, expit
+
+    g = np.asarray(g, np.float64)
+    if gate == "relu":
+        on = (g > 0).astype(np.float64)
+        return g * on, on
+    if gate == "gelu":
+        phi = 0.5 * erfc(-g / np.sqrt(2.0))
+        return g * phi, phi + g * np.exp(-0.5 * g * g) / np.sqrt(2 * np.pi)
+    if gate == "gelu_tanh":
+        c = 2 * np.sqrt(2 / np.pi)
+        z = c * (g + 0.044715 * g ** 3)
+        return g * expit(z), expit(z) + g * expit(z) * expit(-z) * c * (1 + 3 * 0.044715 * g * g)
+    if gate == "sigmoid":
+        return expit(g), expit(g) * expit(-g)
+    return g * expit(g), expit(g) + g * expit(g) * expit(-g)
+
+
+def gated_linear_fwd(x, w, bias, gate):
+    """y (M, F) and g | u (M, 2 F) for w (2 F, K)."""
+    gu = np.asarray(x, np.float64) @ np.asarray(w, np.float64).T + (0.0 if bias is None else np.asarray(bias, np.float64))
+    F = len(w) // 2
+    return gate_act(gu[:, :F], gate)[0] * gu[:, F:], gu
+
+
+def gated_linear_bwd(dy, gu, x, w, gate):
+    """dx, dw, db, and dg | du (M, 2 F)."""
+    dy, gu, x, w = (np.asarray(a, np.float64) for a in (dy, gu, x, w))
+    F = gu.shape[1] // 2
+    act, slope = gate_act(gu[:, :F], gate)
+    d = np.concatenate([dy * gu[:, F:] * slope, dy * act], axis=1)
+    return d @ w, d.T @ x, d.sum(0), d
+
+
+def rotary_pairs(rotated, neighbours):
+    """The two columns of each pair."""
+    i = np.arange(rotated // 2)
+    return (2 * i, 2 * i + 1) if neighbours else (i, i + rotated // 2)
+
+
+def rotary(x, positions, inv_freq, pair_axis, neighbours=False, inverse=False):
+    """x (B, S, H, D) with the pairs turned by positions (axes, B, S) times inv_freq, in float64; and the angles (B, S, pairs)."""
+    x = np.array(x, np.float64)
+    angle = np.moveaxis(np.asarray(positions, np.float64)[np.asarray(pair_axis)], 0, -1) * np.asarray(inv_freq, np.float64)
+    turn = np.exp((-1j if inverse else 1j) * angle)[:, :, None, :]
+    a, b = rotary_pairs(2 * len(inv_freq), neighbours)
+    z = (x[..., a] + 1j * x[..., b]) * turn
+    x[..., a], x[..., b] = z.real, z.imag
+    return x, angle
+
+
+def grad_norm(grads):
+    return float(np.sqrt(sum(np.square(np.asarray(g, np.float64)).sum() for g in grads)))
+
+
+def clip_grads(grads, max_norm):
+    """The global norm, and the gradients scaled down to it."""
+    norm = grad_norm(grads)
+    scale = max_norm / norm if norm > max_norm else 1.0
+    return norm, [np.asarray(g, np.float64) * scale for g in grads]
+
+
+
 def round_class(nbytes: int) -> int:
     """mograd/memory.mojo:59-72."""
     if nbytes <= 512:
