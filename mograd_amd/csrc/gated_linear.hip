@@ -1,6 +1,10 @@
 // C ABI of the gated Linear layer: argument checks, the choice of kernels, the gradient of the gate.
 #include "gated_linear.h"
 
+#include <cmath>
+
+#include "gated_direct.h"
+#include "gemm_16bit_small.h"
 #include "gemm_pad.h"
 #include "mg_deferred.h"
 #include "mg_rows.h"
@@ -84,22 +88,137 @@ static int gate_bwd(const void* dy, const void* gu, void* dgu, int64_t M, int64_
   });
 }
 
-// 16 bits: both projections and y in one launch; y comes from the projections before they are rounded.
+// Which kernel a forward pass takes: the least of these estimates, in us.  kGatedDirect: gated_direct.h; kGatedSmall: 64 x 64 tiles, K in
+// ranges; kGatedDeep: 128 x 128 or 256 x 256 tiles, which copy ragged operands first (a launch, and two passes over them); kGatedApart
+// (fp32): a plain product, then the gate.  Fitted to 800 shapes of 1 to 20000 rows, 32 to 8192 inputs and 32 to 12000 outputs, weights from
+// memory, each by every way: over them the way taken is 1.4 % slower than each one's best for 16 bits on 16-byte chunks, 2.6 % off them, and
+// 4.6 % in fp32 (for 16 bits, 64 x 64 tiles up to 64 rows and 128 x 128 above: 31 %).  Whether the projections are kept, which is one value
+// stored or three, is not looked at, so that y is the same either way.  `values`: two an output.
+enum GatedWay { kGatedDirect, kGatedSmall, kGatedDeep, kGatedApart };
+struct GatedChoice {
+  GatedWay way;
+  int tile;  // kGatedDirect: 16 or 32 rows; kGatedDeep: a Gemm16Tile
+  int splits;
+  double us;
+};
+static double gated_direct_us(int64_t M, int64_t F, int64_t K, double values, bool f32, bool ragged, double cus) {
+  const int rows = M <= 16 ? 16 : 32;
+  const double size = f32 ? 4 : 2, wgs = static_cast<double>(ceil_div(F, 16) * ceil_div(M, rows)), per_cu = std::ceil(wgs / cus);
+  const double wg_kb = static_cast<double>(K) * size * (32 + rows) / 1e3, weights_mb = 2.0 * F * K * size / 1e6;
+  const double again = static_cast<double>(ceil_div(M, rows));  // the weights come once from memory, then from caches
+  if (f32) {
+    const double step = rows == 16 ? 0.0183 : 0.0245, read = rows == 16 ? 0.2204 : 0.2634;
+    return (rows == 16 ? 3.6 : 4.0) + std::max(step * wg_kb * per_cu, read * weights_mb * again) + 1.1 * values * size / 1e6;
+  }
+  const double step = (rows == 16 ? 0.016 : 0.0193) * (ragged ? 3.0 : 1.0), read = rows == 16 ? 0.156 : 0.2137;
+  return 2.9 + std::max(step * wg_kb * per_cu, read * weights_mb * std::pow(again, 0.89)) + 1.7 * values * size / 1e6;
+}
+static GatedChoice choose_gated_16bit(int64_t M, int64_t F, int64_t K, bool ragged) {
+  const double cus = device_info().cu_count, values = 2.0 * M * F, out = values * 2 / 1e6;
+  const double steps = static_cast<double>(ceil_div(K, 64)), weights_mb = 4.0 * F * K / 1e6;
+  constexpr int64_t kTiles = 1 << 23;  // of a launch, which counts its threads in 32 bits
+  GatedChoice best{kGatedDirect, M <= 16 ? 16 : 32, 1, gated_direct_us(M, F, K, values, false, ragged, cus)};
+  if (ceil_div(F, 16) * ceil_div(M, M <= 16 ? 16 : 32) > kTiles) best.us = 1e30;
+  auto offer = [&](GatedWay way, int tile, int splits, double us) {
+    if (us < best.us) best = GatedChoice{way, tile, splits, us};
+  };
+  if (const int64_t tiles = ceil_div(M, 64) * ceil_div(F, 32); (!ragged || K >= 8) && tiles <= kTiles) {
+    for (int s = 1; s <= 16 && (s == 1 || (K >= 256 * s && tiles * s <= 1024)); ++s) {
+      const double per_cu = std::ceil(static_cast<double>(tiles) * s / cus), walk = std::ceil(steps / s), parts = static_cast<double>(tiles) * s * 4096 / 1e6;
+      const double us = ragged ? 3.04 + walk * (per_cu > 1 ? 0.292 * per_cu : 0.382) + 0.252 * out + 0.588 * (per_cu - 1) + (s > 1 ? 2.96 + 1.97 * parts : 0.0)
+                               : 2.97 + walk * (per_cu > 1 ? 0.238 * per_cu : 0.232) + 0.191 * out + 0.475 * (per_cu - 1) + (s > 1 ? 3.16 + 1.6 * parts : 0.0);
+      offer(kGatedSmall, 64, s, std::max(us, 3.0 + (ragged ? 0.354 : 0.215) * weights_mb));
+    }
+  }
+  const double copies = ragged ? 2.4 + (static_cast<double>(M) * K + 2.0 * F * K) / 1e6 : 0.0;
+  if (const int64_t tiles = ceil_div(M, 128) * ceil_div(F, 64); tiles <= kTiles) {
+    const double per_cu = std::ceil(tiles / cus), pairs = std::floor(per_cu / 2), odd = per_cu - 2 * pairs, lines = K % 64 != 0 && K >= 512 ? 1.256 : 1.0;
+    offer(kGatedDeep, kTile128, 1, copies + 3.83 + std::max(2.0, steps) * lines * (0.936 * pairs + (pairs == 0 ? 0.366 : 0.315) * odd) + 0.288 * out + 0.295 * (pairs + odd));
+  }
+  const double tiles = static_cast<double>(ceil_div(M, 256) * ceil_div(F, 128));
+  offer(kGatedDeep, kTile256, 1, copies + 5.92 + std::ceil(tiles / cus) * ((tiles < 0.75 * cus ? 1.096 : 1.367) * std::max(2.0, steps) + 3.66) + 0.328 * out);
+  // MOGRAD_HIP_GATED_TILE = 16 (straight from memory) | 64 | 128 | 256 and MOGRAD_HIP_GATED_SPLITS override the choice.
+  if (env_str("MOGRAD_HIP_GATED_TILE")) {
+    const int only = env_int("MOGRAD_HIP_GATED_TILE", 0);
+    if (only == 16) return GatedChoice{kGatedDirect, M <= 16 ? 16 : 32, 1, 0.0};
+    if (only == 64 && (!ragged || K >= 8)) return GatedChoice{kGatedSmall, 64, std::max(1, env_int("MOGRAD_HIP_GATED_SPLITS", 1)), 0.0};
+    return GatedChoice{kGatedDeep, only == 256 ? kTile256 : kTile128, 1, 0.0};
+  }
+  return best;
+}
+// The plain product's time by its FLOP, the values it leaves and the weights that it reads, within a sixth for most.
+static GatedChoice choose_gated_f32(int64_t M, int64_t F, int64_t K) {
+  const double cus = device_info().cu_count, values = 2.0 * M * F;
+  const double direct = gated_direct_us(M, F, K, values, true, false, cus);
+  const double apart = 6.0 + 11.4 * 4e-9 * M * F * K + 0.45 * values * 4 / 1e6 + 0.29 * 8.0 * F * K / 1e6 + 0.88 * K / 1e3;
+  const int only = env_int("MOGRAD_HIP_GATED_TILE", 0);
+  const bool few = ceil_div(F, 16) * ceil_div(M, 32) <= 1 << 22;
+  if (only == 16 || (only == 0 && direct < apart && few)) return GatedChoice{kGatedDirect, M <= 16 ? 16 : 32, 1, direct};
+  return GatedChoice{kGatedApart, 0, 1, apart};
+}
+
+template <typename T>
+static int launch_gated_direct(const void* x, const void* w, const void* bias, void* y, void* gu, int64_t M, int64_t F, int64_t K, int gate,
+                               int rows, hipStream_t stream) {
+  const int64_t tiles_f = ceil_div(F, 16), blocks = tiles_f * ceil_div(M, rows);
+  constexpr int kThreads = 64 * kGatedDirectWaves;
+  if (blocks > 0xffffffffLL / kThreads) return fail(MG_ERR_INVALID, "gated_linear_fwd: too many output tiles");
+  const GatedDirect<T> p{static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), static_cast<T*>(y), static_cast<T*>(gu),
+                         static_cast<int>(M), static_cast<int>(F), static_cast<int>(K), static_cast<int>(tiles_f), gate};
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (rows == 16) hipLaunchKernelGGL((gated_direct_kernel<T, 1>), grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((gated_direct_kernel<T, 2>), grid, dim3(kThreads), 0, stream, p);
+  MG_LAUNCH_CHECK();
+  return MG_OK;
+}
+
+// 64 x 64 tiles (32 columns of y), K in `splits` ranges.  ANY: operands of any alignment, K at least 8.
+template <typename T, bool ANY>
+static int launch_gated_small(GatedProblem<T> pr, int splits, hipStream_t stream) {
+  const int64_t tiles_m = ceil_div(pr.M, kSmallT), tiles_n = ceil_div(pr.N, kSmallT / 2), tiles = tiles_m * tiles_n;
+  const int k_per_split = static_cast<int>(ceil_div(ceil_div(pr.K, splits), kSmallBK) * kSmallBK);
+  splits = static_cast<int>(ceil_div(pr.K, k_per_split));
+  const int64_t grid = splits > 1 ? gemm_split_grid(tiles, splits, 1) : tiles;
+  if (grid > 0xffffffffLL / 256) return fail(MG_ERR_INVALID, "gated_linear_fwd: too many output tiles");
+  Scratch partial;
+  if (splits > 1) MG_TRY(partial.take(splits * tiles * kSmallT * kSmallT * static_cast<int64_t>(sizeof(float))));
+  pr.partial = partial.as<float>(), pr.tiles_m = static_cast<int>(tiles_m), pr.tiles_n = static_cast<int>(tiles_n);
+  pr.splits = splits, pr.k_per_split = k_per_split;
+  const dim3 blocks(static_cast<unsigned>(grid));
+  if (splits == 1) {
+    hipLaunchKernelGGL((gated_small_kernel<T, false, ANY>), blocks, dim3(256), 0, stream, pr);
+    MG_LAUNCH_CHECK();
+    return MG_OK;
+  }
+  hipLaunchKernelGGL((gated_small_kernel<T, true, ANY>), blocks, dim3(256), 0, stream, pr);
+  MG_LAUNCH_CHECK();
+  hipLaunchKernelGGL((gated_small_sum_kernel<T>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, stream, pr);
+  MG_LAUNCH_CHECK();
+  return MG_OK;
+}
+
+// 16 bits: both projections and y in one launch (two where K is in ranges); y comes from the projections before they are rounded.
 template <typename T>
 static int gated_fwd_16bit(const void* x, const void* w, const void* bias, void* y, void* gu, int64_t M, int64_t F, int64_t K, int gate,
                            hipStream_t stream) {
+  const bool ragged = K % 8 != 0 || !aligned16(x) || !aligned16(w);
+  const GatedChoice choice = choose_gated_16bit(M, F, K, ragged);
+  if (choice.way == kGatedDirect) return launch_gated_direct<T>(x, w, bias, y, gu, M, F, K, gate, choice.tile, stream);
   int64_t ldx = K, ldw = K, no_batch = 0;
   PadCopies<T> pads;
-  if (K % 8 != 0 || !aligned16(x)) MG_TRY(pads.add(&x, 1, M, K, &ldx, &no_batch));
-  if (K % 8 != 0 || !aligned16(w)) MG_TRY(pads.add(&w, 1, 2 * F, K, &ldw, &no_batch));
-  MG_TRY(pads.launch(stream));
+  if (choice.way == kGatedDeep) {
+    if (K % 8 != 0 || !aligned16(x)) MG_TRY(pads.add(&x, 1, M, K, &ldx, &no_batch));
+    if (K % 8 != 0 || !aligned16(w)) MG_TRY(pads.add(&w, 1, 2 * F, K, &ldw, &no_batch));
+    MG_TRY(pads.launch(stream));
+    K = ceil_div(K, 8) * 8;  // (zeros behind K in an image)
+  }
   GatedProblem<T> pr{};
   pr.A = static_cast<const T*>(x), pr.B = static_cast<const T*>(w), pr.bias = static_cast<const T*>(bias), pr.C = static_cast<T*>(y);
-  pr.M = static_cast<int>(M), pr.N = static_cast<int>(F), pr.K = static_cast<int>(ceil_div(K, 8) * 8);  // (zeros behind K in an image)
+  pr.M = static_cast<int>(M), pr.N = static_cast<int>(F), pr.K = static_cast<int>(K);
   pr.lda = ldx, pr.ldb = ldw, pr.ldc = F, pr.batches = pr.splits = 1, pr.k_per_split = pr.K;
   pr.gu = static_cast<T*>(gu), pr.gate = gate;
-  const int64_t large = ceil_div(M, 256) * ceil_div(F, 128);
-  return launch_gated_deep<T>(pr, 2 * large >= device_info().cu_count ? kTile256 : kTile128, stream);
+  if (choice.way == kGatedDeep) return launch_gated_deep<T>(pr, static_cast<Gemm16Tile>(choice.tile), stream);
+  return ragged ? launch_gated_small<T, true>(pr, choice.splits, stream) : launch_gated_small<T, false>(pr, choice.splits, stream);
 }
 
 static int gated_check(const char* who, int64_t M, int64_t F, int64_t K, int gate, int dtype) {
@@ -169,7 +288,9 @@ int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y,
     MG_TRY(hold.begin(s));
     if (dtype == MG_BF16) return mg::gated_fwd_16bit<mg::bf16_t>(x, w, bias, y, gu, M, F, K, gate, s);
     if (dtype == MG_F16) return mg::gated_fwd_16bit<mg::f16_t>(x, w, bias, y, gu, M, F, K, gate, s);
-    // fp32: the projections as one product, whose values are not rounded on the way; 3 M F values of 2 (K + 1) M F products' time.
+    const mg::GatedChoice choice = mg::choose_gated_f32(M, F, K);
+    if (choice.way == mg::kGatedDirect) return mg::launch_gated_direct<float>(x, w, bias, y, gu, M, F, K, gate, choice.tile, s);
+    // the projections as one product, whose values are not rounded on the way; 3 M F values of 2 (K + 1) M F products' time.
     mg::Scratch kept;
     if (!gu) {
       MG_TRY(kept.take(M * 2 * F * static_cast<int64_t>(sizeof(float))));

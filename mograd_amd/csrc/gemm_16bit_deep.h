@@ -101,10 +101,9 @@ __device__ __forceinline__ void gemm16_deep_issue_short(const uint16_t* base, ui
 
 // A wave's 64 x (32 BJ) values into its strip of LDS, rounded.  The accumulators have lanes along n and
 // registers along m; two lanes with neighbouring columns swap packed pairs of rows (see gemm16_write_tile).
-template <typename T, bool HAS_BIAS, bool RELU, int BJ>
-__device__ __forceinline__ void gemm16_deep_stage(const floatx16 (*acc)[BJ], const float (&bias_v)[BJ],
-                                                  uint16_t* __restrict__ mine, int lane) {
-  constexpr int STRIDE = 32 * BJ + 8;
+// `value`: (row block, column block, register) to a value.
+template <typename T, int BJ, typename V, int STRIDE = 32 * BJ + 8>
+__device__ __forceinline__ void gemm16_deep_stage_values(V&& value, uint16_t* __restrict__ mine, int lane) {
   const int odd = lane & 1;
   const uint32_t select = odd ? 0x03020706u : 0x05040100u;
   uint32_t* const base32 = reinterpret_cast<uint32_t*>(mine + ((lane / 32) * 4 + odd) * STRIDE + (lane % 32 - odd));
@@ -114,17 +113,23 @@ __device__ __forceinline__ void gemm16_deep_stage(const floatx16 (*acc)[BJ], con
     for (int tj = 0; tj < BJ; ++tj)
 #pragma unroll
       for (int rp = 0; rp < 8; ++rp) {  // rows 2 rp and 2 rp + 1 of the sixteen
-        float f0 = acc[ti][tj][2 * rp], f1 = acc[ti][tj][2 * rp + 1];
-        if constexpr (HAS_BIAS) f0 += bias_v[tj], f1 += bias_v[tj];
-        if constexpr (RELU) {
-          f0 = f0 > 0.f ? f0 : 0.f;
-          f1 = f1 > 0.f ? f1 : 0.f;
-        }
-        const uint32_t w = gemm16_pack2<T>(f0, f1);
+        const uint32_t w = gemm16_pack2<T>(value(ti, tj, 2 * rp), value(ti, tj, 2 * rp + 1));
         const uint32_t y = __builtin_amdgcn_update_dpp(w, w, kDppQuadXor1, 0xf, 0xf, false);
         const int rl = ti * 32 + (rp / 2) * 8 + (rp % 2) * 2;
         base32[(rl * STRIDE + tj * 32) / 2] = __builtin_amdgcn_perm(y, w, select);
       }
+}
+template <typename T, bool HAS_BIAS, bool RELU, int BJ>
+__device__ __forceinline__ void gemm16_deep_stage(const floatx16 (*acc)[BJ], const float (&bias_v)[BJ],
+                                                  uint16_t* __restrict__ mine, int lane) {
+  gemm16_deep_stage_values<T, BJ>(
+      [&](int ti, int tj, int r) {
+        float f = acc[ti][tj][r];
+        if constexpr (HAS_BIAS) f += bias_v[tj];
+        if constexpr (RELU) f = f > 0.f ? f : 0.f;
+        return f;
+      },
+      mine, lane);
 }
 
 // Output of a wave's 64 x (32 BJ) values (two rows of accumulator blocks): through the wave's own strip of LDS
@@ -343,8 +348,8 @@ __device__ __forceinline__ void gemm16_deep_ln_bwd(const floatx16 (&acc)[2][S::B
   }
 }
 
-// Rows of a wave's strip (64 x 32 BJ rounded values) to C, 16 bytes per lane, whole rows one after the other.
-template <typename T, int BJ>
+// Rows of a wave's strip (64 x 32 BJ rounded values) to C, 16 bytes per lane, whole rows one after the other.  NT: past the caches.
+template <typename T, int BJ, bool NT>
 __device__ __forceinline__ void gemm16_strip_out(const uint16_t* __restrict__ mine, T* __restrict__ C, int64_t ldc, int M, int N,
                                                  int row0, int col0, int lane) {
   constexpr int STRIDE = 32 * BJ + 8, CPR = 4 * BJ;
@@ -365,42 +370,31 @@ __device__ __forceinline__ void gemm16_strip_out(const uint16_t* __restrict__ mi
       continue;
     }
     const gemm_u4_any out = {v.x, v.y, v.z, v.w};
-    *reinterpret_cast<gemm_u4_any*>(at) = out;
+    if constexpr (NT) __builtin_nontemporal_store(out, reinterpret_cast<gemm_u4_any*>(at));
+    else *reinterpret_cast<gemm_u4_any*>(at) = out;
   }
 }
 
-// Output of a wave's 64 rows of a gated layer: y = act(g) u from the unrounded projections, and these where they are kept.
+// Output of a wave's 64 rows of a gated layer: y = act(g) u from the unrounded projections, and these where they are kept.  Those are read
+// in the backward pass, when no cache holds them any more: stored past the caches they leave the operands there ((16384, 1024 <- 384) bf16
+// 56.1 -> 42.4 us, (8192, 2048 <- 768) 67.6 -> 63.7), where y, which the next product reads, gains nothing by it (44.6, 63.4).
 template <typename T, int BJ0>
 __device__ __forceinline__ void gemm16_deep_gated_write(const floatx16 (*acc)[2 * BJ0], const float (&bias_v)[2 * BJ0],
                                                        uint16_t* __restrict__ mine, const GatedProblem<T>& pr, int row0, int col0,
                                                        int lane) {
-  floatx16 part[2][BJ0];
-  const float none[BJ0] = {};
-  gated_with(pr.gate, [&](auto gate) {
-#pragma unroll
-    for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-      for (int tj = 0; tj < BJ0; ++tj)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          part[ti][tj][r] = gated_act<true, decltype(gate)::value>(acc[ti][tj][r] + bias_v[tj]) * (acc[ti][BJ0 + tj][r] + bias_v[BJ0 + tj]);
+  gated_with_fast(pr.gate, [&](auto act) {
+    gemm16_deep_stage_values<T, BJ0>(
+        [&](int ti, int tj, int r) { return act(acc[ti][tj][r] + bias_v[tj]) * (acc[ti][BJ0 + tj][r] + bias_v[BJ0 + tj]); }, mine, lane);
   });
-  gemm16_deep_stage<T, false, false, BJ0>(part, none, mine, lane);
   __builtin_amdgcn_wave_barrier();  // the strip is the wave's own: its LDS accesses are in order
-  gemm16_strip_out<T, BJ0>(mine, pr.C, pr.N, pr.M, pr.N, row0, col0, lane);
+  gemm16_strip_out<T, BJ0, false>(mine, pr.C, pr.N, pr.M, pr.N, row0, col0, lane);
   if (!pr.gu) return;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-      for (int tj = 0; tj < BJ0; ++tj)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) part[ti][tj][r] = acc[ti][half * BJ0 + tj][r] + bias_v[half * BJ0 + tj];
-    gemm16_deep_stage<T, false, false, BJ0>(part, none, mine, lane);
+    gemm16_deep_stage_values<T, BJ0>([&](int ti, int tj, int r) { return acc[ti][half * BJ0 + tj][r] + bias_v[half * BJ0 + tj]; }, mine, lane);
     __builtin_amdgcn_wave_barrier();
-    gemm16_strip_out<T, BJ0>(mine, pr.gu + half * pr.N, 2 * static_cast<int64_t>(pr.N), pr.M, pr.N, row0, col0, lane);
+    gemm16_strip_out<T, BJ0, true>(mine, pr.gu + half * pr.N, 2 * static_cast<int64_t>(pr.N), pr.M, pr.N, row0, col0, lane);
   }
 }
 
@@ -664,12 +658,14 @@ __device__ __forceinline__ void gemm16_deep_block(char* lds, int bid, const Gemm
     }
     uint16_t* mine = reinterpret_cast<uint16_t*>(lds) + wave * 64 * S::kStripStride;
     if constexpr (S::kGated) {
-#pragma unroll
-      for (int h = 0; h < AI; ++h) {
-        gemm16_deep_gated_write<T, BJ0>(&acc[2 * h], bias_v, mine, static_cast<const GatedProblem<T>&>(pr), row0 + 64 * h,
-                                        n0 + wc * kColumns, lane);
+      // (written out: a loop over so much code is left as one, and the accumulators then go to memory)
+      auto half = [&](auto h) {
+        gemm16_deep_gated_write<T, BJ0>(&acc[2 * decltype(h)::value], bias_v, mine, static_cast<const GatedProblem<T>&>(pr),
+                                        row0 + 64 * decltype(h)::value, n0 + wc * kColumns, lane);
         __builtin_amdgcn_wave_barrier();
-      }
+      };
+      half(std::integral_constant<int, 0>{});
+      if constexpr (AI == 2) half(std::integral_constant<int, 1>{});
       return;
     }
 #pragma unroll

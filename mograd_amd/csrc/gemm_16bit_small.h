@@ -10,6 +10,7 @@
 // Copies, LDS images, partial tiles and the order of every sum are those of gemm16_deep_block.
 #pragma once
 
+#include "gated_linear.h"
 #include "gemm_impl.h"
 
 namespace mg {
@@ -110,6 +111,87 @@ __device__ __forceinline__ void gemm16_small_write(const floatx16& acc, uint16_t
   }
 }
 
+// A gated Linear layer (GATED below): a tile's first 32 columns are those of y from its first one on as rows of the gate's weights, its
+// last 32 the same rows of the other ones.  `line` of a tile whose columns of y begin at o0 of O:
+__device__ __forceinline__ int64_t gated_small_row(int line, int o0, int O) {
+  return min(o0 + line % 32, O - 1) + (line < 32 ? 0 : static_cast<int64_t>(O));
+}
+
+// Its output: the four waves' values meet in LDS as they are, a thread takes eight columns of y of one row.  SPLIT_K: the range's sums go
+// to scratch as the waves hold them, [range][tile][wave][register / 4][lane][register % 4], for gated_small_sum_kernel.
+constexpr int kGatedSmallStride = 68;  // floats of a row in LDS
+template <typename T>
+__device__ __forceinline__ void gated_small_out(const GatedProblem<T>& pr, int row, int col, float (&g)[8], float (&u)[8]) {
+  const int n = min(8, pr.N - col);
+  if (pr.bias) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) g[e] += to_float(pr.bias[col + e]), u[e] += to_float(pr.bias[pr.N + col + e]);
+  }
+  T* const y = pr.C + static_cast<int64_t>(row) * pr.N + col;
+  T* const gu = pr.gu + static_cast<int64_t>(row) * 2 * pr.N + col;
+  float v[8];
+  gated_with_fast(pr.gate, [&](auto act) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = act(g[e]) * u[e];
+  });
+  if (n == 8) {
+    gemm16_store8(y, v);
+    if (pr.gu) gemm16_store8(gu, g), gemm16_store8(gu + pr.N, u);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 7; ++e)
+    if (e < n) {
+      y[e] = from_float<T>(v[e]);
+      if (pr.gu) gu[e] = from_float<T>(g[e]), gu[pr.N + e] = from_float<T>(u[e]);
+    }
+}
+template <typename T, bool SPLIT_K>
+__device__ __forceinline__ void gated_small_write(const floatx16& acc, float* __restrict__ lds, const GatedProblem<T>& pr, int tile, int split,
+                                                  int m0, int n0, int wave, int lane) {
+  if constexpr (SPLIT_K) {
+    floatx4* const dst = reinterpret_cast<floatx4*>(pr.partial) +
+                         ((static_cast<int64_t>(split) * pr.tiles_m * pr.tiles_n + tile) * 4 + wave) * 256 + lane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) dst[q * 64] = floatx4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    lds[((wave / 2) * 32 + (r / 4) * 8 + (lane / 32) * 4 + r % 4) * kGatedSmallStride + (wave % 2) * 32 + lane % 32] = acc[r];
+  __syncthreads();
+  const int rl = threadIdx.x / 4, cl = threadIdx.x % 4 * 8, row = m0 + rl, col = n0 + cl;
+  if (row >= pr.M || col >= pr.N) return;
+  const float* const at = lds + rl * kGatedSmallStride + cl;
+  float g[8], u[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) g[e] = at[e], u[e] = at[32 + e];
+  gated_small_out<T>(pr, row, col, g, u);
+}
+
+// The ranges' sums, added in order, and y from them: a workgroup a tile.
+template <typename T>
+__global__ __launch_bounds__(256) void gated_small_sum_kernel(GatedProblem<T> pr) {
+  __shared__ float lds[64 * kGatedSmallStride];
+  int tm, tn;
+  const int tile = blockIdx.x, tiles = pr.tiles_m * pr.tiles_n;
+  gemm_tile_of_block(tile, pr.tiles_m, pr.tiles_n, tm, tn, false);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const floatx4* const src = reinterpret_cast<const floatx4*>(pr.partial) + (static_cast<int64_t>(tile) * 4 + wave) * 256 + lane;
+  floatx16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  for (int s = 0; s < pr.splits; ++s)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const floatx4 v = src[static_cast<int64_t>(s) * tiles * 1024 + q * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * q + e] += v[e];
+    }
+  gated_small_write<T, false>(acc, lds, pr, tile, 0, tm * kSmallT, tn * (kSmallT / 2), wave, lane);
+}
+
 // What a thread carries of an operand that does not lie on 16-byte chunks: its chunks of a step, read from any address
 // (extents along the contiguous axis: at least 8).  A chunk that reaches past the end of its row is read as the sixteen
 // bytes that end it and moved down when it is put into LDS, so that no load stands under a condition and none is waited
@@ -127,13 +209,16 @@ struct SmallAnySource {
     line = slot / 8;
     chunk = (slot % 8) ^ (KC ? (line / 2) % 8 : gemm16_tr_swizzle<kSmallT>(line));
   }
+  // GATED: see gated_small_row.
+  template <bool GATED = false>
   __device__ __forceinline__ void init(const uint16_t* base_, int64_t ld_, int o0_, int O_, int k_begin_, int K_) {
     base = base_, ld = ld_, o0 = o0_, O = O_, k_begin = k_begin_, K = K_;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       int line, chunk;
       place(i, line, chunk);
-      row[i] = KC ? base + static_cast<int64_t>(min(o0 + line, O - 1)) * ld + k_begin + chunk * 8
+      if constexpr (GATED) row[i] = base + gated_small_row(line, o0, O) * ld + k_begin + chunk * 8;
+      else row[i] = KC ? base + static_cast<int64_t>(min(o0 + line, O - 1)) * ld + k_begin + chunk * 8
                   : base + static_cast<int64_t>(k_begin + line) * ld + min(o0 + chunk * 8, O - 8);
     }
   }
@@ -186,7 +271,8 @@ struct SmallAnySource {
 // they cost a launch and a pass of 5 us, and the 128 x 128 kernel that stages them leaves CUs idle: (700, 701 <- 703) bf16
 // forward + backward 38.7 -> 20.6 us, (2048, 1000 <- 1001) forward 20.7 -> 15.1.  A step takes a third longer than a copied one,
 // misaligned chunks being two of the memory path's; more steps under way (four) measured the same.
-template <typename T, bool A_KC, bool B_KC, bool HAS_BIAS, bool SPLIT_K, bool COLSUM, bool MAY_F32 = COLSUM, bool ANY = false>
+template <typename T, bool A_KC, bool B_KC, bool HAS_BIAS, bool SPLIT_K, bool COLSUM, bool MAY_F32 = COLSUM, bool ANY = false,
+          bool GATED = false>
 __device__ __forceinline__ void gemm16_small_block(char* lds, int bid, const Gemm16Problem<T>& pr) {
   constexpr int TT = kSmallT, BK = kSmallBK, NSTAGE = kSmallStages, NW = 4;
   constexpr int NI = gemm16_pipe_requests(TT, BK, NW);  // copy requests per thread, operand and step
@@ -201,7 +287,7 @@ __device__ __forceinline__ void gemm16_small_block(char* lds, int bid, const Gem
   }
   int tm, tn;
   gemm_tile_of_block(tile, pr.tiles_m, pr.tiles_n, tm, tn, !SPLIT_K);
-  const int m0 = tm * TT, n0 = tn * TT;
+  const int m0 = tm * TT, n0 = tn * (GATED ? TT / 2 : TT);
   const int k_begin = SPLIT_K ? split * pr.k_per_split : 0;
   const int k_end = SPLIT_K ? min(K, k_begin + pr.k_per_split) : K;
   const int full_steps = (k_end - k_begin) / BK, rem = (k_end - k_begin) % BK;
@@ -240,10 +326,19 @@ __device__ __forceinline__ void gemm16_small_block(char* lds, int bid, const Gem
   uint4 va[2][NI], vb[2][NI];  // ANY: the steps under way
   if constexpr (ANY) {
     any_a.init(reinterpret_cast<const uint16_t*>(pr.A + batch * pr.bsa), pr.lda, m0, M, k_begin, K);
-    any_b.init(reinterpret_cast<const uint16_t*>(pr.B + batch * pr.bsb), pr.ldb, n0, N, k_begin, K);
+    any_b.template init<GATED>(reinterpret_cast<const uint16_t*>(pr.B + batch * pr.bsb), pr.ldb, n0, N, k_begin, K);
   } else {
     gemm16_pipe_sources<A_KC, BK, TT, NW>(pr.lda, m0, M, src_a);
-    gemm16_pipe_sources<B_KC, BK, TT, NW>(pr.ldb, n0, N, src_b);
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        int line, chunk;
+        SmallAnySource<true>::place(i, line, chunk);
+        src_b[i] = gated_small_row(line, n0, N) * pr.ldb + chunk * 8;
+      }
+    } else {
+      gemm16_pipe_sources<B_KC, BK, TT, NW>(pr.ldb, n0, N, src_b);
+    }
   }
   auto fetch = [&](int set, int step) {
     any_a.fetch(step, va[set]);
@@ -361,6 +456,10 @@ __device__ __forceinline__ void gemm16_small_block(char* lds, int bid, const Gem
     multiply(0);
   }
   __syncthreads();  // every wave is done with the staged tiles: their memory serves the output
+  if constexpr (GATED) {
+    gated_small_write<T, SPLIT_K>(acc, reinterpret_cast<float*>(lds), static_cast<const GatedProblem<T>&>(pr), tile, split, m0, n0, wave, lane);
+    return;
+  }
 
   if constexpr (COLSUM) {
     if (colsum && lane % 32 == 0) {  // every column holds the sums
@@ -383,6 +482,13 @@ __global__ __launch_bounds__(256, 2) void gemm_16bit_small_kernel(Gemm16Problem<
   __shared__ __attribute__((aligned(1024))) char lds[kSmallLdsBytes];
   // (dW = dY^T X is the layout that fp32 weight gradients come in)
   gemm16_small_block<T, A_KC, B_KC, HAS_BIAS, SPLIT_K, false, !A_KC && !B_KC && !HAS_BIAS, ANY>(lds, blockIdx.x, pr);
+}
+
+// Both projections of a gated layer of few tiles, and their product.
+template <typename T, bool SPLIT_K, bool ANY>
+__global__ __launch_bounds__(256, 2) void gated_small_kernel(GatedProblem<T> pr) {
+  __shared__ __attribute__((aligned(1024))) char lds[kSmallLdsBytes];
+  gemm16_small_block<T, true, true, false, SPLIT_K, false, false, ANY, true>(lds, blockIdx.x, pr);
 }
 
 // dX and dW (with db, the column sums of dY) of a Linear layer in one launch, see

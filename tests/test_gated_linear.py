@@ -189,6 +189,23 @@ def test_forward(device, M, F, K, dtype):
         _check_forward(p, _forward(device, p, dtype, gate, offset=1), dtype, gate)
 
 
+# the kernels that a forward pass chooses between, each at shapes that it may not be chosen for
+WAYS = [("16", "1"), ("64", "1"), ("64", "3"), ("128", "1"), ("256", "1")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("M,F,K", [(1, 1, 1), (5, 3, 7), (1, 100, 130), (16, 16, 32), (17, 40, 1000), (65, 33, 264), (130, 129, 65), (260, 140, 520), (300, 70, 777)])
+def test_forward_every_way(device, monkeypatch, M, F, K, dtype):
+    p = _inputs(430, M, F, K, dtype)
+    for tile, splits in WAYS:
+        monkeypatch.setenv("MOGRAD_HIP_GATED_TILE", tile)
+        monkeypatch.setenv("MOGRAD_HIP_GATED_SPLITS", splits)
+        for gate in ("silu", "gelu", "relu"):
+            for offset in (0, 1):
+                _check_forward(p, _forward(device, p, dtype, gate, offset=offset), dtype, gate)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,grads", [(F32, F32), (F16, F16), (BF16, BF16), (BF16, F32)])
 @pytest.mark.parametrize("M,F,K", SHAPES)
