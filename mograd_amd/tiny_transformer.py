@@ -39,16 +39,26 @@ Options that the reference's model does not have:
     act8=True            the activations that only the weight gradients and the post norms' backward read (x1, x2, the ReLU's
                          output, and with post_norm the blocks' outputs) are kept in 8 bits (mg_act8_store, or written so by
                          mg_residual_norm_fwd) and multiplied from there (mg_linear_bwd_act8): `kept_bytes` says what that saves.
+    gated_ff=GATE_SILU   the MLP is W2 (act(Wg x + bg) * (Wu x + bu)), its gate passed through one of GATE_SILU, GATE_GELU,
+                         GATE_GELU_TANH, GATE_SIGMOID, GATE_RELU: w1 (2 ff, d) is Wg over Wu and b1 (2 ff) bg, bu.  Both projections and
+                         their product are one call, mg_gated_linear_fwd, their gradients another, mg_gated_linear_bwd.  (With
+                         act8, x2 and the projections stay as they are: their gradients are not taken from 8 bits.)
+    rotary_base=10000.   queries and keys are turned by their tokens' positions (mg_rotary), pair i of a head's columns by
+                         position * rotary_base^(-2 i / dh), before attention, and their gradients back.  rotary_axes: positions a
+                         token, which go to as many runs of pairs; step() takes them, or 0 .. T-1 for one axis.
+
+adam_step(max_norm=1.0) scales the gradients down to a global norm of at most max_norm on their way into the update (mg_grad_norm,
+mg_adam_step_clipped); `grad_norm` holds what it was.
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Dict, List, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import numpy as np
 
-from ._lib import BF16, F32, I32, I64, DTYPE_SIZE
+from ._lib import BF16, F32, GATE_RELU, GATE_SILU, I32, I64, DTYPE_SIZE
 from .runtime import AnyBuffer, Device, MogradError
 
 BLOCK_PARAMS = ("ln1_g", "ln1_b", "wq", "wk", "wv", "wo", "ln2_g", "ln2_b", "w1", "b1", "w2")
@@ -69,9 +79,15 @@ class _Slice:
 class TinyTransformer:
     def __init__(self, device: Device, vocab_size: int, d_model: int, d_ff: int, n_layers: int, n_heads: int,
                  compute_dtype: int = BF16, eps: float = 1e-5, deferred: bool = True, post_norm: bool = False,
-                 residual_scale: float = 1.0, act8: bool = False):
+                 residual_scale: float = 1.0, act8: bool = False, gated_ff: Optional[int] = None, rotary_base: float = 0.0,
+                 rotary_axes: int = 1):
         if d_model % n_heads:
             raise MogradError(1, "d_model must be a multiple of n_heads")
+        if gated_ff is not None and not GATE_SILU <= gated_ff <= GATE_RELU:
+            raise MogradError(1, f"no such gate: {gated_ff}")
+        pairs = d_model // n_heads // 2
+        if rotary_base and (d_model // n_heads % 2 or rotary_base < 0 or not 1 <= rotary_axes <= pairs):
+            raise MogradError(1, "rotary positions need heads of an even width, a positive base and a pair of columns for every axis")
         self.device, self.lib, self.stream = device, device.lib, device.stream
         self.V, self.d, self.ff, self.L, self.H = vocab_size, d_model, d_ff, n_layers, n_heads
         self.dh = d_model // n_heads
@@ -79,6 +95,10 @@ class TinyTransformer:
         self.eps = eps
         self.deferred = deferred
         self.post_norm, self.residual_scale, self.act8 = bool(post_norm), float(residual_scale), bool(act8)
+        self.gated_ff, self.rotary_base, self.rotary_axes = gated_ff, float(rotary_base), int(rotary_axes)
+        if self.rotary_base:
+            self.inv_freq = AnyBuffer.from_numpy(device, (self.rotary_base ** (-np.arange(pairs) / pairs)).astype(np.float32), F32)
+            self.pair_axis = (C.c_int32 * pairs)(*[i * self.rotary_axes // pairs for i in range(pairs)])
         self.slices: Dict[str, _Slice] = {}
         off = 0
 
@@ -89,8 +109,9 @@ class TinyTransformer:
 
         d, ff, V = d_model, d_ff, vocab_size
         place("embed", (V, d))
+        up = ff if gated_ff is None else 2 * ff
         block_shapes = {"ln1_g": (d,), "ln1_b": (d,), "wq": (d, d), "wk": (d, d), "wv": (d, d), "wo": (d, d),
-                        "ln2_g": (d,), "ln2_b": (d,), "w1": (ff, d), "b1": (ff,), "w2": (d, ff)}
+                        "ln2_g": (d,), "ln2_b": (d,), "w1": (up, d), "b1": (up,), "w2": (d, ff)}
         for layer in range(n_layers):
             for name in BLOCK_PARAMS:
                 if name == "wq":
@@ -180,7 +201,9 @@ class TinyTransformer:
                 "h_mid": new(n * d), "x2": new(n * d), "a": new(n * ff),
                 "mean1": new(n, F32), "rstd1": new(n, F32), "mean2": new(n, F32), "rstd2": new(n, F32),
             })
-        self.tmp = {name: new(n * d) for name in ("dh", "dctx")}
+            if self.gated_ff is not None:
+                self.saved[-1]["gu"] = new(2 * n * ff)
+        self.tmp = {name: new(n * d) for name in (("dh", "dctx") if self.gated_ff is None else ("dh", "dctx", "dx"))}
         self.tmp["dqkv"] = new(3 * n * d)  # dQ | dK | dV per token
         self.tmp["da"] = new(n * ff)
         self.tmp["logits"] = new(n * V)
@@ -188,17 +211,51 @@ class TinyTransformer:
         self.loss = new(1)
         self._plan_key = (B, T)
 
+    # ------------------------------------------------------------------ gated MLP, rotary positions
+
+    def _rotate(self, qkv, B: int, T: int, positions: Optional[AnyBuffer], inverse: int) -> None:
+        """Q and K of a (B, T, 3, H, dh) tensor turned in place; inverse: their gradients turned back."""
+        row, i64s = 3 * self.d, C.c_int64 * 3
+        st = i64s(T * row, row, self.dh)
+        self.lib.mg_rotary(qkv, qkv, None if positions is None else positions.data_ptr(), self.inv_freq.data_ptr(), self.pair_axis, B, T,
+                           2 * self.H, self.dh, self.dh, st, st, i64s(B * T, T, 1), self.rotary_axes,
+                           I32 if positions is None else positions.dtype, 0, inverse, self.cd, self.stream)
+
+    def _check_positions(self, positions: Optional[AnyBuffer], B: int, T: int) -> None:
+        if positions is None:
+            if self.rotary_base and self.rotary_axes != 1:
+                raise MogradError(1, "rotary positions of several axes are given to step()")
+            return
+        if not self.rotary_base:
+            raise MogradError(1, "positions without rotary_base")
+        if positions.dtype not in (I32, I64) or positions.numel != self.rotary_axes * B * T:
+            raise MogradError(1, "positions must be int32 or int64, (rotary_axes, B, T)")
+
+    def _gated_fwd(self, l: int, x, a, gu, n: int) -> None:
+        self.lib.mg_gated_linear_fwd(x, self._w(f"blocks.{l}.w1"), self._w(f"blocks.{l}.b1"), a, gu, n, self.ff, self.d, self.gated_ff,
+                                     self.cd, self.stream)
+
+    def _gated_bwd(self, l: int, da, gu, x, dx, n: int) -> None:
+        args = (da, gu, x, self._w(f"blocks.{l}.w1"), dx, self._g(f"blocks.{l}.w1"), self._g(f"blocks.{l}.b1"), n, self.ff, self.d, 0,
+                self.gated_ff, self.cd)
+        if self.deferred:
+            self.lib.mg_gated_linear_bwd_deferred(*args, F32, self.pending, self.stream)
+        else:
+            self.lib.mg_gated_linear_bwd(*args, self.cd, self.stream)
+
     # ------------------------------------------------------------------ one step
 
-    def step(self, ids: AnyBuffer, labels: AnyBuffer, B: int, T: int, marks=None) -> AnyBuffer:
+    def step(self, ids: AnyBuffer, labels: AnyBuffer, B: int, T: int, marks=None, positions: Optional[AnyBuffer] = None) -> AnyBuffer:
         """Runs forward, loss and backward for `ids`/`labels` ((B, T) int32 or int64 device
         buffers).  Returns the loss buffer (one element, compute dtype); the fp32 gradients
         are in `self.grads`.  Nothing is synchronised.  `marks`, if given, is called with
-        "forward" and "backward" at the boundaries (for event timing)."""
+        "forward" and "backward" at the boundaries (for event timing).  `positions`: (rotary_axes, B, T) int32 or int64
+        device buffer of the tokens' positions (None: their places, for one axis)."""
         if ids.dtype not in (I32, I64) or labels.dtype not in (I32, I64):
             raise MogradError(1, "ids and labels must be int32 or int64")
         if ids.numel != B * T or labels.numel != B * T:
             raise MogradError(1, "ids/labels do not match (B, T)")
+        self._check_positions(positions, B, T)
         self._plan(B, T)
         lib, s, cd = self.lib, self.stream, self.cd
         n, d, ff, V, H, dh = B * T, self.d, self.ff, self.V, self.H, self.dh
@@ -215,7 +272,7 @@ class TinyTransformer:
 
         lib.mg_cast(P(self.master), P(self.work), self.total, F32, cd, s)
         if self._residual_norm():
-            return self._step_residual_norm(ids, labels, B, T, linear, marks)
+            return self._step_residual_norm(ids, labels, B, T, linear, marks, positions)
 
         # ---- forward
         lib.mg_gather(self._w("embed"), P(ids), P(self.h[0]), n, V, d, d, 1, ids.dtype, cd, s)
@@ -227,13 +284,18 @@ class TinyTransformer:
             # One projection with the stacked (3d, d) weight: row t of the (n, 3d) result is
             # Q | K | V of token t, i.e. (B, T, 3, H, dh), which the attention kernels read in place.
             linear(P(c["x1"]), w("wq"), P(c["qkv"]), 3 * d, d)
+            if self.rotary_base:
+                self._rotate(P(c["qkv"]), B, T, positions, 0)
             # O is written (B, T, H, dh) = (n, d), the layout the output projection reads
             lib.mg_flash_attn_fwd_packed(P(c["qkv"]), None, P(c["ctx"]), P(c["lse"]), B, T, H, dh, scale, 1, 0, cd, s)
             lib.mg_matmul_bt_add(P(c["ctx"]), w("wo"), h_in, P(c["h_mid"]), 1, n, d, d, d, 1, d, 1, n * d, d * d, cd, s)
             lib.mg_layer_norm_fwd_stats(P(c["h_mid"]), w("ln2_g"), w("ln2_b"), P(c["x2"]), P(c["mean2"]),
                                         P(c["rstd2"]), n, d, self.eps, cd, s)
-            lib.mg_matmul_bias_relu_bt(P(c["x2"]), w("w1"), w("b1"), P(c["a"]), 1, n, ff, d, d, 1, d, 1, n * d, ff * d, cd,
-                                       s)
+            if self.gated_ff is None:
+                lib.mg_matmul_bias_relu_bt(P(c["x2"]), w("w1"), w("b1"), P(c["a"]), 1, n, ff, d, d, 1, d, 1, n * d, ff * d, cd,
+                                           s)
+            else:
+                self._gated_fwd(l, P(c["x2"]), P(c["a"]), P(c["gu"]), n)
             lib.mg_matmul_bt_add(P(c["a"]), w("w2"), P(c["h_mid"]), h_out, 1, n, d, ff, ff, 1, ff, 1, n * ff, d * ff, cd,
                                  s)
         linear(P(self.h[self.L]), self._w("lm_head"), P(self.tmp["logits"]), V, d)
@@ -267,16 +329,26 @@ class TinyTransformer:
             w = lambda name, l=l: self._w(f"blocks.{l}.{name}")
             g = lambda name, l=l: self._g(f"blocks.{l}.{name}")
             # h_out = h_mid + W2 a; the ReLU's gradient rides on the dX product
-            lin_bwd(t["dh"], P(c["a"]), w("w2"), t["da"], g("w2"), None, d, ff, relu=1)
-            # the layer's input is LayerNorm(h_mid): its backward rides on the dX tiles, dh += the result
-            # (the skip connection's share is already in dh)
-            lin_ln_bwd(t["da"], P(c["x2"]), w("w1"), g("w1"), g("b1"), ff, P(c["h_mid"]), w("ln2_g"), P(c["mean2"]),
-                       P(c["rstd2"]), g("ln2_g"), g("ln2_b"))
+            lin_bwd(t["dh"], P(c["a"]), w("w2"), t["da"], g("w2"), None, d, ff, relu=int(self.gated_ff is None))
+            if self.gated_ff is not None:
+                self._gated_bwd(l, t["da"], P(c["gu"]), P(c["x2"]), t["dx"], n)
+                norm = (t["dx"], P(c["h_mid"]), w("ln2_g"), P(c["mean2"]), P(c["rstd2"]), t["dh"], t["dh"], g("ln2_g"), g("ln2_b"), n, d, cd)
+                if self.deferred:
+                    lib.mg_layer_norm_bwd_stats_deferred(*norm, F32, self.pending, s)
+                else:
+                    lib.mg_layer_norm_bwd_stats_add(*norm, s)
+            else:
+                # the layer's input is LayerNorm(h_mid): its backward rides on the dX tiles, dh += the result
+                # (the skip connection's share is already in dh)
+                lin_ln_bwd(t["da"], P(c["x2"]), w("w1"), g("w1"), g("b1"), ff, P(c["h_mid"]), w("ln2_g"), P(c["mean2"]),
+                           P(c["rstd2"]), g("ln2_g"), g("ln2_b"))
             # h_mid = h_in + W_O ctx
             lin_bwd(t["dh"], P(c["ctx"]), w("wo"), t["dctx"], g("wo"), None, d, d)
             # dctx and ctx are (B, T, H, dh); dQ | dK | dV come back as one (n, 3d) tensor
             lib.mg_flash_attn_bwd_packed(t["dctx"], P(c["ctx"]), P(c["qkv"]), None, P(c["lse"]), t["dqkv"], B, T, H, dh,
                                          scale, 1, 0, cd, s)
+            if self.rotary_base:
+                self._rotate(t["dqkv"], B, T, positions, 1)
             # gradient of the stacked projection: dx1 (n, d) and dW (3d, d) = dwq | dwk | dwv
             lin_ln_bwd(t["dqkv"], P(c["x1"]), w("wq"), g("wq"), None, 3 * d, P(self.h[l]), w("ln1_g"), P(c["mean1"]),
                        P(c["rstd1"]), g("ln1_g"), g("ln1_b"))
@@ -305,6 +377,11 @@ class TinyTransformer:
             for name in ("mean1", "rstd1", "mean2", "rstd2"):
                 c[name] = new(n, F32)
             kept = [("x1", d), ("x2", d), ("a", ff)]
+            if self.gated_ff is not None:
+                c["gu"] = new(2 * n * ff)
+                if self.act8:
+                    c["x2"] = new(n * d)
+                    kept.remove(("x2", d))
             if self.post_norm:
                 kept += [("f1", d), ("f2", d)]
                 for name in ("post_mean1", "post_rstd1", "post_mean2", "post_rstd2"):
@@ -328,7 +405,7 @@ class TinyTransformer:
         buffers = list(self.h) + [b for c in self.saved for b in c.values()]
         return sum(b.numel * DTYPE_SIZE[b.dtype] for b in buffers)
 
-    def _step_residual_norm(self, ids, labels, B, T, linear, marks):
+    def _step_residual_norm(self, ids, labels, B, T, linear, marks, positions):
         lib, s, cd = self.lib, self.stream, self.cd
         n, d, ff, V, H, dh = B * T, self.d, self.ff, self.V, self.H, self.dh
         scale = 1.0 / math.sqrt(dh)
@@ -340,7 +417,7 @@ class TinyTransformer:
         post = lambda l, i: [at(l, f"post{i}_g"), at(l, f"post{i}_b")] if self.post_norm else [None, None]
         post_stats = lambda c, i: [P(c[f"post_mean{i}"]), P(c[f"post_rstd{i}"])] if self.post_norm else [None, None]
         gate = lambda l, i: at(l, f"gate{i}") if self.post_norm else None
-        x_of = lambda c, name: t["x"] if self.act8 else P(c[name])  # (of one layer at a time, if the rest is in 8 bits)
+        x_of = lambda c, name: P(c[name]) if name in c else t["x"]  # (of one layer at a time, if the rest is in 8 bits)
         f_of = lambda c, name: P(c[name]) if self.post_norm and not self.act8 else t["f"]
         kept8 = lambda c, name: P(c[name]) if self.act8 and name in c else None
 
@@ -354,15 +431,20 @@ class TinyTransformer:
         for l in range(self.L):
             c = self.saved[l]
             linear(x_of(c, "x1"), at(l, "wq"), P(c["qkv"]), 3 * d, d)
+            if self.rotary_base:
+                self._rotate(P(c["qkv"]), B, T, positions, 0)
             lib.mg_flash_attn_fwd_packed(P(c["qkv"]), None, P(c["ctx"]), P(c["lse"]), B, T, H, dh, scale, 1, 0, cd, s)
             linear(P(c["ctx"]), at(l, "wo"), f_of(c, "f1"), d, d)
             lib.mg_residual_norm_fwd(f_of(c, "f1"), P(self.h[l]), gate(l, 1), *post(l, 1), at(l, "ln2_g"), at(l, "ln2_b"),
                                      P(c["h_mid"]), x_of(c, "x2"), *post_stats(c, 1), P(c["mean2"]), P(c["rstd2"]),
                                      kept8(c, "f1_8"), kept8(c, "x2_8"), n, d, n, self.residual_scale, self.eps, cd, s)
             a = t["a"] if self.act8 else P(c["a"])
-            lib.mg_matmul_bias_relu_bt(x_of(c, "x2"), at(l, "w1"), at(l, "b1"), a, 1, n, ff, d, d, 1, d, 1, n * d, ff * d, cd, s)
+            if self.gated_ff is None:
+                lib.mg_matmul_bias_relu_bt(x_of(c, "x2"), at(l, "w1"), at(l, "b1"), a, 1, n, ff, d, d, 1, d, 1, n * d, ff * d, cd, s)
+            else:
+                self._gated_fwd(l, x_of(c, "x2"), a, P(c["gu"]), n)
             if self.act8:
-                lib.mg_act8_store(a, P(c["a_8"]), n, ff, 1, cd, s)
+                lib.mg_act8_store(a, P(c["a_8"]), n, ff, int(self.gated_ff is None), cd, s)
             linear(a, at(l, "w2"), f_of(c, "f2"), d, ff)
             nxt = self.saved[l + 1] if l + 1 < self.L else None  # the last block's output meets no norm before the head
             pre = [at(l + 1, "ln1_g"), at(l + 1, "ln1_b")] if nxt else [None, None]
@@ -407,12 +489,17 @@ class TinyTransformer:
                 residual_bwd(l, 2, t["dx"], P(self.h[l + 1]), l + 1, "ln1", P(up["mean1"]), P(up["rstd1"]))
             else:
                 residual_bwd(l, 2, None, None, None, None, None, None)
-            kept_bwd(t["df"], c, "a", at(l, "w2"), t["da"], g(l, "w2"), None, d, ff, relu=1)
-            kept_bwd(t["da"], c, "x2", at(l, "w1"), t["dx"], g(l, "w1"), g(l, "b1"), ff, d)
+            kept_bwd(t["df"], c, "a", at(l, "w2"), t["da"], g(l, "w2"), None, d, ff, relu=int(self.gated_ff is None))
+            if self.gated_ff is None:
+                kept_bwd(t["da"], c, "x2", at(l, "w1"), t["dx"], g(l, "w1"), g(l, "b1"), ff, d)
+            else:
+                self._gated_bwd(l, t["da"], P(c["gu"]), P(c["x2"]), t["dx"], n)
             residual_bwd(l, 1, t["dx"], P(c["h_mid"]), l, "ln2", P(c["mean2"]), P(c["rstd2"]))
             lin_bwd(t["df"], P(c["ctx"]), at(l, "wo"), t["dctx"], g(l, "wo"), None, d, d)
             lib.mg_flash_attn_bwd_packed(t["dctx"], P(c["ctx"]), P(c["qkv"]), None, P(c["lse"]), t["dqkv"], B, T, H, dh, scale, 1, 0,
                                          cd, s)
+            if self.rotary_base:
+                self._rotate(t["dqkv"], B, T, positions, 1)
             kept_bwd(t["dqkv"], c, "x1", at(l, "wq"), t["dx"], g(l, "wq"), None, 3 * d, d)
         c = self.saved[0]
         norm = (t["dx"], P(self.h[0]), at(0, "ln1_g"), P(c["mean1"]), P(c["rstd1"]), t["dh"], t["dh"], g(0, "ln1_g"), g(0, "ln1_b"))
@@ -438,8 +525,8 @@ class TinyTransformer:
         cross-entropy on class ids.  Returns (loss node, {parameter name: leaf node})."""
         from .runtime import Layout, Node
 
-        if self._residual_norm():
-            raise MogradError(2, "the rule tables have no node for post_norm, residual_scale or act8: use step()")
+        if self._residual_norm() or (self.L > 0 and (self.gated_ff is not None or self.rotary_base)):
+            raise MogradError(2, "the rule tables have no node for post_norm, residual_scale, act8, gated_ff or rotary_base: use step()")
         n, d, ff, V, H, dh, cd = B * T, self.d, self.ff, self.V, self.H, self.dh, self.cd
         leaves = {}
 
@@ -510,17 +597,27 @@ class TinyTransformer:
     # ------------------------------------------------------------------ optimizer
 
     def adam_step(self, lr: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
-                  weight_decay: float = 0.0, decoupled: bool = False) -> None:
+                  weight_decay: float = 0.0, decoupled: bool = False, max_norm: Optional[float] = None) -> None:
         """One Adam / AdamW update of every parameter from the gradients of the last
-        `step` (mograd/nn/optim/adam.mojo): a single kernel over the fp32 arenas."""
+        `step` (mograd/nn/optim/adam.mojo): a single kernel over the fp32 arenas.  `max_norm`: from gradients scaled down to
+        a global norm of at most this; self.grad_norm, one fp32 number on the device, is then what the norm was, and
+        self.grads stay as they are."""
         if not hasattr(self, "adam_m"):
             self.adam_m = AnyBuffer.create(F32, self.device, self.total, fill=0.0)
             self.adam_v = AnyBuffer.create(F32, self.device, self.total, fill=0.0)
             self.adam_t = 0
+        args = (self.master.data_ptr(), self.grads.data_ptr(), self.adam_m.data_ptr(), self.adam_v.data_ptr(), self.total, lr,
+                beta1, beta2, eps, weight_decay, self.adam_t + 1, int(decoupled))
+        if max_norm is None:
+            self.lib.mg_adam_step(*args, self.stream)
+        else:
+            if not hasattr(self, "grad_norm"):
+                self.grad_norm = AnyBuffer.create(F32, self.device, 1)
+            # (the gaps between the arena's parameters are zeros)
+            self.lib.mg_grad_norm((C.c_void_p * 1)(self.grads.data_ptr().value), (C.c_int64 * 1)(self.total), (C.c_int * 1)(F32), 1,
+                                  self.grad_norm.data_ptr(), self.stream)
+            self.lib.mg_adam_step_clipped(*args, self.grad_norm.data_ptr(), max_norm, self.stream)
         self.adam_t += 1
-        self.lib.mg_adam_step(self.master.data_ptr(), self.grads.data_ptr(), self.adam_m.data_ptr(),
-                              self.adam_v.data_ptr(), self.total, lr, beta1, beta2, eps, weight_decay, self.adam_t,
-                              int(decoupled), self.stream)
 
     def parameters(self) -> dict:
         """Downloads the fp32 master weights as a tree shaped like load_params' argument."""
@@ -542,28 +639,31 @@ class TinyTransformer:
         2mnk per product, 3 products per Linear (forward, dX, dW), and for causal
         attention half of 4*B*H*T^2*dh forward plus 2.5 times that backward."""
         n, d, ff, V = B * T, self.d, self.ff, self.V
-        per_block = 4 * d * d + 2 * d * ff
+        per_block = 4 * d * d + (2 if self.gated_ff is None else 3) * d * ff
         linear = 3 * 2 * n * (self.L * per_block + V * d)
         attn_fwd = 0.5 * 4 * B * self.H * T * T * self.dh
         return linear + self.L * 3.5 * attn_fwd
 
 
-def init_params(rng: np.random.Generator, vocab_size: int, d_model: int, d_ff: int, n_layers: int, post_norm: bool = False) -> dict:
+def init_params(rng: np.random.Generator, vocab_size: int, d_model: int, d_ff: int, n_layers: int, post_norm: bool = False,
+                gated_ff: bool = False) -> dict:
     """Random parameters with the reference's initialisers: Embedding ~ N(0, 1)
     (nn/modules/embedding.mojo:23-29), Linear weight and bias ~ U(+-sqrt(6 / fan_in))
-    (nn/modules/linear.mojo:29-47), LayerNorm gamma 1, beta 0.  post_norm: POST_NORM_PARAMS too, gates of 1."""
+    (nn/modules/linear.mojo:29-47), LayerNorm gamma 1, beta 0.  post_norm: POST_NORM_PARAMS too, gates of 1.  gated_ff: w1 and b1 of both
+    projections."""
     def lin(o, i):
         b = math.sqrt(6.0 / i)
         return rng.uniform(-b, b, size=(o, i)).astype(np.float32)
 
     d, ff = d_model, d_ff
+    up = 2 * ff if gated_ff else ff
     blocks = []
     for _ in range(n_layers):
         blocks.append({
             "ln1_g": np.ones(d, np.float32), "ln1_b": np.zeros(d, np.float32),
             "wq": lin(d, d), "wk": lin(d, d), "wv": lin(d, d), "wo": lin(d, d),
             "ln2_g": np.ones(d, np.float32), "ln2_b": np.zeros(d, np.float32),
-            "w1": lin(ff, d), "b1": rng.uniform(-math.sqrt(6.0 / d), math.sqrt(6.0 / d), ff).astype(np.float32),
+            "w1": lin(up, d), "b1": rng.uniform(-math.sqrt(6.0 / d), math.sqrt(6.0 / d), up).astype(np.float32),
             "w2": lin(d, ff),
         })
         if post_norm:

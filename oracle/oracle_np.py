@@ -632,11 +632,12 @@ def residual_norm_bwd(dx, dh_out, f, h_out, gate=None, post=None, pre=None, scal
     return out
 
 
-def residual_transformer_step(params, ids, labels, n_heads, scale=1.0, eps=1e-5, store=None, kept=None):
+def residual_transformer_step(params, ids, labels, n_heads, scale=1.0, eps=1e-5, store=None, kept=None, gated=None, turns=None):
     """tiny_transformer_step with each block's output joined to the stream by residual_norm_fwd: normalised and gated
     if the blocks have POST_NORM parameters (post1_g, post1_b, gate1 after attention; post2_g, post2_b, gate2 after the MLP),
     the stream scaled by `scale`.  `kept(layer, name, value)`, if given, is what the backward sees of the activations
-    x1, x2, a, f1, f2 (rows, cols)."""
+    x1, x2, a, f1, f2 (rows, cols).  `gated`: the MLP is a gated one, w1 and b1 of both projections, its gate passed through
+    this (one of GATES).  `turns`: (positions (axes, B, T), inv_freq, pair_axis), by which queries and keys are turned."""
     r = (lambda a: a) if store is None else (lambda a: None if a is None else np.asarray(store(a), dtype=F64))
     kept = kept or (lambda layer, name, value: value)
     ids, labels = np.asarray(ids, dtype=np.int64), np.asarray(labels, dtype=np.int64).reshape(-1)
@@ -659,12 +660,18 @@ def residual_transformer_step(params, ids, labels, n_heads, scale=1.0, eps=1e-5,
     for l, b in enumerate(blocks):
         c = {"x1": x}
         q, k, v = (r(matmul_bias_bt(x, b[w])).reshape(B, T, n_heads, dh) for w in ("wq", "wk", "wv"))
+        if turns is not None:
+            q, k = (r(rotary(t, *turns)[0]) for t in (q, k))
         o, _ = sdpa_fwd(q, k, v, causal=True)
         c["qkv"], c["ctx"] = (q, k, v), r(o).transpose(0, 2, 1, 3).reshape(n, d)
         c["f1"] = r(matmul_bias_bt(c["ctx"], b["wo"]))
         c["mid"] = join(b, 1, c["f1"], h, pair(b, "ln2"))
         c["x2"] = c["mid"]["x"]
-        c["a"] = relu(r(matmul_bias_bt(c["x2"], b["w1"], b["b1"])))
+        if gated is None:
+            c["a"] = relu(r(matmul_bias_bt(c["x2"], b["w1"], b["b1"])))
+        else:
+            a, gu = gated_linear_fwd(c["x2"], b["w1"], b["b1"], gated)
+            c["a"], c["gu"] = r(a), r(gu)
         c["f2"] = r(matmul_bias_bt(c["a"], b["w2"]))
         c["end"] = join(b, 2, c["f2"], c["mid"]["h_out"], pair(blocks[l + 1], "ln1") if l + 1 < L else None)
         h, x = c["end"]["h_out"], c["end"]["x"]
@@ -698,12 +705,16 @@ def residual_transformer_step(params, ids, labels, n_heads, scale=1.0, eps=1e-5,
         b, c, g = blocks[l], saved[l], grads["blocks"][l]
         df = split(l, 2, c["end"], c["f2"], dx, pair(blocks[l + 1], "ln1") if l + 1 < L else None, l + 1, "ln1")
         g["w2"] = r(linear_grad_w(df, c["a"]))
-        da = relu_grad(c["a"], r(linear_grad_x(df, b["w2"])))
+        da = r(linear_grad_x(df, b["w2"]))
+        da = relu_grad(c["a"], da) if gated is None else r(gated_linear_bwd(da, c["gu"], c["x2"], b["w1"], gated)[3])
         g["w1"], g["b1"] = r(linear_grad_w(da, c["x2"])), r(linear_grad_b(da))
         df = split(l, 1, c["mid"], c["f1"], r(linear_grad_x(da, b["w1"])), pair(b, "ln2"), l, "ln2")
         g["wo"] = r(linear_grad_w(df, c["ctx"]))
         do = r(linear_grad_x(df, b["wo"])).reshape(B, T, n_heads, dh).transpose(0, 2, 1, 3)
-        dq, dk, dv = (r(t).reshape(n, d) for t in sdpa_bwd(*c["qkv"], do, causal=True))
+        dq, dk, dv = (r(t) for t in sdpa_bwd(*c["qkv"], do, causal=True))
+        if turns is not None:
+            dq, dk = (r(rotary(t, *turns, inverse=True)[0]) for t in (dq, dk))
+        dq, dk, dv = (t.reshape(n, d) for t in (dq, dk, dv))
         for name, t in (("wq", dq), ("wk", dk), ("wv", dv)):
             g[name] = r(linear_grad_w(t, c["x1"]))
         dx = r(linear_grad_x(dq, b["wq"]) + linear_grad_x(dk, b["wk"]) + linear_grad_x(dv, b["wv"]))
@@ -711,11 +722,6 @@ def residual_transformer_step(params, ids, labels, n_heads, scale=1.0, eps=1e-5,
     grads["blocks"][0].update({"ln1_g": r(dg), "ln1_b": r(db)})
     grads["embed"] = r(scatter_add(ids.reshape(-1), r(state["dh"] + r(din)), V))
     return float(loss), grads
-
-
-# --------------------------------------------------------------------------- #
-# Pool size classes
-# --------------------------------------------------------------------------- #
 
 
 # --------------------------------------------------------------------------- #
@@ -788,6 +794,11 @@ def clip_grads(grads, max_norm):
     scale = max_norm / norm if norm > max_norm else 1.0
     return norm, [np.asarray(g, np.float64) * scale for g in grads]
 
+
+
+# --------------------------------------------------------------------------- #
+# Pool size classes
+# --------------------------------------------------------------------------- #
 
 
 def round_class(nbytes: int) -> int:
