@@ -448,7 +448,7 @@ int mg_sgd_step_clipped(void* w, const void* g, int64_t n, float lr, const float
 int mg_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int64_t count, float* norm, mg_stream stream);
 
 /* The norm as above (`norm` may be NULL), and out[i] = grads[i] * (norm > max_norm ? max_norm / norm : 1), in fp32, rounded once to the
- * tensor's dtype.  out[i] may be grads[i]; no other overlap.  max_norm >= 0.  So gradients of a norm that is not a number stay as they
+ * tensor's dtype.  out[i] may be grads[i]; no other overlap, and no tensor twice among out.  max_norm >= 0.  So gradients of a norm that is not a number stay as they
  * are, and those of an infinite norm become zeros, and NaN where they are infinite.  No counterpart in the reference. */
 int mg_clip_grads(const void* const* grads, void* const* out, const int64_t* numels, const int* dtypes, int64_t count, float max_norm,
                   float* norm, mg_stream stream);

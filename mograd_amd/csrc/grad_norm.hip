@@ -6,6 +6,7 @@
 // billions of them loses nothing that a norm in fp32 could show.  The tensors are cut into pieces, a workgroup each, whose sums go to
 // scratch; whoever needs the norm adds those up in one order, so every result is the same in every run, and there are no atomics.
 #include <algorithm>
+#include <vector>
 
 #include "mg_device.h"
 #include "mg_internal.h"
@@ -34,7 +35,8 @@ __device__ __forceinline__ int norm_piece(const NormTensors& t, int b, int64_t p
     if (t.end[mid] > b) hi = mid;
     else lo = mid + 1;
   }
-  from = static_cast<int64_t>(b - (lo ? t.end[lo - 1] : 0)) * piece;
+  const int begin = lo ? t.end[lo - 1] : 0;
+  from = static_cast<int64_t>(b - begin) * piece;
   to = min(from + piece, t.numel[lo]);
   return lo;
 }
@@ -49,12 +51,29 @@ __device__ __forceinline__ double norm_block_sum(double v, double* slots) {
   return (slots[0] + slots[1]) + (slots[2] + slots[3]);
 }
 
-// A thread's sum of squares of n elements at any address: sixteen bytes at a time, the last elements one by one.
+// Elements before the first 16-byte boundary at or behind p, of n at most.
+template <typename T>
+__device__ __forceinline__ int norm_head(const T* p, int64_t n) {
+  const int head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(T));
+  return head < n ? head : static_cast<int>(n);
+}
+
+// A thread's sum of squares of n elements at any address: those up to a 16-byte boundary one by one, then sixteen bytes at a time, then
+// the last ones.
 template <typename T>
 __device__ __forceinline__ double norm_piece_sum(const T* __restrict__ p, int64_t n) {
   constexpr int VEC = WideVec<T>::value, AHEAD = 4;
-  const int64_t whole = n / VEC;
   double sum[2] = {0.0, 0.0};
+  auto one = [&](int64_t i) {
+    const double d = static_cast<double>(to_float(p[i]));
+    sum[0] = fma(d, d, sum[0]);
+  };
+  const int head = norm_head(p, n);
+  if (threadIdx.x < head) one(threadIdx.x);
+  const int64_t last = head + (n - head) / VEC * VEC + threadIdx.x;
+  if (last < n) one(last);
+  p += head;
+  const int64_t whole = (n - head) / VEC;
   int64_t i = threadIdx.x;
   auto add = [&](const float (&v)[VEC]) {
 #pragma unroll
@@ -66,19 +85,14 @@ __device__ __forceinline__ double norm_piece_sum(const T* __restrict__ p, int64_
   for (; i + (AHEAD - 1) * kNormThreads < whole; i += AHEAD * kNormThreads) {
     float v[AHEAD][VEC];
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) VecAny<T, VEC>::load(p + (i + a * kNormThreads) * VEC, v[a]);
+    for (int a = 0; a < AHEAD; ++a) VecIO<T, VEC>::load(p + (i + a * kNormThreads) * VEC, v[a]);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) add(v[a]);
   }
   for (; i < whole; i += kNormThreads) {
     float v[VEC];
-    VecAny<T, VEC>::load(p + i * VEC, v);
+    VecIO<T, VEC>::load(p + i * VEC, v);
     add(v);
-  }
-  const int64_t last = whole * VEC + threadIdx.x;
-  if (last < n) {
-    const double d = static_cast<double>(to_float(p[last]));
-    sum[0] = fma(d, d, sum[0]);
   }
   return sum[0] + sum[1];
 }
@@ -89,9 +103,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_sums_kernel(NormTensors t, 
   const int which = norm_piece(t, blockIdx.x, piece, from, to);
   double sum;
   switch (t.dtype[which]) {
-    case MG_F32: sum = norm_piece_sum(static_cast<const float*>(t.in[which]) + from, to - from); break;
-    case MG_F16: sum = norm_piece_sum(static_cast<const f16_t*>(t.in[which]) + from, to - from); break;
-    default: sum = norm_piece_sum(static_cast<const bf16_t*>(t.in[which]) + from, to - from); break;
+    case MG_F32: sum = norm_piece_sum<float>(static_cast<const float*>(t.in[which]) + from, to - from); break;
+    case MG_F16: sum = norm_piece_sum<f16_t>(static_cast<const f16_t*>(t.in[which]) + from, to - from); break;
+    default: sum = norm_piece_sum<bf16_t>(static_cast<const bf16_t*>(t.in[which]) + from, to - from); break;
   }
   sum = norm_block_sum(sum, slots);
   if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -110,35 +124,47 @@ __global__ __launch_bounds__(kNormThreads) void norm_finish_kernel(const double*
   if (threadIdx.x == 0) *norm = v;
 }
 
-template <typename T>
-__device__ __forceinline__ void clip_piece(const T* __restrict__ in, T* __restrict__ out, int64_t n, float scale) {
+// SAME: in and out lie alike on their 16-byte chunks, as they do where out is in.
+template <typename T, bool SAME>
+__device__ __forceinline__ void clip_chunks(const T* in, T* out, int64_t n, float scale) {
   constexpr int VEC = WideVec<T>::value, AHEAD = 4;
-  const int64_t whole = n / VEC;
+  auto one = [&](int64_t i) { out[i] = from_float<T>(to_float(in[i]) * scale); };
+  const int head = norm_head(in, n);
+  if (threadIdx.x < head) one(threadIdx.x);
+  const int64_t last = head + (n - head) / VEC * VEC + threadIdx.x;
+  if (last < n) one(last);
+  in += head, out += head;
+  const int64_t whole = (n - head) / VEC;
+  auto store = [&](T* p, float (&v)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] *= scale;
+    if constexpr (!SAME) VecAny<T, VEC>::store(p, v);
+    else VecIO<T, VEC>::store_stream(p, v);
+  };
   int64_t i = threadIdx.x;
   for (; i + (AHEAD - 1) * kNormThreads < whole; i += AHEAD * kNormThreads) {
     float v[AHEAD][VEC];
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) VecAny<T, VEC>::load(in + (i + a * kNormThreads) * VEC, v[a]);
+    for (int a = 0; a < AHEAD; ++a) VecIO<T, VEC>::load_stream(in + (i + a * kNormThreads) * VEC, v[a]);
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[a][e] *= scale;
-      VecAny<T, VEC>::store(out + (i + a * kNormThreads) * VEC, v[a]);
-    }
+    for (int a = 0; a < AHEAD; ++a) store(out + (i + a * kNormThreads) * VEC, v[a]);
   }
   for (; i < whole; i += kNormThreads) {
     float v[VEC];
-    VecAny<T, VEC>::load(in + i * VEC, v);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] *= scale;
-    VecAny<T, VEC>::store(out + i * VEC, v);
+    VecIO<T, VEC>::load_stream(in + i * VEC, v);
+    store(out + i * VEC, v);
   }
-  const int64_t last = whole * VEC + threadIdx.x;
-  if (last < n) out[last] = from_float<T>(to_float(in[last]) * scale);
+}
+template <typename T>
+__device__ __forceinline__ void clip_piece(const T* in, T* out, int64_t n, float scale) {
+  if (reinterpret_cast<uintptr_t>(in) % 16 == reinterpret_cast<uintptr_t>(out) % 16) clip_chunks<T, true>(in, out, n, scale);
+  else clip_chunks<T, false>(in, out, n, scale);
 }
 
 // Every workgroup adds up the sums for itself (16 KB from the second-level cache), then scales its piece.  A scale of 1 in place is
-// nothing to do.
+// nothing to do.  This second reading and the results go past the caches, the first one through them, so that it leaves there what this
+// one finds: bf16, 100 tensors, 3e8 elements 315 us, 5.7 TB/s of reading twice and writing (through the caches 372, both readings past them
+// 337); 290 tensors without gaps, whose chunks start where they like, 382; 68 fp32 tensors of 1.1e7 24.7.
 __global__ __launch_bounds__(kNormThreads) void clip_kernel(NormTensors t, int64_t piece, const double* __restrict__ sums, int64_t count,
                                                             float max_norm, float* __restrict__ norm_out) {
   __shared__ double slots[kNormThreads / kWave];
@@ -149,9 +175,9 @@ __global__ __launch_bounds__(kNormThreads) void clip_kernel(NormTensors t, int64
   const int which = norm_piece(t, blockIdx.x, piece, from, to);
   if (scale == 1.f && t.in[which] == t.out[which]) return;
   switch (t.dtype[which]) {
-    case MG_F32: return clip_piece(static_cast<const float*>(t.in[which]) + from, static_cast<float*>(t.out[which]) + from, to - from, scale);
-    case MG_F16: return clip_piece(static_cast<const f16_t*>(t.in[which]) + from, static_cast<f16_t*>(t.out[which]) + from, to - from, scale);
-    default: return clip_piece(static_cast<const bf16_t*>(t.in[which]) + from, static_cast<bf16_t*>(t.out[which]) + from, to - from, scale);
+    case MG_F32: return clip_piece<float>(static_cast<const float*>(t.in[which]) + from, static_cast<float*>(t.out[which]) + from, to - from, scale);
+    case MG_F16: return clip_piece<f16_t>(static_cast<const f16_t*>(t.in[which]) + from, static_cast<f16_t*>(t.out[which]) + from, to - from, scale);
+    default: return clip_piece<bf16_t>(static_cast<const bf16_t*>(t.in[which]) + from, static_cast<bf16_t*>(t.out[which]) + from, to - from, scale);
   }
 }
 
@@ -203,6 +229,13 @@ static int grad_norm(const char* who, const void* const* grads, void* const* out
   for (int64_t i = 0; i < count; ++i) pieces += ceil_div(numels[i], piece);
   hipStream_t s = to_stream(stream);
   return without_exceptions(who, [&]() -> int {
+    if (clip) {  // (a tensor that is there twice would be scaled by two workgroups at once)
+      std::vector<const void*> outs;
+      for (int64_t i = 0; i < count; ++i)
+        if (numels[i] > 0) outs.push_back(out[i]);
+      std::sort(outs.begin(), outs.end());
+      if (std::adjacent_find(outs.begin(), outs.end()) != outs.end()) return fail(MG_ERR_INVALID, "%s: two of the results are one tensor", who);
+    }
     CaptureHold hold;
     MG_TRY(hold.begin(s));
     Scratch mem;

@@ -83,7 +83,7 @@ PyObject* g_fallbacks = nullptr;      // name -> ctypes wrapper
   X(mg_scatter_add_deferred) X(mg_flash_attn_fwd) X(mg_flash_attn_bwd) X(mg_flash_attn_fwd_bshd)                          \
   X(mg_flash_attn_bwd_bshd) X(mg_flash_attn_fwd_packed) X(mg_flash_attn_bwd_packed) X(mg_act8_store) X(mg_act8_load)       \
   X(mg_linear_bwd_act8) X(mg_residual_norm_fwd) X(mg_residual_norm_bwd) X(mg_gated_linear_fwd) X(mg_gated_linear_bwd)      \
-  X(mg_gated_linear_bwd_deferred) X(mg_adam_step_clipped) X(mg_sgd_step_clipped)
+  X(mg_gated_linear_bwd_deferred) X(mg_adam_step_clipped) X(mg_sgd_step_clipped) X(mg_rotary) X(mg_grad_norm) X(mg_clip_grads)
 
 struct Lib {
 #define X(f) decltype(&::f) f = nullptr;
@@ -129,12 +129,37 @@ bool pointer_of(PyObject* o, void** out) {
   return true;
 }
 
+// An array in host memory that the library reads during the call: a ctypes array (or any contiguous buffer) of elements like T.
+template <class T>
+bool host_array_of(PyObject* o, T** out) {
+  if (o == Py_None) {
+    *out = nullptr;
+    return true;
+  }
+  if (!PyObject_CheckBuffer(o)) return false;
+  Py_buffer view;
+  if (PyObject_GetBuffer(o, &view, PyBUF_ND | PyBUF_FORMAT) != 0) return PyErr_Clear(), false;
+  const char* f = view.format ? view.format : "B";
+  while (*f == '<' || *f == '=' || *f == '@') ++f;
+  const bool kind = std::is_pointer_v<T> ? *f == 'P' : *f == 'i' || *f == 'l' || *f == 'q';
+  const bool fits = kind && f[1] == 0 && view.itemsize == static_cast<Py_ssize_t>(sizeof(T)) && view.ndim == 1;
+  if (fits) *out = static_cast<T*>(view.buf);
+  PyBuffer_Release(&view);  // (the caller's arguments keep the array)
+  return fits;
+}
+
 template <class T>
 bool convert(PyObject* o, T* out) {
+  using Element = std::remove_const_t<std::remove_pointer_t<T>>;
   if constexpr (std::is_floating_point_v<T>) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) return PyErr_Clear(), false;
     *out = static_cast<T>(v);
+    return true;
+  } else if constexpr (std::is_pointer_v<T> && (std::is_integral_v<Element> || std::is_pointer_v<Element>)) {
+    Element* p = nullptr;
+    if (!host_array_of(o, &p)) return false;
+    *out = p;
     return true;
   } else if constexpr (std::is_pointer_v<T>) {
     void* p = nullptr;

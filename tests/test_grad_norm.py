@@ -27,14 +27,14 @@ def test_refusals():
     lib = mograd_amd.load()
     p = 4096
 
-    def call(pointers=(p, p), out=(p, p), numels=(5, 6), dtypes=(F32, BF16), count=2, max_norm=1.0, norm=p, clip=True):
+    def call(pointers=(p, p), out=(p, 2 * p), numels=(5, 6), dtypes=(F32, BF16), count=2, max_norm=1.0, norm=p, clip=True):
         g, n, t = _arrays(pointers, numels, dtypes)
         if clip:
             return lib.mg_clip_grads(g, (C.c_void_p * 2)(*out) if out else None, n, t, count, max_norm, norm, None)
         return lib.mg_grad_norm(g, n, t, count, norm, None)
 
     both = [dict(count=-1), dict(numels=(5, -1)), dict(numels=(5, 1 << 50)), dict(dtypes=(F32, I32)), dict(dtypes=(9, F32)), dict(pointers=(p, None))]
-    for bad in both + [dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(out=None), dict(out=(None, p))]:
+    for bad in both + [dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(out=None), dict(out=(None, p)), dict(out=(p, p))]:
         with pytest.raises(MogradError) as e:
             call(**bad)
         assert e.value.status == 1 and "clip_grads" in str(e.value), bad
