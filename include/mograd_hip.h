@@ -645,7 +645,9 @@ typedef enum mg_gate {
 /* y (M,F) = act(x Wg^T + bg) * (x Wu^T + bu) for x (M,K), all contiguous.  w (2F,K) holds Wg's rows, then Wu's; bias (2F) bg, then bu
  * (NULL for none).  gu (M,2F): where the two projections g | u of each row are left for the backward (NULL: nowhere).  `gate`: an
  * mg_gate.  Products and act in fp32, y from the projections before they are rounded.  Any M, F and K from 1, any address of an
- * element; 16-bit tensors: K at most 2^22 - 64.  Nothing overlaps. */
+ * element; 16-bit tensors: K at most 2^22 - 64.  Nothing overlaps.
+ * fp32 products may be taken from three bf16 numbers a value, 24 bits of it: a row or weight that holds an infinity or a number past
+ * 3.39e38 then gives NaN, and values below 2^-110 lose digits.  So here and in the gradients. */
 int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y, void* gu, int64_t M, int64_t F, int64_t K, int gate,
                         int dtype, mg_stream stream);
 

@@ -5,6 +5,7 @@
 
 #include "gated_direct.h"
 #include "gemm_16bit_small.h"
+#include "gemm_f32_split.h"
 #include "gemm_pad.h"
 #include "mg_deferred.h"
 #include "mg_rows.h"
@@ -32,6 +33,54 @@ __global__ __launch_bounds__(kGatedThreads) void gate_fwd_kernel(const T* __rest
   VecIO<T, VEC>::store(y + row * F + c, g);
 }
 
+// fp32: both projections from three bf16 numbers a value (gemm_f32_split.h) and y in one launch.  A tile has 64 columns of y: columns 32 j of
+// a wave's are the gate's for j = 0 and the other projection's for j = 1.
+template <int AI>
+__global__ __launch_bounds__(kSplitThreads) void gated_split_kernel(SplitProblem p, const float* __restrict__ bias, float* __restrict__ gu, int gate) {
+  __shared__ __attribute__((aligned(1024))) char lds[kSplitLds<AI>];
+  int tm, tn;
+  gemm_tile_of_block(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+  const int F = p.N, m0 = tm * AI * kSplitT, f0 = tn * (kSplitT / 2);
+  floatx16 acc[AI][2];
+  auto row = [&](int r) { return min(f0 + r / 64 * 32 + r % 32, F - 1) + (r % 64 < 32 ? 0 : static_cast<int64_t>(F)); };
+  split_product<AI, true, true>(lds, p, m0, 0, 0, p.K, row, acc);
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, col = f0 + wave % 2 * 32 + lane % 32;
+  if (col >= F) return;
+  const float bg = bias ? bias[col] : 0.f, bu = bias ? bias[F + col] : 0.f;
+  gated_with(gate, [&](auto kind) {
+#pragma unroll
+    for (int n = 0; n < 16 * AI; ++n) {
+      const int i = n / 16, r = n % 16, m = m0 + wave / 2 * 32 * AI + 32 * i + (r / 4) * 8 + (lane / 32) * 4 + r % 4;
+      if (m >= p.M) continue;
+      const float g = acc[i][0][r] + bg, u = acc[i][1][r] + bu;
+      p.c[static_cast<int64_t>(m) * F + col] = gated_act<false, decltype(kind)::value>(g) * u;
+      if (gu) {
+        float* const at = gu + static_cast<int64_t>(m) * 2 * F + col;
+        __builtin_nontemporal_store(g, at);
+        __builtin_nontemporal_store(u, at + F);
+      }
+    }
+  });
+}
+
+static int launch_gated_split(const void* x, const void* w, const void* bias, void* y, void* gu, int64_t M, int64_t F, int64_t K, int gate,
+                              int ai, hipStream_t stream) {
+  const int64_t tiles_m = ceil_div(M, ai * kSplitT), tiles_n = ceil_div(F, kSplitT / 2);
+  if (tiles_m * tiles_n > 0xffffffffLL / kSplitThreads) return fail(MG_ERR_INVALID, "gated_linear_fwd: too many output tiles");
+  SplitProblem p{};
+  p.a = static_cast<const float*>(x), p.b = static_cast<const float*>(w), p.c = static_cast<float*>(y);
+  p.M = static_cast<int>(M), p.N = static_cast<int>(F), p.K = static_cast<int>(K), p.lda = p.ldb = K;
+  p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(kSplitThreads), 0, stream, p,
+                       static_cast<const float*>(bias), static_cast<float*>(gu), gate);
+  };
+  if (ai == 2) launch(gated_split_kernel<2>);
+  else launch(gated_split_kernel<1>);
+  MG_LAUNCH_CHECK();
+  return MG_OK;
+}
+
 // [dg du] from dy, g and u, rounded to the tensors' type as the products take it.  Bound by its bytes, five values an output.
 template <typename T, int VEC, int GATE>
 __global__ __launch_bounds__(kGatedThreads) void gate_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ gu, T* __restrict__ dgu,
@@ -53,6 +102,47 @@ __global__ __launch_bounds__(kGatedThreads) void gate_bwd_kernel(const T* __rest
   }
   VecIO<T, VEC>::store(dgu + row * 2 * F + c, g);
   VecIO<T, VEC>::store(dgu + row * 2 * F + F + c, u);
+}
+
+// The same in fp32, and the column sums of [dg du] over each group of kGateRows rows, (groups, 2 F): a workgroup takes 64 chunks of columns
+// of a group, four rows at a time, and adds up what its threads have of a column in LDS.
+constexpr int kGateRows = 32;
+template <int VEC, int GATE>
+__global__ __launch_bounds__(kGatedThreads) void gate_bwd_sums_kernel(const float* __restrict__ dy, const float* __restrict__ gu,
+                                                                     float* __restrict__ dgu, float* __restrict__ sums, int M, int F, int blocks_f) {
+  __shared__ float parts[4][2][64 * VEC];
+  const int bf = blockIdx.x % blocks_f, group = blockIdx.x / blocks_f, tx = threadIdx.x % 64, ty = threadIdx.x / 64;
+  const int c = (bf * 64 + tx) * VEC, r0 = group * kGateRows;
+  float sg[VEC], su[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sg[i] = su[i] = 0.f;
+  if (c < F) {
+    for (int r = r0 + ty; r < min(r0 + kGateRows, M); r += 4) {
+      const int64_t row = r;
+      float d[VEC], g[VEC], u[VEC];
+      VecIO<float, VEC>::load(dy + row * F + c, d);
+      VecIO<float, VEC>::load(gu + row * 2 * F + c, g);
+      VecIO<float, VEC>::load(gu + row * 2 * F + F + c, u);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        float act, slope;
+        gated_act_slope<false, GATE>(g[i], act, slope);
+        g[i] = d[i] * u[i] * slope;
+        u[i] = d[i] * act;
+        sg[i] += g[i], su[i] += u[i];
+      }
+      VecIO<float, VEC>::store(dgu + row * 2 * F + c, g);
+      VecIO<float, VEC>::store(dgu + row * 2 * F + F + c, u);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) parts[ty][0][tx * VEC + i] = sg[i], parts[ty][1][tx * VEC + i] = su[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * 64 * VEC; i += kGatedThreads) {
+    const int half = i / (64 * VEC), at = i % (64 * VEC), col = bf * 64 * VEC + at;
+    if (col >= F) continue;
+    sums[static_cast<int64_t>(group) * 2 * F + half * F + col] = (parts[0][half][at] + parts[1][half][at]) + (parts[2][half][at] + parts[3][half][at]);
+  }
 }
 
 // Calls launch(VEC, gate, items, items of a row, first workgroup, workgroups) for M rows of F columns, in as many launches as it takes.
@@ -89,15 +179,14 @@ static int gate_bwd(const void* dy, const void* gu, void* dgu, int64_t M, int64_
 }
 
 // Which kernel a forward pass takes: the least of these estimates, in us.  kGatedDirect: gated_direct.h; kGatedSmall: 64 x 64 tiles, K in
-// ranges; kGatedDeep: 128 x 128 or 256 x 256 tiles, which copy ragged operands first (a launch, and two passes over them); kGatedApart
-// (fp32): a plain product, then the gate.  Fitted to 800 shapes of 1 to 20000 rows, 32 to 8192 inputs and 32 to 12000 outputs, weights from
-// memory, each by every way: over them the way taken is 1.4 % slower than each one's best for 16 bits on 16-byte chunks, 2.6 % off them, and
-// 4.6 % in fp32 (for 16 bits, 64 x 64 tiles up to 64 rows and 128 x 128 above: 31 %).  Whether the projections are kept, which is one value
+// ranges; kGatedDeep: 128 x 128 or 256 x 256 tiles, which copy ragged operands first (a launch, and two passes over them).  Fitted to 800 shapes of 1 to 20000 rows, 32 to 8192 inputs and 32 to 12000 outputs, weights from
+// memory, each by every way: over them the way taken is 1.4 % slower than each one's best on 16-byte chunks, 2.6 % off them (64 x 64 tiles
+// up to 64 rows and 128 x 128 above: 31 %).  Whether the projections are kept, which is one value
 // stored or three, is not looked at, so that y is the same either way.  `values`: two an output.
-enum GatedWay { kGatedDirect, kGatedSmall, kGatedDeep, kGatedApart };
+enum GatedWay { kGatedDirect, kGatedSmall, kGatedDeep, kGatedApart, kGatedSplit };
 struct GatedChoice {
   GatedWay way;
-  int tile;  // kGatedDirect: 16 or 32 rows; kGatedDeep: a Gemm16Tile
+  int tile;  // kGatedDirect: 16 or 32 rows; kGatedDeep: a Gemm16Tile; kGatedSplit: 1 or 2 times 128 rows
   int splits;
   double us;
 };
@@ -146,15 +235,60 @@ static GatedChoice choose_gated_16bit(int64_t M, int64_t F, int64_t K, bool ragg
   }
   return best;
 }
-// The plain product's time by its FLOP, the values it leaves and the weights that it reads, within a sixth for most.
+// fp32: a plain product and the gate, within an eighth for most; from three bf16 numbers a value (gemm_f32_split.h) in tiles of 128 or 256
+// rows, within 5 %; straight from memory.  Over 516 shapes of 16 to 20000 rows the way taken is 2.1 % slower than each one's best; without
+// the products of bf16 numbers 15 %.  us, plain product | those: (2048, 4096 <- 4096) 1052 | 718, (16384, 1024 <- 384) 250 | 170,
+// (8192, 256 <- 256) 32 | 18, (256, 1024 <- 4096) 47 | 152, (300, 300 <- 300) 7 | 19.
 static GatedChoice choose_gated_f32(int64_t M, int64_t F, int64_t K) {
-  const double cus = device_info().cu_count, values = 2.0 * M * F;
-  const double direct = gated_direct_us(M, F, K, values, true, false, cus);
-  const double apart = 6.0 + 11.4 * 4e-9 * M * F * K + 0.45 * values * 4 / 1e6 + 0.29 * 8.0 * F * K / 1e6 + 0.88 * K / 1e3;
-  const int only = env_int("MOGRAD_HIP_GATED_TILE", 0);
-  const bool few = ceil_div(F, 16) * ceil_div(M, 32) <= 1 << 22;
-  if (only == 16 || (only == 0 && direct < apart && few)) return GatedChoice{kGatedDirect, M <= 16 ? 16 : 32, 1, direct};
-  return GatedChoice{kGatedApart, 0, 1, apart};
+  const double cus = device_info().cu_count, values = static_cast<double>(M) * F, weights_mb = 8.0 * F * K / 1e6;
+  const int rows = M <= 16 ? 16 : 32;
+  GatedChoice best{kGatedApart, 0, 1, 6.9 + 10.4 * 4e-9 * values * K + 0.448 * values * 8 / 1e6 + 0.21 * weights_mb + 1.6 * K / 1e3};
+  auto offer = [&](GatedWay way, int tile, double us) {
+    if (us < best.us) best = GatedChoice{way, tile, 1, us};
+  };
+  if (ceil_div(F, 16) * ceil_div(M, rows) <= 1 << 22) offer(kGatedDirect, rows, gated_direct_us(M, F, K, 2 * values, true, false, cus));
+  const double steps = static_cast<double>(ceil_div(K, kSplitBK));
+  for (int ai = 1; ai <= 2; ++ai) {
+    const int64_t tiles = ceil_div(M, ai * kSplitT) * ceil_div(F, kSplitT / 2);
+    if (tiles > 1 << 22 || std::max(M, K) > kSplitMost) continue;
+    offer(kGatedSplit, ai, 4.34 + std::ceil(tiles / cus) * (ai == 1 ? 1.117 * steps + 2.8 : 1.845 * steps + 6.9) + 0.169 * values * 12 / 1e6);
+  }
+  // MOGRAD_HIP_GATED_TILE = 16 (straight from memory) | 64 (apart) | 128 | 256 overrides the choice.
+  switch (env_int("MOGRAD_HIP_GATED_TILE", 0)) {
+    case 16: return GatedChoice{kGatedDirect, rows, 1, 0.0};
+    case 64: return GatedChoice{kGatedApart, 0, 1, 0.0};
+    case 128: return GatedChoice{kGatedSplit, 1, 1, 0.0};
+    case 256: return GatedChoice{kGatedSplit, 2, 1, 0.0};
+    default: return best;
+  }
+}
+
+// Which kernels fp32 gradients take: those of any Linear backward (kGatedApart), or the products of bf16 numbers, dW in ranges of rows.  Fitted
+// to the same shapes, within an eighth and 7 %; the way taken is 2.6 % slower than each one's best, the first alone 8 %.  us, any Linear
+// backward's | those: (2048, 512 <- 784) 99 | 68, (2048, 4096 <- 4096) 2052 | 1486, (16384, 1024 <- 384) 586 | 364, (512, 2048 <- 512)
+// 60 | 162.
+static GatedChoice choose_gated_bwd_f32(int64_t M, int64_t F, int64_t K, bool dx, bool db) {
+  const double cus = device_info().cu_count, N = 2.0 * F, values = static_cast<double>(M) * F;
+  GatedChoice best{kGatedApart, 0, 1, 7.4 + 8.87 * (dx ? 4e-9 : 2e-9) * M * K * N + 0.326 * values * 20 / 1e6 + 0.894 * N * K * 4 / 1e6 + 1.15 * M * K * 4 / 1e6 +
+                                          (db ? 0.08 : 0.0) + 1.11 * M / 1e3 + 5.4 * N / 1e3};
+  const double steps_x = static_cast<double>(ceil_div(2 * F, kSplitBK));
+  for (int ai = 1; ai <= 2 && std::max({M, 2 * F, K}) <= kSplitMost; ++ai) {
+    const int64_t tiles_k = ceil_div(K, kSplitT), tiles_w = ceil_div(2 * F, ai * kSplitT) * tiles_k, tiles_x = dx ? ceil_div(M, ai * kSplitT) * tiles_k : 0;
+    if (tiles_w > 1 << 21 || tiles_x > 1 << 21) continue;
+    const double step = ai == 1 ? 1.58 : 2.37, ends = ai == 1 ? 2.3 : 5.1;
+    for (int s = 1; s <= 24 && (s == 1 || (M >= 64 * s && tiles_w * s <= 600)); ++s) {
+      const double steps_w = static_cast<double>(ceil_div(ceil_div(M, s), kSplitBK));
+      const double load = (tiles_w * s * (steps_w * step + ends) + tiles_x * (steps_x * step + ends)) / cus, chain = std::max(steps_w, dx ? steps_x : 0.0) * step + ends;
+      const double us = 4.5 + std::max(load, chain) + 0.36 * std::min(load, chain) + 0.196 * values * 20 / 1e6 + (s > 1 ? 2.2 + 0.243 * s * N * K * 4 / 1e6 : 0.0) + (db ? 4.1 : 0.0);
+      if (us < best.us) best = GatedChoice{kGatedSplit, ai, s, us};
+    }
+  }
+  // MOGRAD_HIP_GATED_BWD_TILE = 64 (apart) | 128 | 256 and MOGRAD_HIP_GATED_SPLITS override the choice.
+  if (env_str("MOGRAD_HIP_GATED_BWD_TILE")) {
+    const int only = env_int("MOGRAD_HIP_GATED_BWD_TILE", 0);
+    return only == 64 ? GatedChoice{kGatedApart, 0, 1, 0.0} : GatedChoice{kGatedSplit, only == 256 ? 2 : 1, std::max(1, env_int("MOGRAD_HIP_GATED_SPLITS", 1)), 0.0};
+  }
+  return best;
 }
 
 template <typename T>
@@ -232,6 +366,74 @@ static int gated_check(const char* who, int64_t M, int64_t F, int64_t K, int gat
   return MG_OK;
 }
 
+// fp32: the gate's gradient with its column sums, then dW and dX as products of three bf16 numbers a value in one launch, then the sums over
+// dW's ranges of rows and over the groups of db in one launch, or left on `list`.
+static int gated_bwd_split(const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t F, int64_t K,
+                           bool dx_accumulate, int gate, int ai, int splits, DeferredList* list, hipStream_t stream) {
+  const int64_t N = 2 * F, groups = ceil_div(M, kGateRows), numel = N * K;
+  Scratch dgu, db_part, partial;
+  MG_TRY(dgu.take(M * N * static_cast<int64_t>(sizeof(float))));
+  if (db) {
+    MG_TRY(db_part.take(groups * N * static_cast<int64_t>(sizeof(float))));
+    const bool wide = F % 4 == 0 && aligned16(dy) && aligned16(gu);
+    const int64_t blocks_f = ceil_div(F, wide ? 256 : 64);
+    if (blocks_f * groups > 0xffffffffLL / kGatedThreads) return fail(MG_ERR_INVALID, "gated_linear_bwd: too many rows");
+    const dim3 grid(static_cast<unsigned>(blocks_f * groups));
+    gated_with(gate, [&](auto kind) {
+      constexpr int GATE = decltype(kind)::value;
+      auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kGatedThreads), 0, stream, static_cast<const float*>(dy), static_cast<const float*>(gu), dgu.as<float>(),
+                           db_part.as<float>(), static_cast<int>(M), static_cast<int>(F), static_cast<int>(blocks_f));
+      };
+      if (wide) launch(gate_bwd_sums_kernel<4, GATE>);
+      else launch(gate_bwd_sums_kernel<1, GATE>);
+    });
+    MG_LAUNCH_CHECK();
+  } else {
+    MG_TRY(gate_bwd<float>(dy, gu, dgu.as<char>(), M, F, gate, stream));
+  }
+  const int k_per_split = static_cast<int>(ceil_div(ceil_div(M, splits), kSplitBK) * kSplitBK);
+  splits = static_cast<int>(ceil_div(M, k_per_split));
+  if (splits > 1) MG_TRY(partial.take(splits * numel * static_cast<int64_t>(sizeof(float))));
+  SplitProblem pw{}, px{};
+  pw.a = px.a = dgu.as<float>(), pw.b = static_cast<const float*>(x), px.b = static_cast<const float*>(w);
+  pw.c = splits > 1 ? partial.as<float>() : static_cast<float*>(dw), px.c = static_cast<float*>(dx);
+  pw.M = px.K = static_cast<int>(N), pw.N = px.N = static_cast<int>(K), pw.K = px.M = static_cast<int>(M);
+  pw.lda = px.lda = N, pw.ldb = px.ldb = pw.ldc = px.ldc = K;
+  pw.tiles_m = static_cast<int>(ceil_div(N, ai * kSplitT)), px.tiles_m = static_cast<int>(ceil_div(M, ai * kSplitT));
+  pw.tiles_n = px.tiles_n = static_cast<int>(ceil_div(K, kSplitT));
+  pw.k_per_split = k_per_split, pw.splits = splits, px.splits = 1, px.accumulate = dx_accumulate;
+  const int64_t tiles = static_cast<int64_t>(pw.tiles_m) * pw.tiles_n, n_dw = splits > 1 ? gemm_split_grid(tiles, splits, 1) : tiles;
+  const int64_t n_dx = dx ? static_cast<int64_t>(px.tiles_m) * px.tiles_n : 0;
+  if (n_dw + n_dx > 0xffffffffLL / kSplitThreads) return fail(MG_ERR_INVALID, "gated_linear_bwd: too many output tiles");
+  const dim3 grid(static_cast<unsigned>(n_dw + n_dx));
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kSplitThreads), 0, stream, pw, px, static_cast<int>(n_dw)); };
+  if (ai == 2 && splits > 1) launch(split_linear_bwd_kernel<2, true>);
+  else if (ai == 2) launch(split_linear_bwd_kernel<2, false>);
+  else if (splits > 1) launch(split_linear_bwd_kernel<1, true>);
+  else launch(split_linear_bwd_kernel<1, false>);
+  MG_LAUNCH_CHECK();
+  const int64_t dw_blocks = splits > 1 ? ceil_div(numel, 1024) : 0, db_blocks = db ? ceil_div(N, 64) : 0;
+  if (list) {
+    list->out_dtype = MG_F32;
+    if (splits > 1) {
+      list->push(kDeferSplitRows, partial.as<float>(), dw, numel, static_cast<int>(N), static_cast<int>(K), splits, ceil_div(ceil_div(numel, 4), 1024));
+      list->hold(partial);
+    }
+    if (db) {
+      list->push(kDeferBiasRows, db_part.as<float>(), db, 0, 0, static_cast<int>(N), static_cast<int>(groups), ceil_div(db_blocks, 4));
+      list->hold(db_part);
+    }
+    return MG_OK;
+  }
+  if (dw_blocks + db_blocks == 0) return MG_OK;
+  hipLaunchKernelGGL((linear_bwd_finish_kernel<float, false>), dim3(static_cast<unsigned>(dw_blocks + db_blocks)), dim3(256), 0, stream, partial.as<float>(),
+                     static_cast<float*>(dw), static_cast<int>(N), numel, splits, static_cast<int>(K), static_cast<int>(dw_blocks), db_part.as<float>(),
+                     static_cast<float*>(db), db ? static_cast<int>(groups) : 0, static_cast<int>(N));
+  MG_LAUNCH_CHECK();
+  return MG_OK;
+}
+
 // The three gradients; `list`: that of a `_deferred` call, or null.
 static int gated_bwd(const char* who, const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
                      int64_t F, int64_t K, int dx_accumulate, int gate, int dtype, int grad_dtype, DeferredList* list, mg_stream stream) {
@@ -248,6 +450,11 @@ static int gated_bwd(const char* who, const void* dy, const void* gu, const void
   return without_exceptions(who, [&]() -> int {
     CaptureHold hold;
     if (!list) MG_TRY(hold.begin(s));  // (a list's blocks outlive the call, and go back to the pool with it)
+    if (dtype == MG_F32) {
+      const GatedChoice choice = choose_gated_bwd_f32(M, F, K, dx != nullptr, db != nullptr);
+      if (choice.way == kGatedSplit)
+        return gated_bwd_split(dy, gu, x, w, dx, dw, db, M, F, K, dx_accumulate != 0, gate, choice.tile, choice.splits, list, s);
+    }
     Scratch dgu;
     MG_TRY(dgu.take(M * 2 * F * dtype_size(dtype)));
     switch (dtype) {
@@ -289,6 +496,7 @@ int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y,
     if (dtype == MG_BF16) return mg::gated_fwd_16bit<mg::bf16_t>(x, w, bias, y, gu, M, F, K, gate, s);
     if (dtype == MG_F16) return mg::gated_fwd_16bit<mg::f16_t>(x, w, bias, y, gu, M, F, K, gate, s);
     const mg::GatedChoice choice = mg::choose_gated_f32(M, F, K);
+    if (choice.way == mg::kGatedSplit) return mg::launch_gated_split(x, w, bias, y, gu, M, F, K, gate, choice.tile, s);
     if (choice.way == mg::kGatedDirect) return mg::launch_gated_direct<float>(x, w, bias, y, gu, M, F, K, gate, choice.tile, s);
     // the projections as one product, whose values are not rounded on the way; 3 M F values of 2 (K + 1) M F products' time.
     mg::Scratch kept;

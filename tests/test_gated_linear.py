@@ -219,8 +219,43 @@ def test_backward(device, M, F, K, dtype, grads):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,F,K", [(1, 1, 1), (5, 3, 7), (70, 100, 130), (129, 65, 33), (260, 140, 264), (1030, 70, 129), (300, 301, 77)])
+def test_backward_every_way(device, monkeypatch, M, F, K):
+    """fp32: any Linear backward's kernels, and products of bf16 numbers in either tile and with ranges of rows."""
+    p = _inputs(431, M, F, K, F32)
+    pending = C.c_void_p()
+    device.lib.mg_deferred_create(C.byref(pending))
+    for tile, splits in (("64", "1"), ("128", "1"), ("128", "3"), ("256", "1"), ("256", "5")):
+        monkeypatch.setenv("MOGRAD_HIP_GATED_BWD_TILE", tile)
+        monkeypatch.setenv("MOGRAD_HIP_GATED_SPLITS", splits)
+        for gate in ("silu", "gelu_tanh"):
+            for offset in (0, 1):
+                _check_backward(p, _backward(device, p, F32, F32, gate, offset=offset), F32, F32, gate)
+        old = round_to_dtype(normal(432, 0, (M, K)), F32)
+        _check_backward(p, _backward(device, p, F32, F32, gate, accumulate=old), F32, F32, gate, old)
+        got = _backward(device, p, F32, F32, gate, dx=False, db=False)
+        _check_backward(p, got, F32, F32, gate)
+        later = _backward(device, p, F32, F32, gate, pending=pending)
+        assert np.array_equal(later["dw"], _backward(device, p, F32, F32, gate)["dw"])
+        _check_backward(p, later, F32, F32, gate)
+    device.lib.mg_deferred_destroy(pending)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-25, 1e15])
+def test_fp32_far_from_one(device, monkeypatch, size):
+    """Products of bf16 numbers keep fp32's digits and range."""
+    p = _inputs(433, 150, 70, 100, F32, bias=False)
+    p["x"] = (p["x"] * np.float32(size)).astype(np.float32)
+    p["w"] = (p["w"] / np.float32(size)).astype(np.float32)
+    for tile in ("128", "256"):
+        monkeypatch.setenv("MOGRAD_HIP_GATED_TILE", tile)
+        _check_forward(p, _forward(device, p, F32, "silu"), F32, "silu")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("M,F,K", [(5, 24, 40), (700, 200, 384), (2000, 100, 77)])
+@pytest.mark.parametrize("M,F,K", [(5, 24, 40), (700, 200, 384), (2000, 100, 77), (3000, 500, 300)])
 def test_deferred_sums_are_the_immediate_ones(device, M, F, K, dtype):
     p = _inputs(421, M, F, K, dtype)
     pending = C.c_void_p()
