@@ -449,7 +449,7 @@ int mg_grad_norm(const void* const* grads, const int64_t* numels, const int* dty
 
 /* The norm as above (`norm` may be NULL), and out[i] = grads[i] * (norm > max_norm ? max_norm / norm : 1), in fp32, rounded once to the
  * tensor's dtype.  out[i] may be grads[i]; no other overlap, and no tensor twice among out.  max_norm >= 0.  So gradients of a norm that is not a number stay as they
- * are, and those of an infinite norm become zeros, and NaN where they are infinite.  No counterpart in the reference. */
+ * are, and those of an infinite norm (also one past fp32's range) become zeros, and NaN where they are infinite.  No counterpart in the reference. */
 int mg_clip_grads(const void* const* grads, void* const* out, const int64_t* numels, const int* dtypes, int64_t count, float max_norm,
                   float* norm, mg_stream stream);
 
@@ -656,7 +656,7 @@ int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y,
  *   dw(2F,K) = dg^T x | du^T x
  *   db(2F)  = column sums of dg | du (NULL to skip).
  * act'(0) of max(g, 0) is 0.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the unrounded fp32 sums.  M == 0: dw and db
- * are zeros. */
+ * are zeros.  Nothing overlaps. */
 int mg_gated_linear_bwd(const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t F,
                         int64_t K, int dx_accumulate, int gate, int dtype, int grad_dtype, mg_stream stream);
 /* The same with the sums of dw and db deferred (see mg_deferred). */

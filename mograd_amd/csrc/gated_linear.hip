@@ -81,7 +81,9 @@ static int launch_gated_split(const void* x, const void* w, const void* bias, vo
   return MG_OK;
 }
 
-// [dg du] from dy, g and u, rounded to the tensors' type as the products take it.  Bound by its bytes, five values an output.
+// [dg du] from dy, g and u, rounded to the tensors' type as the products take it.  Bound by its bytes, five values an output: (16384, 1024) bf16
+// 27 us, 6.2 TB/s.  The projections were put away in the forward pass and are read for the last time here: past the caches, which keep
+// what this writes for the products (with them gradients of (16384, 1024 <- 384) bf16 93.9 -> 89.8 us, (32768, 2048 <- 512) 432 -> 427).
 template <typename T, int VEC, int GATE>
 __global__ __launch_bounds__(kGatedThreads) void gate_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ gu, T* __restrict__ dgu,
                                                                 int64_t items, int F, uint32_t per_row, int64_t first_block) {
@@ -91,8 +93,8 @@ __global__ __launch_bounds__(kGatedThreads) void gate_bwd_kernel(const T* __rest
   const int c = static_cast<int>(item - row * per_row) * VEC;
   float d[VEC], g[VEC], u[VEC];
   VecIO<T, VEC>::load(dy + row * F + c, d);
-  VecIO<T, VEC>::load(gu + row * 2 * F + c, g);
-  VecIO<T, VEC>::load(gu + row * 2 * F + F + c, u);
+  VecIO<T, VEC>::load_stream(gu + row * 2 * F + c, g);
+  VecIO<T, VEC>::load_stream(gu + row * 2 * F + F + c, u);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     float act, slope;

@@ -6,10 +6,11 @@
 // (time, height, width of a patch), each pair goes by one of them.
 //
 // The angle.  fp32 positions of a million times a frequency near 1 are off by 0.06 of a radian, so the product is taken in 64 bits,
-// in quarter turns, its whole part dropped there, and only the rest, at most pi / 4, goes to fp32, where the Taylor series of sine
-// and cosine up to t^9 and t^10 are within 2e-9 of them.  (Positions up to 2^31: 4e-7 of a radian, of the product's rounding.)
-// An angle serves all heads of a token: a workgroup takes as many tokens as make a table of up to 256 pairs, a thread an entry, and
-// then walks the tokens' columns with the table in LDS.  Bound by its bytes.
+// in turns, its whole part dropped there, then that of quarter turns, and only the rest, at most pi / 4, goes to fp32, where the Taylor
+// series of sine and cosine up to t^9 and t^10 are within 2e-9 of them.  (Positions up to 2^31: 4e-7 of a radian, of the product's rounding.)
+// An angle serves all heads of a token: a workgroup takes as many tokens as make a table of 256 pairs, or up to 1024 where its heads are
+// few, and then walks the tokens' columns with the table in LDS.  Bound by its bytes: (1, 32768, 32, 128) bf16 99 us, 5.4 TB/s.  Heads whose
+// columns are no whole chunks go by chunks at any address, and the few columns left over one by one: 66 columns 100 us, 2.8 TB/s.
 #include <algorithm>
 
 #include "mg_device.h"
@@ -20,6 +21,7 @@ namespace mg {
 
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryPairs = 256;  // the most that a head's columns may have
+constexpr int kRotaryTable = 1024, kRotaryTokens = 256;  // the most that a workgroup has of them, and of tokens
 
 template <typename T>
 struct Rotary {
@@ -35,23 +37,23 @@ struct Rotary {
   uint8_t axis[kRotaryPairs];
 };
 
-// Sine and cosine of `turns` quarter turns, which fp32 need not hold.
-__device__ __forceinline__ float2 rotary_sincos(double quarters) {
-  const double whole = rint(quarters);
+// Sine and cosine of `turns` turns.
+__device__ __forceinline__ float2 rotary_sincos(double turns) {
+  const double quarters = 4.0 * (turns - rint(turns)), whole = rint(quarters);
   const float t = static_cast<float>((quarters - whole) * 1.5707963267948966);
   const float q = t * t;
   const float s = t + t * q * (-1.6666667e-1f + q * (8.3333333e-3f + q * (-1.9841270e-4f + q * 2.7557319e-6f)));
   const float c = 1.f + q * (-0.5f + q * (4.1666667e-2f + q * (-1.3888889e-3f + q * (2.4801587e-5f + q * -2.7557319e-7f))));
-  const int n = static_cast<int>(static_cast<int64_t>(whole) & 3);
+  const int n = static_cast<int>(whole) & 3;
   const float a = n & 1 ? c : s, b = n & 1 ? s : c;
   return make_float2(n & 2 ? -a : a, (n == 1 || n == 2) ? -b : b);
 }
 
-// ANY: chunks at any address.  VEC == 1: a pair at a time.
-template <typename T, int VEC, bool ANY>
+// ANY: chunks at any address, and what is left over of the pairs and of the rest goes a pair, or a column, at a time.
+template <typename T, bool ANY>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(Rotary<T> r, int64_t first_block) {
-  __shared__ float2 table[kRotaryPairs];  // (sin, cos)
-  __shared__ int64_t at_x[kRotaryPairs], at_y[kRotaryPairs];
+  __shared__ float2 table[kRotaryTable];  // (sin, cos)
+  __shared__ int64_t at_x[kRotaryTokens], at_y[kRotaryTokens];
   const int64_t token0 = (first_block + blockIdx.x) * r.tokens_per_block;
   const int here = static_cast<int>(min(static_cast<int64_t>(r.tokens_per_block), r.tokens - token0));
   const int tid = threadIdx.x;
@@ -60,8 +62,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(Rotary<T> r, int
     at_x[tid] = b * r.xs[0] + s * r.xs[1];
     at_y[tid] = b * r.ys[0] + s * r.ys[1];
   }
-  if (tid < here * r.pairs) {
-    const int tk = tid / r.pairs, i = tid - tk * r.pairs;
+  for (int entry = tid; entry < here * r.pairs; entry += kRotaryThreads) {
+    const int tk = entry / r.pairs, i = entry - tk * r.pairs;
     const int64_t token = token0 + tk, b = token / r.S, s = token - b * r.S;
     double position;
     if (!r.positions) {
@@ -71,12 +73,13 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(Rotary<T> r, int
       position = r.wide_positions ? static_cast<double>(static_cast<const int64_t*>(r.positions)[at])
                                   : static_cast<double>(static_cast<const int32_t*>(r.positions)[at]);
     }
-    float2 sc = rotary_sincos(position * (static_cast<double>(r.inv_freq[i]) * 0.63661977236758134));
+    float2 sc = rotary_sincos(position * (static_cast<double>(r.inv_freq[i]) * 0.15915494309189535));
     if (r.inverse) sc.x = -sc.x;
-    table[tid] = sc;
+    table[entry] = sc;
   }
   __syncthreads();
 
+  constexpr int VEC = WideVec<T>::value;
   auto load = [](const T* p, float (&v)[VEC]) {
     if constexpr (ANY) VecAny<T, VEC>::load(p, v);
     else VecIO<T, VEC>::load(p, v);
@@ -85,27 +88,30 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(Rotary<T> r, int
     if constexpr (ANY) VecAny<T, VEC>::store(p, v);
     else VecIO<T, VEC>::store(p, v);
   };
-  // Items of a head: chunks of pairs (halves: a chunk of either half; neighbours: VEC / 2 pairs, one at least), then those of the rest.
-  const int turned = r.neighbours && VEC > 1 ? 2 * r.pairs / VEC : r.pairs / VEC, per_head = turned + r.rest / VEC;
+  // Items of a head: chunks of pairs (halves: a chunk of either half; neighbours: VEC / 2 pairs), chunks of the rest, and what is left over.
+  const int a0 = r.neighbours ? 2 * r.pairs / VEC : r.pairs / VEC, a1 = a0 + r.rest / VEC;
+  const int done = r.neighbours ? a0 * (VEC / 2) : a0 * VEC;  // pairs in chunks
+  const int a2 = ANY ? a1 + r.pairs - done : a1, per_head = ANY ? a2 + r.rest % VEC : a2;
   const int items = here * r.heads * per_head;
   for (int item = tid; item < items; item += kRotaryThreads) {
     const int row = item / per_head, c = item - row * per_head, tk = row / r.heads, h = row - tk * r.heads;
     const T* const x = r.x + at_x[tk] + h * r.xs[2];
     T* const y = r.y + at_y[tk] + h * r.ys[2];
-    if (c >= turned) {
-      const int at = 2 * r.pairs + (c - turned) * VEC;
+    const float2* const sc = table + tk * r.pairs;
+    if (c >= a0 && c < a1) {
+      const int at = 2 * r.pairs + (c - a0) * VEC;
       if (x == y) continue;
       float v[VEC];
       load(x + at, v);
       store(y + at, v);
-      continue;
-    }
-    const float2* const sc = table + tk * r.pairs;
-    if constexpr (VEC == 1) {
-      const int a = r.neighbours ? 2 * c : c, b = r.neighbours ? 2 * c + 1 : c + r.pairs;
+    } else if (ANY && c >= a2) {
+      const int at = 2 * r.pairs + r.rest / VEC * VEC + c - a2;
+      if (x != y) y[at] = x[at];
+    } else if (ANY && c >= a1) {
+      const int i = done + c - a1, a = r.neighbours ? 2 * i : i, b = r.neighbours ? 2 * i + 1 : i + r.pairs;
       const float va = to_float(x[a]), vb = to_float(x[b]);
-      y[a] = from_float<T>(va * sc[c].y - vb * sc[c].x);
-      y[b] = from_float<T>(va * sc[c].x + vb * sc[c].y);
+      y[a] = from_float<T>(va * sc[i].y - vb * sc[i].x);
+      y[b] = from_float<T>(va * sc[i].x + vb * sc[i].y);
     } else if (r.neighbours) {
       float v[VEC];
       load(x + c * VEC, v);
@@ -138,18 +144,19 @@ template <typename T>
 static int launch_rotary(Rotary<T> r, hipStream_t stream) {
   constexpr int VEC = WideVec<T>::value;
   constexpr int64_t kBlocks = 1 << 23;  // of a launch, which counts its threads in 32 bits
-  // A table of up to 256 entries, but a workgroup or two a CU first.
+  // A table of 256 entries, of more where the tokens' columns are few chunks for 256 threads, but a workgroup or two a CU first.
   const int64_t few = std::max<int64_t>(1, r.tokens / (2 * device_info().cu_count));
-  r.tokens_per_block = static_cast<int>(std::min<int64_t>(kRotaryPairs / r.pairs, few));
+  const int64_t chunks_of_token = std::max<int64_t>(1, static_cast<int64_t>(r.heads) * (r.pairs + r.rest) / VEC);
+  const int64_t full = std::max<int64_t>(256 / r.pairs, std::min<int64_t>(kRotaryTable / r.pairs, ceil_div(512, chunks_of_token)));
+  r.tokens_per_block = static_cast<int>(std::min<int64_t>({full, few, kRotaryTokens}));
   const bool chunks = (r.neighbours ? 2 * r.pairs : r.pairs) % VEC == 0 && r.rest % VEC == 0;
-  bool on_chunks = aligned16(r.x) && aligned16(r.y);
+  bool on_chunks = chunks && aligned16(r.x) && aligned16(r.y);
   for (int i = 0; i < 3; ++i) on_chunks = on_chunks && r.xs[i] % VEC == 0 && r.ys[i] % VEC == 0;
   const int64_t blocks = ceil_div(r.tokens, r.tokens_per_block);
   for (int64_t first = 0; first < blocks; first += kBlocks) {
     const dim3 grid(static_cast<unsigned>(std::min(blocks - first, kBlocks))), threads(kRotaryThreads);
-    if (!chunks) hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, threads, 0, stream, r, first);
-    else if (on_chunks) hipLaunchKernelGGL((rotary_kernel<T, VEC, false>), grid, threads, 0, stream, r, first);
-    else hipLaunchKernelGGL((rotary_kernel<T, VEC, true>), grid, threads, 0, stream, r, first);
+    if (on_chunks) hipLaunchKernelGGL((rotary_kernel<T, false>), grid, threads, 0, stream, r, first);
+    else hipLaunchKernelGGL((rotary_kernel<T, true>), grid, threads, 0, stream, r, first);
     MG_LAUNCH_CHECK();
   }
   return MG_OK;
@@ -178,6 +185,7 @@ int mg_rotary(const void* x, void* y, const void* positions, const float* inv_fr
   for (int i = 0; i < 3; ++i) {
     if (x_strides[i] < 0 || y_strides[i] < 0) return mg::fail(MG_ERR_INVALID, "%s: negative stride", who);
     if (extents[i] > 1 && y_strides[i] == 0) return mg::fail(MG_ERR_INVALID, "%s: y's rows lie on each other", who);
+    if (extents[i] > 1 && x == y && x && x_strides[i] != y_strides[i]) return mg::fail(MG_ERR_INVALID, "%s: in place with other strides", who);
   }
   const int pairs = static_cast<int>(rotated / 2);
   if (positions) {

@@ -48,7 +48,7 @@ def test_refusals():
     for bad in (dict(dtype=I32), dict(dtype=7), dict(B=-1), dict(S=-1), dict(H=-1), dict(D=0), dict(D=6), dict(rotated=0), dict(rotated=7), dict(rotated=-2),
                 dict(D=600, rotated=514), dict(B=1 << 41), dict(B=1 << 30, S=1 << 20), dict(xs=None), dict(ys=None), dict(ps=None),
                 dict(xs=i64s(-1, 32, 16)), dict(ys=i64s(96, -32, 16)), dict(ys=i64s(96, 32, 0)), dict(ps=i64s(6, 3, -1)), dict(pos=F32), dict(pos=BF16), dict(axes=0),
-                dict(axes=256), dict(axes=2), dict(axis=None), dict(axis=i32s([0, -1, 0, 0])), dict(x=None), dict(y=None), dict(inv_freq=None)):
+                dict(axes=256), dict(axes=2), dict(axis=None), dict(axis=i32s([0, -1, 0, 0])), dict(x=None), dict(y=None), dict(inv_freq=None), dict(xs=i64s(192, 64, 16))):
         with pytest.raises(MogradError) as e:
             call(**bad)
         assert e.value.status == 1 and "rotary" in str(e.value), bad
