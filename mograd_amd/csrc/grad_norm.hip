@@ -124,6 +124,15 @@ __global__ __launch_bounds__(kNormThreads) void norm_finish_kernel(const double*
   if (threadIdx.x == 0) *norm = v;
 }
 
+// The sum of `count` sums, as norm_of_sums adds them, which finds one then.
+__global__ __launch_bounds__(kNormThreads) void norm_total_kernel(const double* __restrict__ sums, int64_t count, double* __restrict__ total) {
+  __shared__ double slots[kNormThreads / kWave];
+  double v = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += kNormThreads) v += sums[i];
+  v = norm_block_sum(v, slots);
+  if (threadIdx.x == 0) *total = v;
+}
+
 // SAME: in and out lie alike on their 16-byte chunks, as they do where out is in.
 template <typename T, bool SAME>
 __device__ __forceinline__ void clip_chunks(const T* in, T* out, int64_t n, float scale) {
@@ -239,8 +248,8 @@ static int grad_norm(const char* who, const void* const* grads, void* const* out
     CaptureHold hold;
     MG_TRY(hold.begin(s));
     Scratch mem;
-    MG_TRY(mem.take(pieces * static_cast<int64_t>(sizeof(double))));
-    double* const sums = mem.as<double>();
+    MG_TRY(mem.take((pieces + 1) * static_cast<int64_t>(sizeof(double))));
+    double* sums = mem.as<double>();
     MG_TRY(norm_launches(grads, nullptr, numels, dtypes, count, piece, [&](const NormTensors& t, unsigned blocks, int64_t before) {
       hipLaunchKernelGGL(norm_sums_kernel, dim3(blocks), dim3(kNormThreads), 0, s, t, piece, sums + before);
     }));
@@ -248,6 +257,12 @@ static int grad_norm(const char* who, const void* const* grads, void* const* out
       hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(kNormThreads), 0, s, sums, pieces, norm);
       MG_LAUNCH_CHECK();
       return MG_OK;
+    }
+    // Of thousands of tensors there are as many more pieces; then the sums are added up once, and not in each workgroup.
+    if (pieces > 4 * kNormPieces) {
+      hipLaunchKernelGGL(norm_total_kernel, dim3(1), dim3(kNormThreads), 0, s, sums, pieces, sums + pieces);
+      MG_LAUNCH_CHECK();
+      sums += pieces, pieces = 1;
     }
     return norm_launches(grads, out, numels, dtypes, count, piece, [&](const NormTensors& t, unsigned blocks, int64_t before) {
       hipLaunchKernelGGL(clip_kernel, dim3(blocks), dim3(kNormThreads), 0, s, t, piece, sums, pieces, max_norm, before == 0 ? norm : nullptr);

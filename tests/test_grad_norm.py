@@ -209,3 +209,26 @@ def test_twice_gives_the_same_bits(device):
     g = _gradients(604, [100000, 33, 4096], [F32, BF16, F16])
     a, b = (_clip(device, g, [F32, BF16, F16], 0.7) for _ in range(2))
     assert a[0] == b[0] and all(np.array_equal(x, y) for x, y in zip(a[1], b[1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_thousands_of_small_tensors(device, dtype):
+    """More pieces than each workgroup adds up for itself; the tensors lie in one array, without gaps."""
+    sizes = [i % 6 for i in range(10001)]
+    g = _gradients(605, sizes, [dtype] * len(sizes))
+    flat = np.concatenate(g)
+    start = np.cumsum([0] + sizes)
+    buf, out = AnyBuffer.from_numpy(device, flat, dtype), AnyBuffer.create(dtype, device, flat.size, fill=7.0)
+    norm, norm2 = (AnyBuffer.create(F32, device, 1, fill=-1.0) for _ in range(2))
+    at = lambda b: [AnyBuffer(b.storage, dtype, n, int(k)).data_ptr().value if n else None for n, k in zip(sizes, start)]
+    want_norm, want = O.clip_grads(g, O.grad_norm(g) * 0.4)
+    p, n, t = _arrays(at(buf), sizes, [dtype] * len(sizes))
+    most = float(O.grad_norm(g) * 0.4)
+    device.lib.mg_clip_grads(p, (C.c_void_p * len(sizes))(*at(out)), n, t, len(sizes), most, norm.data_ptr(), device.stream)
+    device.lib.mg_grad_norm(p, n, t, len(sizes), norm2.data_ptr(), device.stream)
+    assert norm.to_numpy()[0] == norm2.to_numpy()[0]
+    assert abs(norm.to_numpy()[0] - want_norm) <= 2 * U * want_norm
+    w = np.concatenate(want)
+    _close(out.to_numpy(), w, _half_step(w, dtype) + 4 * U * np.abs(w), "clipped")
+    assert np.array_equal(buf.to_numpy(), flat)
