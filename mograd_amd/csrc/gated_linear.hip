@@ -106,35 +106,42 @@ __global__ __launch_bounds__(kGatedThreads) void gate_bwd_kernel(const T* __rest
   VecIO<T, VEC>::store(dgu + row * 2 * F + F + c, u);
 }
 
-// The same in fp32, and the column sums of [dg du] over each group of kGateRows rows, (groups, 2 F): a workgroup takes 64 chunks of columns
-// of a group, four rows at a time, and adds up what its threads have of a column in LDS.
+// The same, and the column sums of [dg du], before they are rounded, over each group of `rows` rows, (groups, 2 F): a workgroup takes 64
+// chunks of columns of a group, four rows at a time, and adds up what its threads have of a column in LDS.  (The products' own column sums
+// would be those of rounded values, 1.4 times as far from the exact ones as a rounding of db alone.)
 constexpr int kGateRows = 32;
-template <int VEC, int GATE>
-__global__ __launch_bounds__(kGatedThreads) void gate_bwd_sums_kernel(const float* __restrict__ dy, const float* __restrict__ gu,
-                                                                     float* __restrict__ dgu, float* __restrict__ sums, int M, int F, int blocks_f) {
+template <typename T, int VEC, int GATE>
+__global__ __launch_bounds__(kGatedThreads) void gate_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ gu, T* __restrict__ dgu,
+                                                                     float* __restrict__ sums, int M, int F, int blocks_f, int rows) {
   __shared__ float parts[4][2][64 * VEC];
   const int bf = blockIdx.x % blocks_f, group = blockIdx.x / blocks_f, tx = threadIdx.x % 64, ty = threadIdx.x / 64;
-  const int c = (bf * 64 + tx) * VEC, r0 = group * kGateRows;
+  const int c = (bf * 64 + tx) * VEC;
+  const int64_t r0 = static_cast<int64_t>(group) * rows, r1 = min(r0 + rows, static_cast<int64_t>(M));
   float sg[VEC], su[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) sg[i] = su[i] = 0.f;
   if (c < F) {
-    for (int r = r0 + ty; r < min(r0 + kGateRows, M); r += 4) {
-      const int64_t row = r;
+#pragma unroll 2
+    for (int64_t row = r0 + ty; row < r1; row += 4) {
       float d[VEC], g[VEC], u[VEC];
-      VecIO<float, VEC>::load(dy + row * F + c, d);
-      VecIO<float, VEC>::load(gu + row * 2 * F + c, g);
-      VecIO<float, VEC>::load(gu + row * 2 * F + F + c, u);
+      VecIO<T, VEC>::load(dy + row * F + c, d);
+      if constexpr (sizeof(T) == 2) {
+        VecIO<T, VEC>::load_stream(gu + row * 2 * F + c, g);
+        VecIO<T, VEC>::load_stream(gu + row * 2 * F + F + c, u);
+      } else {
+        VecIO<T, VEC>::load(gu + row * 2 * F + c, g);
+        VecIO<T, VEC>::load(gu + row * 2 * F + F + c, u);
+      }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         float act, slope;
-        gated_act_slope<false, GATE>(g[i], act, slope);
+        gated_act_slope<sizeof(T) == 2, GATE>(g[i], act, slope);
         g[i] = d[i] * u[i] * slope;
         u[i] = d[i] * act;
         sg[i] += g[i], su[i] += u[i];
       }
-      VecIO<float, VEC>::store(dgu + row * 2 * F + c, g);
-      VecIO<float, VEC>::store(dgu + row * 2 * F + F + c, u);
+      VecIO<T, VEC>::store(dgu + row * 2 * F + c, g);
+      VecIO<T, VEC>::store(dgu + row * 2 * F + F + c, u);
     }
   }
 #pragma unroll
@@ -178,6 +185,45 @@ static int gate_bwd(const void* dy, const void* gu, void* dgu, int64_t M, int64_
     hipLaunchKernelGGL((gate_bwd_kernel<T, decltype(vec)::value, decltype(g)::value>), grid, dim3(kGatedThreads), 0, stream,
                        static_cast<const T*>(dy), static_cast<const T*>(gu), static_cast<T*>(dgu), items, static_cast<int>(F), per_row, first);
   });
+}
+
+// Whether a thread takes 16 bytes, and how many workgroups lie side by side.
+static bool gate_sums_wide(int64_t F, int dtype, const void* dy, const void* gu) {
+  return F % (16 / dtype_size(dtype)) == 0 && aligned16(dy) && aligned16(gu);
+}
+static int64_t gate_sums_across(int64_t F, int dtype, bool wide) { return ceil_div(F, wide ? 64 * 16 / dtype_size(dtype) : 64); }
+
+// Rows of a group in 16 bits: as few as leave four workgroups a CU, four rows at least.  Fewer leave more sums to add, more leave CUs without
+// work: all gradients in bf16 with 4 | 8 | 16 | 32 | 64 rows, us: (512, 2048 <- 1024) 31.5 | 32.8 | 35.6 | 43.0 | 56.4,
+// (4096, 1024 <- 1024) 60.9 | 58.1 | 59.8 | 65.9 | 79.8, (16384, 1024 <- 384) 108.9 | 100.5 | 100.3 | 97.0 | 108.5.
+static int gate_group_rows(int64_t M, int64_t F, int dtype, const void* dy, const void* gu) {
+  const int64_t across = gate_sums_across(F, dtype, gate_sums_wide(F, dtype, dy, gu)), most = 4 * device_info().cu_count;
+  int rows = 4;
+  while (rows < (1 << 24) && ceil_div(M, rows) * across > most && rows < M) rows *= 2;
+  return rows;
+}
+
+// [dg du] and its sums over groups of `rows` rows, for which this takes scratch.
+template <typename T>
+static int gate_bwd_sums(const void* dy, const void* gu, void* dgu, Scratch& sums, int64_t M, int64_t F, int gate, int rows, hipStream_t stream) {
+  constexpr int VEC = WideVec<T>::value;
+  constexpr int kType = sizeof(T) == 4 ? MG_F32 : MG_F16;  // (by its size)
+  const bool wide = gate_sums_wide(F, kType, dy, gu);
+  const int64_t blocks_f = gate_sums_across(F, kType, wide), groups = ceil_div(M, rows);
+  if (blocks_f * groups > 0xffffffffLL / kGatedThreads) return fail(MG_ERR_INVALID, "gated_linear_bwd: too many rows");
+  MG_TRY(sums.take(groups * 2 * F * static_cast<int64_t>(sizeof(float))));
+  gated_with(gate, [&](auto kind) {
+    constexpr int GATE = decltype(kind)::value;
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks_f * groups)), dim3(kGatedThreads), 0, stream, static_cast<const T*>(dy),
+                         static_cast<const T*>(gu), static_cast<T*>(dgu), sums.as<float>(), static_cast<int>(M), static_cast<int>(F),
+                         static_cast<int>(blocks_f), rows);
+    };
+    if (wide) launch(gate_bwd_sums_kernel<T, VEC, GATE>);
+    else launch(gate_bwd_sums_kernel<T, 1, GATE>);
+  });
+  MG_LAUNCH_CHECK();
+  return MG_OK;
 }
 
 // Which kernel a forward pass takes: the least of these estimates, in us.  kGatedDirect: gated_direct.h; kGatedSmall: 64 x 64 tiles, K in
@@ -376,21 +422,7 @@ static int gated_bwd_split(const void* dy, const void* gu, const void* x, const 
   Scratch dgu, db_part, partial;
   MG_TRY(dgu.take(M * N * static_cast<int64_t>(sizeof(float))));
   if (db) {
-    MG_TRY(db_part.take(groups * N * static_cast<int64_t>(sizeof(float))));
-    const bool wide = F % 4 == 0 && aligned16(dy) && aligned16(gu);
-    const int64_t blocks_f = ceil_div(F, wide ? 256 : 64);
-    if (blocks_f * groups > 0xffffffffLL / kGatedThreads) return fail(MG_ERR_INVALID, "gated_linear_bwd: too many rows");
-    const dim3 grid(static_cast<unsigned>(blocks_f * groups));
-    gated_with(gate, [&](auto kind) {
-      constexpr int GATE = decltype(kind)::value;
-      auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(kGatedThreads), 0, stream, static_cast<const float*>(dy), static_cast<const float*>(gu), dgu.as<float>(),
-                           db_part.as<float>(), static_cast<int>(M), static_cast<int>(F), static_cast<int>(blocks_f));
-      };
-      if (wide) launch(gate_bwd_sums_kernel<4, GATE>);
-      else launch(gate_bwd_sums_kernel<1, GATE>);
-    });
-    MG_LAUNCH_CHECK();
+    MG_TRY(gate_bwd_sums<float>(dy, gu, dgu.as<char>(), db_part, M, F, gate, kGateRows, stream));
   } else {
     MG_TRY(gate_bwd<float>(dy, gu, dgu.as<char>(), M, F, gate, stream));
   }
@@ -457,14 +489,31 @@ static int gated_bwd(const char* who, const void* dy, const void* gu, const void
       if (choice.way == kGatedSplit)
         return gated_bwd_split(dy, gu, x, w, dx, dw, db, M, F, K, dx_accumulate != 0, gate, choice.tile, choice.splits, list, s);
     }
-    Scratch dgu;
+    Scratch dgu, db_part;
     MG_TRY(dgu.take(M * 2 * F * dtype_size(dtype)));
+    const bool sums = db && dtype != MG_F32;
+    const int rows = sums ? gate_group_rows(M, F, dtype, dy, gu) : 0;
     switch (dtype) {
       case MG_F32: MG_TRY(gate_bwd<float>(dy, gu, dgu.as<char>(), M, F, gate, s)); break;
-      case MG_F16: MG_TRY(gate_bwd<f16_t>(dy, gu, dgu.as<char>(), M, F, gate, s)); break;
-      default: MG_TRY(gate_bwd<bf16_t>(dy, gu, dgu.as<char>(), M, F, gate, s)); break;
+      case MG_F16:
+        if (sums) MG_TRY(gate_bwd_sums<f16_t>(dy, gu, dgu.as<char>(), db_part, M, F, gate, rows, s));
+        else MG_TRY(gate_bwd<f16_t>(dy, gu, dgu.as<char>(), M, F, gate, s));
+        break;
+      default:
+        if (sums) MG_TRY(gate_bwd_sums<bf16_t>(dy, gu, dgu.as<char>(), db_part, M, F, gate, rows, s));
+        else MG_TRY(gate_bwd<bf16_t>(dy, gu, dgu.as<char>(), M, F, gate, s));
+        break;
     }
-    auto products = [&] { return mg_linear_bwd_fused(dgu.as<char>(), x, w, dx, dw, db, M, 2 * F, K, dx_accumulate, 0, dtype, stream); };
+    auto products = [&]() -> int {
+      MG_TRY(mg_linear_bwd_fused(dgu.as<char>(), x, w, dx, dw, sums ? nullptr : db, M, 2 * F, K, dx_accumulate, 0, dtype, stream));
+      if (!sums) return MG_OK;
+      const int64_t groups = ceil_div(M, rows);
+      const int cus = device_info().cu_count;
+      if (dtype == MG_F16) reduce_partials_or_defer<f16_t>(db_part, static_cast<f16_t*>(db), nullptr, nullptr, groups, 2 * F, cus, s);
+      else reduce_partials_or_defer<bf16_t>(db_part, static_cast<bf16_t*>(db), nullptr, nullptr, groups, 2 * F, cus, s);
+      MG_LAUNCH_CHECK();
+      return MG_OK;
+    };
     if (list) {
       DeferredScope scope(list, dtype, grad_dtype);
       return products();

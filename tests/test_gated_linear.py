@@ -326,3 +326,20 @@ def test_twice_gives_the_same_bits(device):
     for n in a:
         assert np.array_equal(a[n], b[n]), n
     assert np.array_equal(_forward(device, p, BF16, "silu")[0], _forward(device, p, BF16, "silu")[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("M,F,K", [(1, 1, 8), (3, 40, 24), (37, 130, 16), (300, 1001, 64), (2100, 136, 40), (5000, 1024, 8), (4097, 77, 9)])
+def test_bias_gradients_are_sums_of_unrounded_values(device, M, F, K, dtype):
+    """db is rounded once, as its own type: none of the rounding of the projections' gradients is in it."""
+    for i, gate in enumerate(GATES):
+        p = _inputs(640 + i, M, F, K, dtype, bias=False)
+        _, _, db, d = O.gated_linear_bwd(p["dy"], p["gu"], p["x"], p["w"], gate)
+        act_off, slope_off = _act_error(p["gu"][:, :F].astype(np.float64), gate, 0.0)
+        dy = np.abs(p["dy"])
+        off = np.concatenate([dy * np.abs(p["gu"][:, F:]) * slope_off, dy * act_off], axis=1) + 4 * U * np.abs(d)
+        bound = off.sum(0) + (M + 16) * U * (np.abs(d) + off).sum(0)
+        for grads in (dtype, F32):
+            got = _backward(device, p, dtype, grads, gate)["db"]
+            _close(got, db, bound + _half_step(np.abs(db) + bound, grads), "db")
