@@ -91,18 +91,18 @@ __device__ __forceinline__ void gated_act_slope(float g, float& act, float& slop
   }
 }
 
-// Calls f with act as a function for 16-bit outputs.  The three gates made of a sigmoid share their code, s (a0 + a1 g) with s the
-// sigmoid of g (c1 + c3 g^2), so that a kernel's epilogue has three copies of its loops and not five.
+// Calls f with act as a function for 16-bit outputs.  The three gates made of a sigmoid share their code, s times g or 1 with s the
+// sigmoid of g (c1 + c3 g^2), so that a kernel's epilogue has three copies of its loops and not five.  (g or 1 is a choice and no sum
+// a0 + a1 g: 0 g is NaN for an infinite g, where the sigmoid is 1 or 0.)
 template <typename F>
 __device__ __forceinline__ void gated_with_fast(int gate, F&& f) {
   if (gate == MG_GATE_RELU) return f([](float g) { return gated_act<true, MG_GATE_RELU>(g); });
   if (gate == MG_GATE_GELU) return f([](float g) { return gated_act<true, MG_GATE_GELU>(g); });
   const bool tanh = gate == MG_GATE_GELU_TANH, plain = gate == MG_GATE_SIGMOID;
   const float c1 = -1.44269504f * (tanh ? kGeluTanh2C : 1.f), c3 = tanh ? -1.44269504f * 0.044715f * kGeluTanh2C : 0.f;
-  const float a0 = plain ? 1.f : 0.f, a1 = plain ? 0.f : 1.f;
   f([=](float g) {
     const float e = __builtin_amdgcn_exp2f(g * fmaf(c3, fminf(g * g, 1e30f), c1));
-    return __builtin_amdgcn_rcpf(1.f + e) * fmaf(a1, g, a0);
+    return __builtin_amdgcn_rcpf(1.f + e) * (plain ? 1.f : g);
   });
 }
 
