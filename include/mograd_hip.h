@@ -10,9 +10,9 @@
  *   - All data pointers are DEVICE pointers unless a parameter is documented as host.
  *   - The caller owns inputs and outputs.  Outputs need no initialisation.  Scratch is
  *     taken from the library's pool and returned before the call returns (mg_linear_bwd_act8,
- *     mg_residual_norm_bwd, mg_gated_linear_fwd, mg_gated_linear_bwd, mg_grad_norm and
- *     mg_clip_grads on a stream that is being captured keep it for the graph, see
- *     mg_pool_free_recorded); this is safe because all work of one call is enqueued on the
+ *     mg_residual_norm_bwd, mg_gated_linear_fwd, mg_gated_linear_bwd and its `_deferred` form, mg_grad_norm
+ *     and mg_clip_grads on a stream that is being captured keep it for the graph, see
+ *     mg_pool_free_recorded; the other `_deferred` forms do not); this is safe because all work of one call is enqueued on the
  *     one stream passed in, and the pool hands memory back out only to later calls (the
  *     reference's single in-order-stream contract, mograd/memory.mojo:27-31).  This makes
  *     the library a one-stream-per-device library: every entry point that takes scratch
@@ -682,9 +682,11 @@ int mg_rotary(const void* x, void* y, const void* positions, const float* inv_fr
               int64_t H, int64_t D, int64_t rotated, const int64_t* x_strides, const int64_t* y_strides, const int64_t* pos_strides,
               int axes, int pos_dtype, int neighbours, int inverse, int dtype, mg_stream stream);
 
-/* mg_linear_bwd_act8, mg_residual_norm_bwd, mg_gated_linear_fwd, mg_gated_linear_bwd, mg_grad_norm and mg_clip_grads take scratch from
- * the pool.  Recorded into a HIP graph they keep it: what such a call took goes only to calls that are recorded on the same stream in the same capture, so that graphs, the branches of a graph, and
- * eager calls never share it.  It stays so, also where the capture fails, until mg_pool_free_recorded. */
+/* mg_linear_bwd_act8, mg_residual_norm_bwd, mg_gated_linear_fwd, mg_gated_linear_bwd, mg_gated_linear_bwd_deferred, mg_grad_norm and
+ * mg_clip_grads take scratch from the pool.  Recorded into a HIP graph they keep it: what such a call took goes only to calls that are
+ * recorded on the same stream in the same capture, so that graphs, the branches of a graph, and eager calls never share it.  It stays so,
+ * also where the capture fails, until mg_pool_free_recorded.  Of the `_deferred` form that is also what its list holds; the list is
+ * finished on the same stream in the same capture. */
 
 #ifdef __cplusplus
 }

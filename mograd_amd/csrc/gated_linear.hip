@@ -483,7 +483,7 @@ static int gated_bwd(const char* who, const void* dy, const void* gu, const void
   hipStream_t s = to_stream(stream);
   return without_exceptions(who, [&]() -> int {
     CaptureHold hold;
-    if (!list) MG_TRY(hold.begin(s));  // (a list's blocks outlive the call, and go back to the pool with it)
+    MG_TRY(hold.begin(s));
     if (dtype == MG_F32) {
       const GatedChoice choice = choose_gated_bwd_f32(M, F, K, dx != nullptr, db != nullptr);
       if (choice.way == kGatedSplit)

@@ -63,7 +63,7 @@ class Scratch {
 
 // For the length of an entry point's call on a stream that is being captured into a graph: what the call takes from the pool goes
 // only to calls that are recorded on the same stream in the same capture, which run behind it in every replay, since every replay
-// writes it again; mg_pool_free_recorded ends that.  The pool may ask the driver for memory in the midst of the capture.  (No effect
+// writes it again (also what a list of pending sums keeps beyond the call); mg_pool_free_recorded ends that.  The pool may ask the driver for memory in the midst of the capture.  (No effect
 // on other streams.)
 class CaptureHold {
  public:

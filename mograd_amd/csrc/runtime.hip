@@ -96,6 +96,8 @@ struct Pool {
   FreeLists free_lists;
   std::map<Recording, FreeLists> recorded;  // (the blocks are still in `live`)
   std::unordered_map<void*, int64_t> live;  // ptr -> class bytes (pooled) or -nbytes (unpooled)
+  // Blocks taken for a recording, which they go back to whoever releases them, and when: a list of pending sums does so after the call.
+  std::unordered_map<void*, Recording> taken_for;
   mg_pool_stats stats{};
 };
 
@@ -218,6 +220,7 @@ int pool_take(void** out, int64_t nbytes) {
       return fail(MG_ERR_OOM, "mograd: out of device memory allocating %s", fmt_bytes(n).c_str());
     }
     pool.live[p] = cls;
+    if (t_holding) pool.taken_for[p] = t_recording;
     *out = p;
     return MG_OK;
   }
@@ -246,6 +249,7 @@ int pool_take(void** out, int64_t nbytes) {
     pool.stats.reserved_bytes += cls;
   }
   pool.live[p] = cls;
+  if (t_holding) pool.taken_for[p] = t_recording;
   mg_pool_stats& s = pool.stats;
   s.allocated_bytes += cls;
   if (s.allocated_bytes > s.peak_allocated) s.peak_allocated = s.allocated_bytes;
@@ -258,9 +262,9 @@ static int release_locked(Pool& pool, void* ptr) {
   auto it = pool.live.find(ptr);
   if (it == pool.live.end()) return fail(MG_ERR_INVALID, "pool_free: pointer %p was not allocated by this pool", ptr);
   const int64_t cls = it->second;
-  if (t_holding) {
+  if (auto own = pool.taken_for.find(ptr); own != pool.taken_for.end()) {
     try {
-      pool.recorded[t_recording][cls].push_back(ptr);
+      pool.recorded[own->second][cls].push_back(ptr);
     } catch (const std::exception&) {  // (no memory for the list: the block stays the graph's)
     }
     return MG_OK;
@@ -285,6 +289,7 @@ int pool_release(void* ptr) {
 static int free_recorded() {
   std::lock_guard<std::mutex> lock(g_pool_mu);
   Pool& pool = current_pool();
+  pool.taken_for.clear();
   for (auto& recording : pool.recorded)
     for (auto& list : recording.second)
       while (!list.second.empty()) {
