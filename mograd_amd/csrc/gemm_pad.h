@@ -37,8 +37,8 @@ __device__ __forceinline__ void pad_columns(int b, const PadJobs<T>& jobs) {
   reinterpret_cast<uint4*>(j.dst)[i] = gemm_gather_chunk(src, j.cols - c0);
 }
 template <typename T>
-__global__ __launch_bounds__(256) void pad_columns_kernel(PadJobs<T> jobs) {
-  pad_columns(blockIdx.x, jobs);
+__global__ __launch_bounds__(256) void pad_columns_kernel(PadJobs<T> jobs, int first_block) {
+  pad_columns(first_block + static_cast<int>(blockIdx.x), jobs);
 }
 // The same, and an activation in 8 bits restored by the first workgroups.
 template <typename T>
@@ -78,8 +78,12 @@ struct PadCopies {
   int launch(hipStream_t stream) {
     if (count == 0 || blocks == 0) return MG_OK;
     if (blocks > 0x7fffffffLL) return fail(MG_ERR_INVALID, "matmul: operand too large");
-    hipLaunchKernelGGL((pad_columns_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, jobs);
-    MG_LAUNCH_CHECK();
+    constexpr int64_t kBlocks = 1 << 23;  // of a launch, which counts its threads in 32 bits
+    for (int64_t first = 0; first < blocks; first += kBlocks) {
+      hipLaunchKernelGGL((pad_columns_kernel<T>), dim3(static_cast<unsigned>(std::min(blocks - first, kBlocks))), dim3(256), 0, stream, jobs,
+                         static_cast<int>(first));
+      MG_LAUNCH_CHECK();
+    }
     return MG_OK;
   }
   // The copies, and `in` restored to (rows, cols) of T, in one launch where there are copies, none of what is restored, and chunks

@@ -80,3 +80,22 @@ except MogradError as e:
 out += [len(launches()), stub.stub_mallocs()]
 """)
     assert got == [3, 0, 0]
+
+
+def test_copies_of_more_chunks_than_a_launch_counts(over_stub):
+    """Odd rows are copied to rows on chunks, a thread a chunk of 16 bytes: 2^24 workgroups of 256 are 2^32 threads.  Every chunk has its
+    thread, also in the other products that make such copies."""
+    got = over_stub(CALLS + """
+def chunks(rows, cols):
+    unit = 64 if cols >= 2048 else 8
+    return -(-rows * (-(-cols // unit) * unit // 8) // 256)
+
+for M, F, K in ((1001, 8192, (1 << 22) - 71), (8192, 1001, (1 << 22) - 71), (1001, 1 << 20, 65537), ((1 << 31) - 1, 1, 17)):
+    forward(M, F, K)
+    out.append((chunks(M, K) + chunks(2 * F, K), sum(l[0] for l in launches()[:-1])))
+lib.mg_matmul_bt(p, p, p, 1, 1 << 25, 129, 2051, 2051, 1, 2051, 1, 0, 0, BF16, None)
+out.append((chunks(1 << 25, 2051) + chunks(129, 2051), sum(l[0] for l in launches()[:-1])))
+""")
+    assert len(got) == 5
+    for least, given in got:
+        assert least >= 1 << 24 and least <= given <= least + 1
