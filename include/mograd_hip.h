@@ -644,8 +644,9 @@ typedef enum mg_gate {
 
 /* y (M,F) = act(x Wg^T + bg) * (x Wu^T + bu) for x (M,K), all contiguous.  w (2F,K) holds Wg's rows, then Wu's; bias (2F) bg, then bu
  * (NULL for none).  gu (M,2F): where the two projections g | u of each row are left for the backward (NULL: nowhere).  `gate`: an
- * mg_gate.  Products and act in fp32, y from the projections before they are rounded.  Any M, F and K from 1, any address of an
- * element; 16-bit tensors: K at most 2^22 - 64.  Nothing overlaps.
+ * mg_gate.  Products and act in fp32, y from the projections before they are rounded.  Any address of an element, any M, F
+ * and K from 1 to 2^28, 16-bit tensors: K at most 2^22 - 64.  (Above, M to 2^31 - 1, F to 2^30 - 1, K to 2^31 - 2^16, a call is taken where its
+ * launches can count their workgroups, and an error elsewhere.)  Nothing overlaps.
  * fp32 products may be taken from three bf16 numbers a value, 24 bits of it: a row or weight that holds an infinity or a number past
  * 3.39e38 then gives NaN, and values below 2^-110 lose digits.  So here and in the gradients. */
 int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y, void* gu, int64_t M, int64_t F, int64_t K, int gate,
@@ -655,8 +656,8 @@ int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y,
  *   dx(M,K) = dg Wg + du Wu     (NULL to skip; dx_accumulate != 0: added to dx)
  *   dw(2F,K) = dg^T x | du^T x
  *   db(2F)  = column sums of dg | du before they are rounded (NULL to skip).
- * act'(0) of max(g, 0) is 0.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the unrounded fp32 sums.  M == 0: dw and db
- * are zeros.  Nothing overlaps. */
+ * act'(0) of max(g, 0) is 0.  Sizes as above, M and 2 F at most 2^31 - 2^16.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the
+ * unrounded fp32 sums.  M == 0: dw and db are zeros.  Nothing overlaps. */
 int mg_gated_linear_bwd(const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t F,
                         int64_t K, int dx_accumulate, int gate, int dtype, int grad_dtype, mg_stream stream);
 /* The same with the sums of dw and db deferred (see mg_deferred). */

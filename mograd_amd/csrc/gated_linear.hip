@@ -403,10 +403,14 @@ static int gated_fwd_16bit(const void* x, const void* w, const void* bias, void*
   return ragged ? launch_gated_small<T, true>(pr, choice.splits, stream) : launch_gated_small<T, false>(pr, choice.splits, stream);
 }
 
+// The longest walk of a product, K of the forward, M and 2 F of the gradients: a split walk's ranges are whole steps, whose ends are counted in
+// 32 bits, so that of (2^31 - 300) rows in 32 ranges the last one would end at 2^31 and be read as far as that.
+constexpr int64_t kGatedLongest = kSplitMost;
+
 static int gated_check(const char* who, int64_t M, int64_t F, int64_t K, int gate, int dtype) {
   if (!is_float_dtype(dtype)) return fail(MG_ERR_INVALID, "%s: unsupported dtype %s", who, dtype_name(dtype));
   if (gate < MG_GATE_SILU || gate > MG_GATE_RELU) return fail(MG_ERR_INVALID, "%s: no such gate: %d", who, gate);
-  if (M < 0 || F <= 0 || K <= 0 || M > 0x7fffffffLL || F > 0x3fffffffLL || K > 0x7fffffffLL)
+  if (M < 0 || F <= 0 || K <= 0 || M > 0x7fffffffLL || F > 0x3fffffffLL || K > kGatedLongest)
     return fail(MG_ERR_INVALID, "%s: bad shape M=%lld F=%lld K=%lld", who, static_cast<long long>(M), static_cast<long long>(F),
                 static_cast<long long>(K));
   if (dtype != MG_F32 && K + 64 > kGemmDeepMaxLd)
@@ -472,6 +476,8 @@ static int gated_bwd_split(const void* dy, const void* gu, const void* x, const 
 static int gated_bwd(const char* who, const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M,
                      int64_t F, int64_t K, int dx_accumulate, int gate, int dtype, int grad_dtype, DeferredList* list, mg_stream stream) {
   MG_TRY(gated_check(who, M, F, K, gate, dtype));
+  if (std::max(M, 2 * F) > kGatedLongest)
+    return fail(MG_ERR_INVALID, "%s: bad shape M=%lld F=%lld", who, static_cast<long long>(M), static_cast<long long>(F));
   if (!is_float_dtype(grad_dtype) || (grad_dtype != dtype && grad_dtype != MG_F32))
     return fail(MG_ERR_INVALID, "%s: grad_dtype must be the tensors' dtype or float32, got %s", who, dtype_name(grad_dtype));
   if (!dw || (M > 0 && (!dy || !gu || !x || (dx && !w)))) return fail(MG_ERR_INVALID, "%s: null pointer argument", who);

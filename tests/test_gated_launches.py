@@ -99,3 +99,54 @@ out.append((chunks(1 << 25, 2051) + chunks(129, 2051), sum(l[0] for l in launche
     assert len(got) == 5
     for least, given in got:
         assert least >= 1 << 24 and least <= given <= least + 1
+
+
+def test_sizes_that_a_walk_cannot_count_are_refused(over_stub):
+    """Ranges of a walk end on whole steps, past 2^31 where the walk is that long: K of the forward, M and 2 F of the gradients."""
+    got = over_stub(CALLS + """
+def status(call, *args, **kw):
+    try:
+        call(*args, **kw)
+        return 0
+    except MogradError as e:
+        return e.status
+
+most = 0x7fff0000
+for dtype in (F32, BF16):
+    for dx, db in ((True, True), (False, False)):
+        for extra, want in ((0, 0), (1, 1)):
+            out.append((status(backward, most + extra, 1, 1, dtype, dx=False, db=db), want))
+            out.append((status(backward, 1, most // 2 + extra, 1, dtype, dx=dx, db=False), want if extra else None))
+    out.append((status(backward, (1 << 31) - 1, 1, 1, dtype, dx=False), 1))
+for M, F in ((1, 1), (4, 2), (17, 1)):
+    out += [(status(forward, M, F, most, F32), 0), (status(forward, M, F, most + 1, F32), 1), (status(forward, M, F, (1 << 31) - 1, F32), 1)]
+out.append((status(forward, (1 << 31) - 1, 1, 17), 0))
+""")
+    for i, (status, want) in enumerate(got):
+        assert want is None or status == want, i
+
+
+def test_sizes_up_to_2_28_are_taken(over_stub):
+    """Every launch counts its threads, whatever is large, as long as the tensors are a card's."""
+    got = over_stub(CALLS + """
+import random
+rng = random.Random(3)
+near = lambda: max(1, min(1 << 28, int(2.0 ** rng.uniform(0, 28.2)) + rng.choice((0, 0, 1, -1))))
+for _ in range(6000):
+    M, F, K, dtype, odd = near(), near(), near(), rng.choice((F32, F16, BF16)), rng.random() < 0.3
+    size = 4 if dtype == F32 else 2
+    if dtype != F32:
+        K = min(K, (1 << 22) - 64)
+    if size * (M * K + 2 * F * K + 3 * M * F) > 200e9:
+        continue
+    q = p16 if odd and dtype != F32 else p
+    try:
+        forward(M, F, K, dtype, keep=rng.random() < 0.5, x=q, w=q)
+        if size * (2 * M * K + 2 * F * K + 5 * M * F) < 200e9:
+            backward(M, F, K, dtype, rng.choice((dtype, F32)), dx=rng.random() < 0.7, db=rng.random() < 0.7)
+        launches()
+        out.append(0)
+    except MogradError as e:
+        out.append((M, F, K, dtype, odd, str(e)))
+""")
+    assert len(got) > 2000 and not any(got), [g for g in got if g][:5]
