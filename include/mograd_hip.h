@@ -647,8 +647,8 @@ typedef enum mg_gate {
  * mg_gate.  Products and act in fp32, y from the projections before they are rounded.  Any address of an element, any M, F
  * and K from 1 to 2^28, 16-bit tensors: K at most 2^22 - 64.  (Above, M to 2^31 - 1, F to 2^30 - 1, K to 2^31 - 2^16, a call is taken where its
  * launches can count their workgroups, and an error elsewhere.)  Nothing overlaps.
- * fp32 products may be taken from three bf16 numbers a value, 24 bits of it: a row or weight that holds an infinity or a number past
- * 3.39e38 then gives NaN, and values below 2^-110 lose digits.  So here and in the gradients. */
+ * fp32 products may be taken from three bf16 numbers a value, 24 bits of it, as the sizes alone decide: a row or weight that holds an
+ * infinity or a number past 3.39e38 then gives NaN, and values below 2^-110 lose digits.  So here and in the gradients. */
 int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y, void* gu, int64_t M, int64_t F, int64_t K, int gate,
                         int dtype, mg_stream stream);
 
