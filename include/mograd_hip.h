@@ -656,7 +656,7 @@ int mg_gated_linear_fwd(const void* x, const void* w, const void* bias, void* y,
  *   dx(M,K) = dg Wg + du Wu     (NULL to skip; dx_accumulate != 0: added to dx)
  *   dw(2F,K) = dg^T x | du^T x
  *   db(2F)  = column sums of dg | du before they are rounded (NULL to skip).
- * act'(0) of max(g, 0) is 0.  Sizes as above, M and 2 F at most 2^31 - 2^16.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the
+ * act'(0) of max(g, 0) is 0.  (fp16: a dg or du past 65504 is infinite in dx and dw.)  Sizes as above, M and 2 F at most 2^31 - 2^16.  grad_dtype, the type of dw and db: `dtype`, or MG_F32 for the
  * unrounded fp32 sums.  M == 0: dw and db are zeros.  Nothing overlaps. */
 int mg_gated_linear_bwd(const void* dy, const void* gu, const void* x, const void* w, void* dx, void* dw, void* db, int64_t M, int64_t F,
                         int64_t K, int dx_accumulate, int gate, int dtype, int grad_dtype, mg_stream stream);

@@ -6,7 +6,7 @@
 // A matrix instruction takes 16 rows of a weight, 16 of x and 64 bytes of k of each: sixteen bytes a lane, lane l holding row l % 16
 // and bytes 16 (l / 16) on, so that a load instruction takes whole runs.  (fp32: four instructions of 4 k each, k = 4 (l / 16) + j for
 // j = 0 .. 3; both operands alike, so the order in which k is added is all that it changes.)  The next unit is on its way while one is
-// multiplied: 12 KB a wave, 8 to 16 waves a CU.  (8, 8192 <- 4096) bf16 28 us, 4.8 TB/s; in 128 x 128 tiles 40.  More waves to a
+// multiplied: 12 KB a wave, 8 to 16 waves a CU.  (8, 8192 <- 4096) bf16 29 us, 4.6 TB/s; in 128 x 128 tiles 40.  More waves to a
 // workgroup are 7 % faster there and slower for shorter rows ((10, 10336 <- 120) 3.3 us, with 8 waves 4.6).
 #pragma once
 

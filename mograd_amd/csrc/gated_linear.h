@@ -29,7 +29,7 @@ __host__ __device__ __forceinline__ void gated_with(int gate, F&& f) {
 
 // s = 1 / (1 + e^-z) and t = 1 - s, either to a few units in its own last place: from e^-|z|, which neither overflows nor leaves
 // anything to cancel.  FAST: e^z as 2^(z log2 e) with the hardware's exponential and reciprocal, |z| 2^-24 and 2^-23 off, which
-// 16 bits do not see; fp32 takes the exact ones.
+// 16 bits do not see, and 0 below 2^-126; fp32 takes the exact ones.
 template <bool FAST>
 __device__ __forceinline__ void gated_sigmoid(float z, float& s, float& t) {
   float e, r;
